@@ -1,4 +1,5 @@
-/* inferno_b200_attn.h -- C ABI of the B200 (sm_100a) causal-attention kernels.
+/* inferno_b200_attn.h -- C ABI of the B200 (sm_100a) causal-attention kernels
+ * and of the operators around attention in a transformer block.
  *
  * Drop-in boundary for the attention sub-path of K9Megahertz/Inferno.  The
  * reference has no plugin or FFI mechanism; its operator API is source level
@@ -142,6 +143,24 @@ int ib200_linear_fwd_ws(const void* x, const void* w, const void* bias, int bias
                         void* workspace, size_t workspace_bytes, ib200_stream_t stream);
 int ib200_linear_bwd_ws(const void* x, const void* w, const void* dy, void* dx, void* dw, void* db, int db_dtype,
                         int M, int K, int N, void* workspace, size_t workspace_bytes, ib200_stream_t stream);
+
+/* Layer norm over the last axis: y = (x - mean) rstd weight + bias with mean = sum(x) / C, rstd = 1 / sqrt(sum((x - mean)^2) / C + eps).
+ * x: M rows of C elements (IB200_DTYPE_*), x_pitch elements from row to row; y is dense.  weight and bias: [C] of type param_dtype,
+ * either may be NULL (ones, zeros).  mean and rstd: [M] fp32, what the backward needs; both NULL: not written.  A row is at most
+ * 32 KB (C <= 8192 fp32, 16384 bf16), longer ones are refused with IB200_ERR_UNSUPPORTED; any C and any pitch within that, rows
+ * that do not begin on 16 bytes at a lower speed.  Replaces layernorm_forward_kernel (src/inferno/cuda/cudalayernorm.cu:16-136;
+ * src/inferno/modules/layernorm.cpp:25-98). */
+int ib200_layer_norm_fwd(const void* x, int64_t x_pitch, const void* weight, const void* bias, int param_dtype, void* y, float* mean,
+                         float* rstd, int M, int C, float eps, int dtype, ib200_stream_t stream);
+
+/* dx (dense, type of x), dw and db (type param_dtype) from dy; any of the three may be NULL.  dw and db are summed in fp32 in an order
+ * that depends on M, C and the GPU alone: they repeat bit for bit.  The workspace (16-byte aligned, not initialised) is needed for dw
+ * and db; ib200_layer_norm_workspace_bytes gives its size.  Replaces layernorm_input_grad_kernel and layernorm_param_grad_kernel
+ * (src/inferno/cuda/cudalayernorm.cu:212-400). */
+size_t ib200_layer_norm_workspace_bytes(int M, int C, int dtype);
+int ib200_layer_norm_bwd(const void* x, int64_t x_pitch, const void* weight, const void* dy, int64_t dy_pitch, const float* mean,
+                         const float* rstd, void* dx, void* dw, void* db, int param_dtype, int M, int C, int dtype, void* workspace,
+                         size_t workspace_bytes, ib200_stream_t stream);
 
 /* Capacity in bytes of the scratch buffer that is compiled into the library for
  * ib200_attn_bwd_static (one copy lives in the memory of every GPU that loads the library,

@@ -23,6 +23,7 @@ EXPORTS = (
     "ib200_status_string", "ib200_last_cuda_error", "ib200_version", "ib200_attn_set_timing_events", "ib200_attn_bwd_static", "ib200_attn_fwd_strided", "ib200_attn_fwd_chunk", "ib200_attn_bwd_strided", "ib200_gemm_bf16", "ib200_linear_fwd", "ib200_linear_bwd",
     "ib200_cast_f32_to_bf16", "ib200_cast_bf16_to_f32", "ib200_attn_item_order", "ib200_attn_fwd_item_rows", "ib200_attn_check_static",
     "ib200_selftest_wait_expiry", "ib200_linear_workspace_bytes", "ib200_linear_fwd_ws", "ib200_linear_bwd_ws",
+    "ib200_layer_norm_workspace_bytes", "ib200_layer_norm_fwd", "ib200_layer_norm_bwd",
 )
 
 
@@ -76,6 +77,13 @@ def lib() -> ctypes.CDLL:
         L.ib200_cast_f32_to_bf16.restype = i
         L.ib200_cast_bf16_to_f32.argtypes = [vp, vp, sz, vp]
         L.ib200_cast_bf16_to_f32.restype = i
+        i64 = ctypes.c_int64
+        L.ib200_layer_norm_workspace_bytes.argtypes = [i, i, i]
+        L.ib200_layer_norm_workspace_bytes.restype = sz
+        L.ib200_layer_norm_fwd.argtypes = [vp, i64, vp, vp, i, vp, vp, vp, i, i, f, i, vp]
+        L.ib200_layer_norm_fwd.restype = i
+        L.ib200_layer_norm_bwd.argtypes = [vp, i64, vp, vp, i64, vp, vp, vp, vp, vp, i, i, i, i, vp, sz, vp]
+        L.ib200_layer_norm_bwd.restype = i
         ip = ctypes.POINTER(ctypes.c_int)
         L.ib200_attn_item_order.argtypes = [i, i, i, i, i, i, ip, ip, i, ip]
         L.ib200_attn_item_order.restype = i

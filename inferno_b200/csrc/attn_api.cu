@@ -14,6 +14,7 @@
 #include "attn_bwd_persist.cuh"
 #include "attn_fwd.cuh"
 #include "attn_fwd_persist.cuh"
+#include "layer_norm.cuh"
 #include "linear_gemm.cuh"
 
 namespace {
@@ -623,6 +624,55 @@ int linear_bwd_core(const void* x, const void* w, const void* dy, void* dx, void
     return launch_linear_finish(acc, dw, static_cast<long>(K) * N, part, slabs, N, have_ws ? db : nullptr, db_bf16, stream);
 }
 
+// ---- layer norm ----------------------------------------------------------------------
+constexpr int kLnMaxChunks = 4;        // 16-byte chunks of a row that a thread holds
+
+// Threads per row: as few as hold the row in four chunks each.  0: the row is too long.
+int ln_threads_per_row(int C, int dtype) {
+    const long bytes = static_cast<long>(C) * (dtype == IB200_DTYPE_F32 ? 4 : 2);
+    for (int tpr : {32, 128, 512})
+        if (bytes <= 16L * kLnMaxChunks * tpr) return tpr;
+    return 0;
+}
+int ln_bwd_blocks(int M, int C, int dtype, int sms) {
+    const int tpr = ln_threads_per_row(C, dtype), rows = tpr == 32 ? 8 : 1, per_sm = tpr == 32 ? 2 : 512 / tpr;
+    return std::min((M - 1) / rows + 1, per_sm * sms);
+}
+
+template <class S>
+int launch_ln(bool backward, const LnRows& p, int blocks, cudaStream_t stream) {
+    return backward ? launch_pdl<ln_bwd_kernel<S>>(blocks, S::THREADS, 0, stream, p)
+                    : launch_pdl<ln_fwd_kernel<S>>((p.M - 1) / S::ROWS + 1, S::THREADS, 0, stream, p);
+}
+template <class T, int TPR>
+int launch_ln_row(bool aligned, bool backward, const LnRows& p, int blocks, cudaStream_t stream) {
+    if (!aligned) return launch_ln<LnShape<T, TPR, kLnMaxChunks, false>>(backward, p, blocks, stream);
+    switch ((p.C - 1) / LnShape<T, TPR, 1, true>::CHUNK_COLS) {
+        case 0: return launch_ln<LnShape<T, TPR, 1, true>>(backward, p, blocks, stream);
+        case 1: return launch_ln<LnShape<T, TPR, 2, true>>(backward, p, blocks, stream);
+        case 2: return launch_ln<LnShape<T, TPR, 3, true>>(backward, p, blocks, stream);
+        default: return launch_ln<LnShape<T, TPR, 4, true>>(backward, p, blocks, stream);
+    }
+}
+template <class T>
+int launch_ln_type(int dtype, bool backward, const LnRows& p, int blocks, cudaStream_t stream) {
+    constexpr int kVec = 16 / sizeof(T);
+    const bool aligned = p.C % kVec == 0 && p.x_pitch % kVec == 0 && p.dy_pitch % kVec == 0 && aligned16(p.x) && aligned16(p.dy) && aligned16(p.w) &&
+                         aligned16(p.b) && aligned16(p.out);
+    switch (ln_threads_per_row(p.C, dtype)) {
+        case 32: return launch_ln_row<T, 32>(aligned, backward, p, blocks, stream);
+        case 128: return launch_ln_row<T, 128>(aligned, backward, p, blocks, stream);
+        default: return launch_ln_row<T, 512>(aligned, backward, p, blocks, stream);
+    }
+}
+
+int ln_check(const void* x, long x_pitch, int M, int C, int dtype, int param_dtype) {
+    if (!x || M <= 0 || C <= 0 || x_pitch < 0) return IB200_ERR_INVALID_ARGUMENT;
+    if ((dtype != IB200_DTYPE_F32 && dtype != IB200_DTYPE_BF16) || (param_dtype != IB200_DTYPE_F32 && param_dtype != IB200_DTYPE_BF16)) return IB200_ERR_INVALID_ARGUMENT;
+    return ln_threads_per_row(C, dtype) ? IB200_OK : IB200_ERR_UNSUPPORTED;
+}
+bool ln_whole_elements(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % (dtype == IB200_DTYPE_F32 ? 4 : 2) == 0; }
+
 int fwd_core(const void* q, const void* k, const void* v, void* o, float* lse, const ib200_layout* lq_, const ib200_layout* lk_,
              const ib200_layout* lv_, const ib200_layout* lo_, int B, int H, int T, int D, float scale, int causal, int dtype,
              int math_mode, void* workspace, size_t workspace_bytes, long cut_heads /*0: B * H*/, cudaStream_t stream) {
@@ -893,6 +943,51 @@ int ib200_linear_bwd_ws(const void* x, const void* w, const void* dy, void* dx, 
     if (db_dtype != IB200_DTYPE_F32 && db_dtype != IB200_DTYPE_BF16) return IB200_ERR_INVALID_ARGUMENT;
     if (!workspace || !aligned16(workspace) || (M > 0 && K > 0 && N > 0 && workspace_bytes < linear_bwd_ws_bytes(K, N))) return IB200_ERR_WORKSPACE;
     return linear_bwd_core(x, w, dy, dx, dw, db, db_dtype == IB200_DTYPE_BF16, M, K, N, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t ib200_layer_norm_workspace_bytes(int M, int C, int dtype) {
+    if (M <= 0 || C <= 0 || !ln_threads_per_row(C, dtype)) return 0;
+    const DeviceInfo* dev = device_info();
+    return static_cast<size_t>(ln_bwd_blocks(M, C, dtype, dev ? dev->sms : 148)) * 2 * C * 4;
+}
+
+int ib200_layer_norm_fwd(const void* x, int64_t x_pitch, const void* weight, const void* bias, int param_dtype, void* y, float* mean, float* rstd, int M, int C,
+                         float eps, int dtype, ib200_stream_t stream) {
+    int rc = ln_check(x, x_pitch, M, C, dtype, param_dtype);
+    if (rc != IB200_OK) return rc;
+    if (!y || !mean != !rstd || !(eps >= 0.f) || !isfinite(eps)) return IB200_ERR_INVALID_ARGUMENT;
+    if (!ln_whole_elements(x, dtype) || !ln_whole_elements(y, dtype) || !ln_whole_elements(weight, param_dtype) || !ln_whole_elements(bias, param_dtype) ||
+        !ln_whole_elements(mean, IB200_DTYPE_F32) || !ln_whole_elements(rstd, IB200_DTYPE_F32))
+        return IB200_ERR_MISALIGNED;
+    if ((rc = device_ok()) != IB200_OK) return rc;
+    const LnRows p{x, static_cast<long>(x_pitch), nullptr, 0, weight, bias, param_dtype == IB200_DTYPE_BF16, y, mean, rstd, nullptr, M, C, eps};
+    return dtype == IB200_DTYPE_F32 ? launch_ln_type<float>(dtype, false, p, 0, reinterpret_cast<cudaStream_t>(stream))
+                                    : launch_ln_type<__nv_bfloat16>(dtype, false, p, 0, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int ib200_layer_norm_bwd(const void* x, int64_t x_pitch, const void* weight, const void* dy, int64_t dy_pitch, const float* mean, const float* rstd, void* dx,
+                         void* dw, void* db, int param_dtype, int M, int C, int dtype, void* workspace, size_t workspace_bytes, ib200_stream_t stream_) {
+    cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+    int rc = ln_check(x, x_pitch, M, C, dtype, param_dtype);
+    if (rc != IB200_OK) return rc;
+    if (!dy || dy_pitch < 0 || !mean || !rstd) return IB200_ERR_INVALID_ARGUMENT;
+    if (!dx && !dw && !db) return IB200_OK;
+    if (!ln_whole_elements(x, dtype) || !ln_whole_elements(dy, dtype) || !ln_whole_elements(dx, dtype) || !ln_whole_elements(weight, param_dtype) ||
+        !ln_whole_elements(dw, param_dtype) || !ln_whole_elements(db, param_dtype) || !ln_whole_elements(mean, IB200_DTYPE_F32) ||
+        !ln_whole_elements(rstd, IB200_DTYPE_F32))
+        return IB200_ERR_MISALIGNED;
+    const bool params = dw || db;
+    if (params && (!workspace || !aligned16(workspace) || workspace_bytes < ib200_layer_norm_workspace_bytes(M, C, dtype))) return IB200_ERR_WORKSPACE;
+    const DeviceInfo* dev = device_info();
+    if (!dev) return IB200_ERR_NO_DEVICE;
+    const int blocks = ln_bwd_blocks(M, C, dtype, dev->sms);
+    float* part = params ? static_cast<float*>(workspace) : nullptr;
+    const LnRows p{x, static_cast<long>(x_pitch), dy, static_cast<long>(dy_pitch), weight, nullptr, param_dtype == IB200_DTYPE_BF16, dx, const_cast<float*>(mean),
+                   const_cast<float*>(rstd), part, M, C, 0.f};
+    rc = dtype == IB200_DTYPE_F32 ? launch_ln_type<float>(dtype, true, p, blocks, stream) : launch_ln_type<__nv_bfloat16>(dtype, true, p, blocks, stream);
+    if (rc != IB200_OK || !params) return rc;
+    return launch_pdl<ln_finish_kernel>(dim3((C + kLnFinishCols - 1) / kLnFinishCols, 2), 256, 0, stream, part, blocks, C, dw, db,
+                                        static_cast<int>(param_dtype == IB200_DTYPE_BF16));
 }
 
 static int read_and_clear_status(void* header, cudaStream_t stream, int* device_code) {

@@ -52,6 +52,9 @@ struct Abi {
     decltype(&ib200_linear_workspace_bytes) linear_workspace_bytes = nullptr;
     decltype(&ib200_linear_fwd_ws) linear_fwd = nullptr;
     decltype(&ib200_linear_bwd_ws) linear_bwd = nullptr;
+    decltype(&ib200_layer_norm_workspace_bytes) layer_norm_workspace_bytes = nullptr;
+    decltype(&ib200_layer_norm_fwd) layer_norm_fwd = nullptr;
+    decltype(&ib200_layer_norm_bwd) layer_norm_bwd = nullptr;
     decltype(&ib200_attn_set_timing_events) set_timing_events = nullptr;
     decltype(&ib200_status_string) status_string = nullptr;
     PyObject* error_class = nullptr;      // the package's exception type, constructed from (status, where)
@@ -98,7 +101,7 @@ Tensor empty_bytes(size_t bytes, c10::Device device) { return at::empty({static_
 void reserve(Tensor& buf, size_t bytes, c10::Device device) {
     if (!buf.defined() || static_cast<size_t>(buf.numel()) < bytes) buf = empty_bytes(bytes, device);
 }
-// A projection's scratch.  While the stream is being captured it comes from the graph's own memory, and goes back there after the
+// The scratch of a projection or a layer norm.  While the stream is being captured it comes from the graph's own memory, and goes back there after the
 // call: the graph then depends on nothing that a later call could replace.
 Tensor linear_scratch(Workspace& ws, size_t bytes, c10::Device device) {
     if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return empty_bytes(bytes, device);
@@ -567,6 +570,159 @@ Tensor linear(const Tensor& x, const Tensor& w, const Tensor& bias) {
     return y;
 }
 
+// ---- layer norm ----------------------------------------------------------------------
+int type_code(const Tensor& t, const char* op, const char* name) {
+    TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16, op, ": ", name, " must be float32 or bfloat16");
+    return dtype_code(t);
+}
+// Shapes first, as for the projections.
+void check_layer_norm(const Tensor& x, const Tensor& weight, const Tensor& bias) {
+    TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0, "layer_norm: x needs a last axis to normalise, x is ", x.sizes());
+    const int64_t C = x.size(-1);
+    TORCH_CHECK_VALUE(x.numel() / C <= 0x7fffffff && C <= 0x7fffffff, "layer_norm: too many rows or columns, x is ", x.sizes());
+    for (const Tensor* p : {&weight, &bias})
+        TORCH_CHECK_VALUE(!p->defined() || (p->dim() == 1 && p->size(0) == C), "layer_norm: weight and bias must be [", C, "] like the last axis of x");
+    TORCH_CHECK(x.is_cuda(), "layer_norm: x is not on a CUDA device (there is no CPU path)");
+    type_code(x, "layer_norm", "x");
+    for (const Tensor* p : {&weight, &bias}) {
+        if (!p->defined()) continue;
+        type_code(*p, "layer_norm", "weight and bias");
+        TORCH_CHECK_VALUE(p->device() == x.device(), "layer_norm: weight and bias must be on x's device");
+    }
+    TORCH_CHECK_TYPE(!weight.defined() || !bias.defined() || weight.scalar_type() == bias.scalar_type(), "layer_norm: weight and bias must have the same dtype");
+}
+// The rows of a [..., C] tensor one pitch apart: in place where its axes allow it, otherwise a dense copy.
+struct RowView {
+    Tensor t;
+    int64_t pitch;
+};
+RowView row_view(const Tensor& t) {
+    const int64_t C = t.size(-1);
+    if (t.numel() == 0) return {t, C};
+    bool ok = C == 1 || t.stride(-1) == 1;
+    int64_t pitch = C, span = 0;      // span: elements from one index of the axis above to the next, if the rows go on evenly
+    for (int64_t a = t.dim() - 2; ok && a >= 0; --a) {
+        if (t.size(a) == 1) continue;
+        if (span == 0) pitch = t.stride(a);
+        else ok = t.stride(a) == span;
+        span = t.stride(a) * t.size(a);
+        if (span == 0) ok = false;    // a broadcast axis: copied
+    }
+    if (ok) return {t, pitch};
+    return {t.contiguous(), C};
+}
+
+struct Norm {
+    Tensor y, mean, rstd;
+};
+Norm layer_norm_forward(const Tensor& x_, const Tensor& weight_, const Tensor& bias_, double eps, bool stats) {
+    check_layer_norm(x_, weight_, bias_);
+    TORCH_CHECK_VALUE(eps >= 0 && std::isfinite(eps), "layer_norm: eps must be finite and not negative, got ", eps);
+    const c10::cuda::CUDAGuard guard(x_.device());
+    const int64_t C = x_.size(-1);
+    const RowView x = row_view(x_);
+    const Tensor w = weight_.defined() ? weight_.contiguous() : weight_, b = bias_.defined() ? bias_.contiguous() : bias_;
+    const int param = w.defined() ? dtype_code(w) : b.defined() ? dtype_code(b) : IB200_DTYPE_F32;
+    Norm r;
+    r.y = at::empty(x_.sizes(), x_.options());
+    if (stats) {
+        auto shape = x_.sizes().vec();
+        shape.pop_back();
+        r.mean = at::empty(shape, x_.options().dtype(at::kFloat));
+        r.rstd = at::empty(shape, x_.options().dtype(at::kFloat));
+    }
+    if (x_.numel() == 0) return r;
+    auto ptr = [](const Tensor& t) -> void* { return t.defined() ? t.data_ptr() : nullptr; };
+    cudaStream_t stream = c10::cuda::getCurrentCUDAStream(x_.device().index()).stream();
+    check_status(g_abi.layer_norm_fwd(x.t.data_ptr(), x.pitch, ptr(w), ptr(b), param, r.y.data_ptr(), static_cast<float*>(ptr(r.mean)),
+                                      static_cast<float*>(ptr(r.rstd)), static_cast<int>(x_.numel() / C), static_cast<int>(C), static_cast<float>(eps), dtype_code(x_),
+                                      reinterpret_cast<ib200_stream_t>(stream)),
+                 "ib200_layer_norm_fwd");
+    return r;
+}
+
+struct NormGrads {
+    Tensor dx, dw, db;
+};
+// dw and db have the type of `weight` (without one: `param_type`).
+NormGrads layer_norm_backward(const Tensor& x_, const Tensor& dy_, const Tensor& mean_, const Tensor& rstd_, const Tensor& weight_, bool need_dx, bool need_dw,
+                              bool need_db, at::ScalarType param_type) {
+    check_layer_norm(x_, weight_, Tensor());
+    const int64_t C = x_.size(-1), M = x_.numel() / C;
+    TORCH_CHECK_VALUE(dy_.sizes() == x_.sizes() && dy_.device() == x_.device(), "layer_norm: dy must have x's shape and device, dy is ", dy_.sizes(), ", x is ",
+                      x_.sizes());
+    TORCH_CHECK_TYPE(dy_.scalar_type() == x_.scalar_type(), "layer_norm: dy must have x's dtype");
+    for (const Tensor* t : {&mean_, &rstd_})
+        TORCH_CHECK_VALUE(t->numel() == M && t->scalar_type() == at::kFloat && t->device() == x_.device(),
+                          "layer_norm: mean and rstd must be float32, one value per row of x, on its device");
+    const c10::cuda::CUDAGuard guard(x_.device());
+    const RowView x = row_view(x_), dy = row_view(dy_);
+    const Tensor mean = mean_.contiguous(), rstd = rstd_.contiguous(), w = weight_.defined() ? weight_.contiguous() : weight_;
+    if (w.defined()) param_type = w.scalar_type();
+    NormGrads g;
+    if (need_dx) g.dx = at::empty(x_.sizes(), x_.options());
+    const auto param = x_.options().dtype(param_type);
+    if (need_dw) g.dw = M ? at::empty({C}, param) : at::zeros({C}, param);
+    if (need_db) g.db = M ? at::empty({C}, param) : at::zeros({C}, param);
+    if (M == 0 || (!need_dx && !need_dw && !need_db)) return g;
+    auto ptr = [](const Tensor& t) -> void* { return t.defined() ? t.data_ptr() : nullptr; };
+    const int m = static_cast<int>(M), c = static_cast<int>(C), dtype = dtype_code(x_);
+    const size_t bytes = need_dw || need_db ? g_abi.layer_norm_workspace_bytes(m, c, dtype) : 0;
+    cudaStream_t stream = c10::cuda::getCurrentCUDAStream(x_.device().index()).stream();
+    Workspace& ws = workspace_of(x_.device().index(), stream);
+    std::lock_guard<std::mutex> lock(ws.launching);
+    const Tensor scratch = bytes ? linear_scratch(ws, bytes, x_.device()) : Tensor();
+    check_status(g_abi.layer_norm_bwd(x.t.data_ptr(), x.pitch, ptr(w), dy.t.data_ptr(), dy.pitch, mean.data_ptr<float>(), rstd.data_ptr<float>(), ptr(g.dx), ptr(g.dw),
+                                      ptr(g.db), param_type == at::kBFloat16 ? IB200_DTYPE_BF16 : IB200_DTYPE_F32, m, c, dtype, ptr(scratch), bytes,
+                                      reinterpret_cast<ib200_stream_t>(stream)),
+                 "ib200_layer_norm_bwd");
+    return g;
+}
+
+struct LayerNormBackward : torch::autograd::Node {
+    SavedVariable x, weight, mean, rstd;
+    bool has_weight = false;
+    at::ScalarType param_type = at::kFloat;
+
+    variable_list apply(variable_list&& grads) override {
+        return in_node([&] { return backward(grads); });
+    }
+    variable_list backward(const variable_list& grads) {
+        if (!grads[0].defined()) return variable_list(3);
+        const Tensor tx = x.unpack(), tw = has_weight ? weight.unpack() : Tensor(), tm = mean.unpack(), tr = rstd.unpack();
+        at::AutoDispatchBelowADInplaceOrView below;
+        const NormGrads g = layer_norm_backward(tx, grads[0], tm, tr, tw, task_should_compute_output(0), task_should_compute_output(1),
+                                                task_should_compute_output(2), param_type);
+        return {g.dx, g.dw, g.db};
+    }
+    void release_variables() override {
+        x.reset_data(); weight.reset_data(); mean.reset_data(); rstd.reset_data();
+    }
+    std::string name() const override { return "LayerNormBackward"; }
+};
+
+Tensor layer_norm(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps) {
+    refuse_tangents({&x, &weight, &bias}, "layer_norm");
+    const bool differentiable = torch::autograd::compute_requires_grad(x, weight, bias);
+    Norm r;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        r = layer_norm_forward(x, weight, bias, eps, differentiable);
+    }
+    if (differentiable) {
+        auto node = std::shared_ptr<LayerNormBackward>(new LayerNormBackward(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(x, weight, bias));
+        node->x = SavedVariable(x, false);
+        node->mean = SavedVariable(r.mean, false);
+        node->rstd = SavedVariable(r.rstd, false);
+        node->has_weight = weight.defined();
+        if (weight.defined()) node->weight = SavedVariable(weight, false);
+        if (bias.defined()) node->param_type = bias.scalar_type();
+        torch::autograd::set_history(r.y, node);
+    }
+    return r.y;
+}
+
 // ---- Python boundary ---------------------------------------------------------------
 // Plain METH_FASTCALL functions: positional arguments, None for an absent tensor or the default scale.
 const Tensor& arg_tensor(PyObject* o) {
@@ -574,11 +730,14 @@ const Tensor& arg_tensor(PyObject* o) {
     return THPVariable_Unpack(o);
 }
 Tensor arg_opt_tensor(PyObject* o) { return o == Py_None ? Tensor() : arg_tensor(o); }
-std::optional<double> arg_scale(PyObject* o) {
-    if (o == Py_None) return std::nullopt;
+double arg_double(PyObject* o) {
     const double d = PyFloat_AsDouble(o);
     if (d == -1.0 && PyErr_Occurred()) throw python_error();
     return d;
+}
+std::optional<double> arg_scale(PyObject* o) {
+    if (o == Py_None) return std::nullopt;
+    return arg_double(o);
 }
 int64_t arg_int(PyObject* o) {
     const long long v = PyLong_AsLongLong(o);
@@ -642,6 +801,9 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
         get(g_abi.linear_workspace_bytes, "ib200_linear_workspace_bytes");
         get(g_abi.linear_fwd, "ib200_linear_fwd_ws");
         get(g_abi.linear_bwd, "ib200_linear_bwd_ws");
+        get(g_abi.layer_norm_workspace_bytes, "ib200_layer_norm_workspace_bytes");
+        get(g_abi.layer_norm_fwd, "ib200_layer_norm_fwd");
+        get(g_abi.layer_norm_bwd, "ib200_layer_norm_bwd");
         get(g_abi.set_timing_events, "ib200_attn_set_timing_events");
         get(g_abi.status_string, "ib200_status_string");
         Py_INCREF(a[1]);
@@ -771,6 +933,54 @@ PyObject* py_linear_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// (x, weight, bias, eps) -> y, differentiable
+PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        want(n, 4);
+        const Tensor& x = arg_tensor(a[0]);
+        const Tensor weight = arg_opt_tensor(a[1]), bias = arg_opt_tensor(a[2]);
+        const double eps = arg_double(a[3]);
+        Tensor y;
+        {
+            pybind11::gil_scoped_release nogil;
+            y = layer_norm(x, weight, bias, eps);
+        }
+        return wrap(y);
+    });
+}
+// (x, weight, bias, eps) -> (y, mean, rstd)
+PyObject* py_layer_norm_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        want(n, 4);
+        const Tensor& x = arg_tensor(a[0]);
+        const Tensor weight = arg_opt_tensor(a[1]), bias = arg_opt_tensor(a[2]);
+        const double eps = arg_double(a[3]);
+        Norm r;
+        {
+            pybind11::gil_scoped_release nogil;
+            at::AutoDispatchBelowADInplaceOrView below;
+            r = layer_norm_forward(x, weight, bias, eps, true);
+        }
+        return wrap_tuple({&r.y, &r.mean, &r.rstd});
+    });
+}
+// (x, dy, mean, rstd, weight, need_dx, need_dw, need_db) -> (dx, dw, db)
+PyObject* py_layer_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        want(n, 8);
+        const Tensor &x = arg_tensor(a[0]), &dy = arg_tensor(a[1]), &mean = arg_tensor(a[2]), &rstd = arg_tensor(a[3]);
+        const Tensor weight = arg_opt_tensor(a[4]);
+        const bool need_dx = arg_bool(a[5]), need_dw = arg_bool(a[6]), need_db = arg_bool(a[7]);
+        NormGrads g;
+        {
+            pybind11::gil_scoped_release nogil;
+            at::AutoDispatchBelowADInplaceOrView below;
+            g = layer_norm_backward(x, dy, mean, rstd, weight, need_dx, need_dw, need_db, at::kFloat);
+        }
+        return wrap_tuple({&g.dx, &g.dw, &g.db});
+    });
+}
+
 // () -> {(device index, stream handle): workspace tensor}
 PyObject* py_workspaces(PyObject*, PyObject* const*, Py_ssize_t) {
     return guarded([&]() -> PyObject* {
@@ -834,6 +1044,9 @@ PyMethodDef g_methods[] = {IB200_PY(bind),
                            IB200_PY(linear),
                            IB200_PY(linear_forward),
                            IB200_PY(linear_backward),
+                           IB200_PY(layer_norm),
+                           IB200_PY(layer_norm_forward),
+                           IB200_PY(layer_norm_backward),
                            IB200_PY(workspaces),
                            IB200_PY(queue_timing_events),
                            {nullptr, nullptr, 0, nullptr}};
