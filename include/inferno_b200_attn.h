@@ -116,7 +116,7 @@ int ib200_attn_bwd_strided(const void* q, const void* k, const void* v, const vo
 /* The projections either side of attention.  C[M,N] = A[M,K] B[K,N] (+ bias[N]), bf16 operands and output, fp32
  * accumulation on the tensor cores, fp32 bias.  a_transposed = 0: A stored [M rows, K contiguous]; 1: stored
  * [K rows, M contiguous].  b_transposed = 0: B stored [K rows, N contiguous]; 1: stored [N rows, K contiguous].
- * M, N, K multiples of 8; bases 16-byte aligned.  Replaces cublas_mm_row_major + the broadcast add of the reference's
+ * Rows as stored are multiples of 8 elements: N, and K (M where A is stored transposed); bases 16-byte aligned.  Replaces cublas_mm_row_major + the broadcast add of the reference's
  * Linear::forward (src/inferno/modules/linear.cpp:99-106, src/inferno/cuda/cudamatmul.cu:1058-1112,
  * src/inferno/cuda/cudaadd.cu:20-142); a transposed operand costs a descriptor, not the copy the reference makes
  * (src/inferno/gradfn/mmbackward.cpp:77-80).  An expired device-side wait of these kernels is recorded in the status
@@ -143,6 +143,33 @@ int ib200_linear_fwd_ws(const void* x, const void* w, const void* bias, int bias
                         void* workspace, size_t workspace_bytes, ib200_stream_t stream);
 int ib200_linear_bwd_ws(const void* x, const void* w, const void* dy, void* dx, void* dw, void* db, int db_dtype,
                         int M, int K, int N, void* workspace, size_t workspace_bytes, ib200_stream_t stream);
+
+/* y[M,N] = act(x[M,K] w[K,N] + bias[N]) + residual[M,N], all but the product in its epilogue.  activation IB200_ACT_GELU is the reference's
+ * tanh form, gelu(z) = z / (1 + exp(-2u)) with u = sqrt(2 / pi) (z + 0.044715 z^3).  bias (of type bias_dtype) and residual (bf16, dense) may be
+ * NULL.  preact: if not NULL (activation GELU only), z = x w + bias is kept there for the backward as fp16, [M, N], limited to +-16,
+ * beyond which gelu' is 0 or 1.  K and N multiples of 8, any M; bases 16-byte aligned.  The workspace is used by products that are cut along K
+ * (ib200_fused_linear_workspace_bytes, 0: none); without one they are not cut.  y and preact must not overlap the operands, y not preact.
+ * Replaces Linear::forward, the gelu op and the residual addition behind them (src/inferno/modules/linear.cpp:99-106,
+ * src/inferno/cuda/cudagelu.cu:40-66, src/inferno/cuda/cudaadd.cu:20-142). */
+enum { IB200_ACT_NONE = 0, IB200_ACT_GELU = 1 };
+size_t ib200_fused_linear_workspace_bytes(int M, int K, int N, int activation, int pass);
+int ib200_fused_linear_fwd(const void* x, const void* w, const void* bias, int bias_dtype, const void* residual, int activation,
+                           void* y, void* preact, int M, int K, int N, void* workspace, size_t workspace_bytes, ib200_stream_t stream);
+
+/* Its backward: dz = dy gelu'(preact) (activation GELU; dz = dy without one, preact NULL), dx = dz w^T, dw = x^T dz, db = column sums of dz (of
+ * type db_dtype); any of dx / dw / db may be NULL.  The gradient of the residual is dy itself.  The workspace is always needed.  dw is
+ * added up as in ib200_linear_bwd_ws; dx and db repeat bit for bit.  Replaces MMBackward and GeluBackward
+ * (src/inferno/gradfn/mmbackward.cpp:36-98; kernel src/inferno/cuda/cudagelu.cu:138-202). */
+int ib200_fused_linear_bwd(const void* x, const void* w, const void* dy, const void* preact, int activation, void* dx, void* dw,
+                           void* db, int db_dtype, int M, int K, int N, void* workspace, size_t workspace_bytes, ib200_stream_t stream);
+
+/* Backward of the feed-forward block y[M,C] = h w2 + b2 (+ residual), h = gelu(x[M,C] w1[C,H] + b1): two ib200_fused_linear_fwd calls, which leave
+ * preact (fp16) and h [M,H].  dz = (dy w2^T) gelu'(preact) is formed in the epilogue of that product and its columns are summed there (db1), dw2 =
+ * h^T dy, db2 = column sums of dy, dx = dz w1^T, dw1 = x^T dz; any output may be NULL.  C and H multiples of 8, any M. */
+size_t ib200_feed_forward_workspace_bytes(int M, int C, int H);
+int ib200_feed_forward_bwd(const void* x, const void* w1, const void* preact, const void* h, const void* w2, const void* dy, void* dx,
+                           void* dw1, void* db1, int db1_dtype, void* dw2, void* db2, int db2_dtype, int M, int C, int H,
+                           void* workspace, size_t workspace_bytes, ib200_stream_t stream);
 
 /* Layer norm over the last axis: y = (x - mean) rstd weight + bias with mean = sum(x) / C, rstd = 1 / sqrt(sum((x - mean)^2) / C + eps).
  * x: M rows of C elements (IB200_DTYPE_*), x_pitch elements from row to row; y is dense.  weight and bias: [C] of type param_dtype,

@@ -17,13 +17,15 @@ STATIC_SCRATCH_BYTES = 32 * 1024 * 1024
 DTYPE_F32, DTYPE_BF16 = 0, 1
 MATH_SPLIT_BF16 = 0
 PASS_FWD, PASS_BWD = 0, 1
+ACT_NONE, ACT_GELU = 0, 1
 
 EXPORTS = (
     "ib200_attn_workspace_bytes", "ib200_attn_fwd", "ib200_attn_bwd", "ib200_attn_check",
     "ib200_status_string", "ib200_last_cuda_error", "ib200_version", "ib200_attn_set_timing_events", "ib200_attn_bwd_static", "ib200_attn_fwd_strided", "ib200_attn_fwd_chunk", "ib200_attn_bwd_strided", "ib200_gemm_bf16", "ib200_linear_fwd", "ib200_linear_bwd",
     "ib200_cast_f32_to_bf16", "ib200_cast_bf16_to_f32", "ib200_attn_item_order", "ib200_attn_fwd_item_rows", "ib200_attn_check_static",
     "ib200_selftest_wait_expiry", "ib200_linear_workspace_bytes", "ib200_linear_fwd_ws", "ib200_linear_bwd_ws",
-    "ib200_layer_norm_workspace_bytes", "ib200_layer_norm_fwd", "ib200_layer_norm_bwd",
+    "ib200_fused_linear_workspace_bytes", "ib200_fused_linear_fwd", "ib200_fused_linear_bwd",
+    "ib200_feed_forward_workspace_bytes", "ib200_feed_forward_bwd", "ib200_layer_norm_workspace_bytes", "ib200_layer_norm_fwd", "ib200_layer_norm_bwd",
 )
 
 
@@ -78,6 +80,16 @@ def lib() -> ctypes.CDLL:
         L.ib200_cast_bf16_to_f32.argtypes = [vp, vp, sz, vp]
         L.ib200_cast_bf16_to_f32.restype = i
         i64 = ctypes.c_int64
+        L.ib200_fused_linear_workspace_bytes.argtypes = [i, i, i, i, i]
+        L.ib200_fused_linear_workspace_bytes.restype = sz
+        L.ib200_fused_linear_fwd.argtypes = [vp, vp, vp, i, vp, i, vp, vp, i, i, i, vp, sz, vp]
+        L.ib200_fused_linear_fwd.restype = i
+        L.ib200_fused_linear_bwd.argtypes = [vp, vp, vp, vp, i, vp, vp, vp, i, i, i, i, vp, sz, vp]
+        L.ib200_fused_linear_bwd.restype = i
+        L.ib200_feed_forward_workspace_bytes.argtypes = [i, i, i]
+        L.ib200_feed_forward_workspace_bytes.restype = sz
+        L.ib200_feed_forward_bwd.argtypes = [vp] * 9 + [i, vp, vp, i, i, i, i, vp, sz, vp]
+        L.ib200_feed_forward_bwd.restype = i
         L.ib200_layer_norm_workspace_bytes.argtypes = [i, i, i]
         L.ib200_layer_norm_workspace_bytes.restype = sz
         L.ib200_layer_norm_fwd.argtypes = [vp, i64, vp, vp, i, vp, vp, vp, i, i, f, i, vp]

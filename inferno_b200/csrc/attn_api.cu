@@ -484,11 +484,25 @@ bool gemm_wants_split(const GemmDesc& d, int pairs) { return d.tiles() * 2 <= pa
 // Next to other tiles (dX) a product with no more tiles than two rounds is cut as well: its slices then even out the load.
 bool gemm_wants_split_beside(const GemmDesc& d, int pairs) { return d.tiles() <= 2 * pairs && d.k_slices() >= 2 * kMinPartSlices; }
 
+// A fused epilogue of the `whole` product (kEpi*): what it reads beside its accumulator, and what it writes beside c.
+struct GemmEpi {
+    int mode = kEpiBias;
+    const void* aux = nullptr;      // residual (bf16) or z (fp16), [M, N]
+    void* pre = nullptr;            // z, fp16 [M, N]
+    float* colsum = nullptr;        // [ceil(M / 32)][N]
+};
+template <int EPI>
+int launch_gemm_form(int pairs, const GemmMaps& maps, const GemmParams& p, cudaStream_t stream) {
+    if (!allow_smem<gemm_bf16_kernel<EPI>>(GemmSmem<EPI>::BYTES)) return IB200_ERR_CUDA;
+    return launch_pdl<gemm_bf16_kernel<EPI>>(2 * pairs, GemmTraits::THREADS, GemmSmem<EPI>::BYTES, stream, maps, p);
+}
+
 // One launch: `whole` cut into whole tiles (may be null), `other` cut into whole tiles or, with split != kPartWhole, along K.
-int launch_gemms(const GemmDesc* whole, const GemmDesc* other, int split, float* acc, const void* bias, int bias_bf16, cudaStream_t stream) {
+int launch_gemms(const GemmDesc* whole, const GemmDesc* other, int split, float* acc, const void* bias, int bias_bf16, cudaStream_t stream,
+                 const GemmEpi& epi = GemmEpi()) {
     using TR = GemmTraits;
     const DeviceInfo* dev = device_info();
-    if (!dev || !allow_smem<gemm_bf16_kernel>(TR::SMEM_BYTES)) return IB200_ERR_CUDA;
+    if (!dev) return IB200_ERR_CUDA;
     const int max_pairs = dev->sms / 2;
     GemmMaps maps;
     GemmParams p{};
@@ -497,6 +511,11 @@ int launch_gemms(const GemmDesc* whole, const GemmDesc* other, int split, float*
     if (!other) { maps.a[1] = maps.a[0]; maps.b[1] = maps.b[0]; maps.c[1] = maps.c[0]; }
     maps.sum = maps.c[1];
     if (split == kPartReduceF32 && !make_tmap_2d(&maps.sum, acc, other->M, other->N, 32, true)) return IB200_ERR_CUDA;
+    maps.aux = maps.pre = maps.c[0];
+    if ((epi.aux && !make_tmap_2d(&maps.aux, epi.aux, whole->M, whole->N, 32)) || (epi.pre && !make_tmap_2d(&maps.pre, epi.pre, whole->M, whole->N, 32))) return IB200_ERR_CUDA;
+    p.has_aux = epi.aux != nullptr;
+    p.write_pre = epi.pre != nullptr;
+    p.colsum = epi.colsum;
     p.split = split;
     p.bias = bias;
     p.bias_bf16 = bias_bf16;
@@ -535,25 +554,36 @@ int launch_gemms(const GemmDesc* whole, const GemmDesc* other, int split, float*
     void* builtin = nullptr;
     p.status = static_scratch(&builtin) == IB200_OK ? static_cast<int*>(builtin) : nullptr;
     IB200_SET_BOUNDS(0, 0, 0, 0, 0, 1, TR::TM_COLS, p.status, stream);
-    return launch_pdl<gemm_bf16_kernel>(2 * pairs, TR::THREADS, TR::SMEM_BYTES, stream, maps, p);
+    switch (epi.mode) {
+        case kEpiResidual: return launch_gemm_form<kEpiResidual>(pairs, maps, p, stream);
+        case kEpiGelu: return launch_gemm_form<kEpiGelu>(pairs, maps, p, stream);
+        case kEpiSlope: return launch_gemm_form<kEpiSlope>(pairs, maps, p, stream);
+        default: return launch_gemm_form<kEpiBias>(pairs, maps, p, stream);
+    }
 }
 
 int gemm_check(const GemmDesc& d) {
     if (!d.a || !d.b || !d.c) return IB200_ERR_INVALID_ARGUMENT;
     if (d.M <= 0 || d.N <= 0 || d.K <= 0 || (d.a_mn != 0 && d.a_mn != 1) || (d.b_mn != 0 && d.b_mn != 1)) return IB200_ERR_INVALID_ARGUMENT;
-    if (d.M % 8 || d.N % 8 || d.K % 8) return IB200_ERR_UNSUPPORTED;
+    // a row of each matrix, as it is stored, is a whole number of 16-byte units
+    if ((d.a_mn ? d.M : d.K) % 8 || (d.b_mn ? d.N : d.K) % 8 || d.N % 8) return IB200_ERR_UNSUPPORTED;
     if (!aligned16(d.a) || !aligned16(d.b) || !aligned16(d.c)) return IB200_ERR_MISALIGNED;
     return device_ok();
 }
 
-int launch_linear_finish(const float* acc, void* out, long n, const float* part, int slabs, int N, void* db, int db_bf16, cudaStream_t stream) {
-    const long n8 = n / 8;
-    const int db_blocks = db ? (N + kFinishCols - 1) / kFinishCols : 0;
-    long blocks = acc ? std::min<long>((n8 + 255) / 256, 148 * 8) : 0;
-    if (blocks + db_blocks == 0) return IB200_OK;
-    return launch_pdl<linear_finish_kernel>(static_cast<int>(blocks) + db_blocks, 256, 0, stream, reinterpret_cast<const float4*>(acc), static_cast<uint4*>(out), n8,
-                                            part, slabs, N, db, db_bf16, db_blocks);
+FinishJob finish_job(const float* acc, void* out, long n, const float* part, int slabs, int N, void* db, int db_bf16) {
+    return FinishJob{reinterpret_cast<const float4*>(acc), static_cast<uint4*>(out), n / 8, part, slabs, N, db, db_bf16, db ? (N + kFinishCols - 1) / kFinishCols : 0};
 }
+int launch_linear_finish(const FinishJob& one, const FinishJob& two, cudaStream_t stream) {
+    const long n8 = std::max(one.acc ? one.n8 : 0, two.acc ? two.n8 : 0);
+    const long blocks = std::min<long>((n8 + 255) / 256, 148 * 8) + one.db_blocks + two.db_blocks;
+    if (blocks == 0) return IB200_OK;
+    FinishJobs jobs;
+    jobs.j[0] = one;
+    jobs.j[1] = two;
+    return launch_pdl<linear_finish_kernel>(static_cast<int>(blocks), 256, 0, stream, jobs);
+}
+int launch_linear_finish(const FinishJob& one, cudaStream_t stream) { return launch_linear_finish(one, FinishJob{}, stream); }
 
 // One product.  With a workspace of at least M * N floats a split product is added up in fp32.
 int gemm_single(const GemmDesc& d, const void* bias, int bias_bf16, void* ws, size_t ws_bytes, cudaStream_t stream) {
@@ -570,7 +600,33 @@ int gemm_single(const GemmDesc& d, const void* bias, int bias_bf16, void* ws, si
     }
     if (!cuda_ok(cudaMemsetAsync(ws, 0, n * 4, stream))) return IB200_ERR_CUDA;
     if ((rc = launch_gemms(nullptr, &d, kPartReduceF32, static_cast<float*>(ws), bias, bias_bf16, stream))) return rc;
-    return launch_linear_finish(static_cast<const float*>(ws), d.c, static_cast<long>(n), nullptr, 0, 0, nullptr, 0, stream);
+    return launch_linear_finish(finish_job(static_cast<const float*>(ws), d.c, static_cast<long>(n), nullptr, 0, 0, nullptr, 0), stream);
+}
+
+bool valid_dtype(int dtype) { return dtype == IB200_DTYPE_F32 || dtype == IB200_DTYPE_BF16; }
+
+// y = act(x w + bias) + residual.
+int fused_linear_fwd_core(const GemmDesc& d, const void* bias, int bias_bf16, const void* residual, void* pre, bool gelu, void* ws, size_t ws_bytes,
+                          cudaStream_t stream) {
+    if (!gelu && !residual) return gemm_single(d, bias, bias_bf16, ws, ws_bytes, stream);
+    if (!aligned16(bias) || !aligned16(residual) || !aligned16(pre)) return IB200_ERR_MISALIGNED;
+    int rc = gemm_check(d);
+    if (rc != IB200_OK) return rc;
+    const DeviceInfo* dev = device_info();
+    if (!dev) return IB200_ERR_CUDA;
+    const size_t n = static_cast<size_t>(d.M) * d.N;
+    if (gemm_wants_split(d, dev->sms / 2) && ws && ws_bytes >= n * 4) {
+        if (!cuda_ok(cudaMemsetAsync(ws, 0, n * 4, stream))) return IB200_ERR_CUDA;
+        if ((rc = launch_gemms(nullptr, &d, kPartReduceF32, static_cast<float*>(ws), nullptr, 0, stream))) return rc;
+        const FusedFinish p{static_cast<const float4*>(ws), bias, bias_bf16, gelu, static_cast<const uint4*>(residual), static_cast<uint4*>(pre), static_cast<uint4*>(d.c),
+                            static_cast<long>(n / 8), d.N};
+        return launch_pdl<linear_fused_finish_kernel>(static_cast<int>(std::min<long>((p.n8 + 255) / 256, 148 * 8)), 256, 0, stream, p);
+    }
+    GemmEpi epi;
+    epi.mode = gelu ? kEpiGelu : kEpiResidual;
+    epi.aux = residual;
+    epi.pre = pre;
+    return launch_gemms(&d, nullptr, kPartWhole, nullptr, bias, bias_bf16, stream, epi);
 }
 
 // Row slabs of the column sums: enough blocks for the chip, and few enough partial sums to add up afterwards.
@@ -581,13 +637,28 @@ int colsum_slabs(int M, int N) {
 }
 size_t linear_bwd_ws_bytes(int K, int N) { return round_up(static_cast<size_t>(K) * N * 4, 256) + static_cast<size_t>(kMaxColsumSlabs) * N * 4; }
 
+// The helper ahead of a backward's products: column sums of dy (`part`), zeroing of the accumulators, and with `pre` dz = dy gelu'(z).
+int launch_linear_prep(const void* dy, const void* pre, void* dz, float* part, int M, int N, bool atomic, float* zero, size_t zero_floats, cudaStream_t stream) {
+    const int slabs = colsum_slabs(M, N), rows = (M + slabs - 1) / slabs;
+    const dim3 grid((N + kColsumCols - 1) / kColsumCols, part || pre ? slabs : 64);
+    float4* z4 = reinterpret_cast<float4*>(zero);
+    const long n4 = static_cast<long>(zero_floats / 4);
+    const auto* g = static_cast<const __nv_bfloat16*>(dy);
+    return pre ? launch_pdl<linear_prep_kernel<true>>(grid, 256, 0, stream, g, static_cast<const __half*>(pre), static_cast<__nv_bfloat16*>(dz), part, M, N, rows,
+                                                      static_cast<int>(atomic), z4, n4)
+               : launch_pdl<linear_prep_kernel<false>>(grid, 256, 0, stream, g, static_cast<const __half*>(nullptr), static_cast<__nv_bfloat16*>(nullptr), part, M, N,
+                                                       rows, static_cast<int>(atomic), z4, n4);
+}
+
+// With `pre` (and a workspace) dy is first multiplied by gelu'(pre), into `dz`.
 int linear_bwd_core(const void* x, const void* w, const void* dy, void* dx, void* dw, void* db, int db_bf16, int M, int K, int N, void* ws, size_t ws_bytes,
-                    cudaStream_t stream) {
+                    cudaStream_t stream, const void* pre = nullptr, void* dz = nullptr) {
     if (!x || !w || !dy) return IB200_ERR_INVALID_ARGUMENT;
-    // dx[M,K] = dy[M,N] w^T: w is stored [K, N], i.e. the "B" of this product stored [N_out = K rows, contraction N contiguous]
-    const GemmDesc gx{dy, w, dx, M, K, N, 0, 0};
-    // dw[K,N] = x^T dy: x is stored [M, K], i.e. the "A" of this product stored [contraction M rows, K contiguous]
-    const GemmDesc gw{x, dy, dw, K, N, M, 1, 1};
+    const void* g = pre ? dz : dy;
+    // dx[M,K] = g[M,N] w^T: w is stored [K, N], i.e. the "B" of this product stored [N_out = K rows, contraction N contiguous]
+    const GemmDesc gx{g, w, dx, M, K, N, 0, 0};
+    // dw[K,N] = x^T g: x is stored [M, K], i.e. the "A" of this product stored [contraction M rows, K contiguous]
+    const GemmDesc gw{x, g, dw, K, N, M, 1, 1};
     int rc;
     if (dx && (rc = gemm_check(gx))) return rc;
     if (dw && (rc = gemm_check(gw))) return rc;
@@ -602,17 +673,12 @@ int linear_bwd_core(const void* x, const void* w, const void* dy, void* dx, void
     const bool split = dw && have_ws && (dx ? gemm_wants_split_beside(gw, pairs) : gemm_wants_split(gw, pairs));
     float* acc = split ? static_cast<float*>(ws) : nullptr;
     float* part = nullptr;
-    const int slabs = colsum_slabs(M, N);
     if (db) {
         part = have_ws ? reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + round_up(static_cast<size_t>(K) * N * 4, 256)) : static_cast<float*>(db);
         if (!have_ws && !cuda_ok(cudaMemsetAsync(db, 0, static_cast<size_t>(N) * 4, stream))) return IB200_ERR_CUDA;
     }
-    if (db || split) {
-        const int rows = (M + slabs - 1) / slabs;
-        const dim3 grid((N + kColsumCols - 1) / kColsumCols, db ? slabs : 64);
-        if ((rc = launch_pdl<linear_prep_kernel>(grid, 256, 0, stream, static_cast<const __nv_bfloat16*>(dy), part, M, N, rows, have_ws ? 0 : 1,
-                                                 reinterpret_cast<float4*>(acc), split ? static_cast<long>(K) * N / 4 : 0)))
-            return rc;
+    if (db || split || pre) {
+        if ((rc = launch_linear_prep(dy, pre, dz, part, M, N, !have_ws, acc, split ? static_cast<size_t>(K) * N : 0, stream))) return rc;
     }
     if (have_ws && dx && dw) {
         if ((rc = launch_gemms(&gx, &gw, split ? kPartReduceF32 : kPartWhole, acc, nullptr, 0, stream))) return rc;
@@ -621,7 +687,61 @@ int linear_bwd_core(const void* x, const void* w, const void* dy, void* dx, void
         if (dw && split && (rc = launch_gemms(nullptr, &gw, kPartReduceF32, acc, nullptr, 0, stream))) return rc;
         if (dw && !split && (rc = gemm_single(gw, nullptr, 0, nullptr, 0, stream))) return rc;
     }
-    return launch_linear_finish(acc, dw, static_cast<long>(K) * N, part, slabs, N, have_ws ? db : nullptr, db_bf16, stream);
+    return launch_linear_finish(finish_job(acc, dw, static_cast<long>(K) * N, part, colsum_slabs(M, N), N, have_ws ? db : nullptr, db_bf16), stream);
+}
+
+// The feed-forward block's backward: dz = (dy w2^T) gelu'(z) with the columns' sums in the epilogue of that product, which shares its launch with
+// dw2 = h^T dy; then dx = dz w1^T and dw1 = x^T dz in another.  Workspace: [acc1 | acc2 | dy's column sums | dz's column sums | dz].
+struct FfWorkspace {
+    size_t acc1, acc2, part2, part1, dz, bytes;
+    FfWorkspace(int M, int C, int H) {
+        const size_t w = round_up(static_cast<size_t>(C) * H * 4, 256);
+        acc1 = 0;
+        acc2 = w;
+        part2 = 2 * w;
+        part1 = part2 + round_up(static_cast<size_t>(kMaxColsumSlabs) * C * 4, 256);
+        dz = part1 + round_up((static_cast<size_t>(M) + 31) / 32 * H * 4, 256);
+        bytes = dz + round_up(static_cast<size_t>(M) * H * 2, 256);
+    }
+};
+int ff_bwd_core(const void* x, const void* w1, const void* pre, const void* h, const void* w2, const void* dy, void* dx, void* dw1, void* db1, int db1_bf16,
+                void* dw2, void* db2, int db2_bf16, int M, int C, int H, uint8_t* ws, cudaStream_t stream) {
+    const FfWorkspace L(M, C, H);
+    const bool inner = dx || dw1 || db1;
+    void* dz = ws + L.dz;
+    const GemmDesc gz{dy, w2, dz, M, H, C, 0, 0}, gw2{h, dy, dw2, H, C, M, 1, 1}, gx{dz, w1, dx, M, C, H, 0, 0}, gw1{x, dz, dw1, C, H, M, 1, 1};
+    int rc;
+    if ((inner && (rc = gemm_check(gz))) || (dw2 && (rc = gemm_check(gw2))) || (dx && (rc = gemm_check(gx))) || (dw1 && (rc = gemm_check(gw1)))) return rc;
+    if (!aligned16(dy) || !aligned16(pre)) return IB200_ERR_MISALIGNED;
+    const DeviceInfo* dev = device_info();
+    if (!dev) return IB200_ERR_NO_DEVICE;
+    const int pairs = dev->sms / 2;
+    const bool split2 = dw2 && (inner ? gemm_wants_split_beside(gw2, pairs) : gemm_wants_split(gw2, pairs));
+    const bool split1 = dw1 && (dx ? gemm_wants_split_beside(gw1, pairs) : gemm_wants_split(gw1, pairs));
+    float *acc1 = split1 ? reinterpret_cast<float*>(ws + L.acc1) : nullptr, *acc2 = split2 ? reinterpret_cast<float*>(ws + L.acc2) : nullptr;
+    float *part1 = db1 ? reinterpret_cast<float*>(ws + L.part1) : nullptr, *part2 = db2 ? reinterpret_cast<float*>(ws + L.part2) : nullptr;
+    if (db2 || split1 || split2) {
+        const size_t zero_bytes = split1 && split2 ? L.part2 : split1 || split2 ? L.acc2 : 0;      // the accumulators lie side by side
+        if ((rc = launch_linear_prep(dy, nullptr, nullptr, part2, M, C, false, split1 ? acc1 : acc2, zero_bytes / 4, stream))) return rc;
+    }
+    GemmEpi slope;
+    slope.mode = kEpiSlope;
+    slope.aux = pre;
+    slope.colsum = part1;
+    if (inner) {
+        if ((rc = launch_gemms(&gz, dw2 ? &gw2 : nullptr, split2 ? kPartReduceF32 : kPartWhole, acc2, nullptr, 0, stream, slope))) return rc;
+    } else if (dw2) {
+        if ((rc = split2 ? launch_gemms(nullptr, &gw2, kPartReduceF32, acc2, nullptr, 0, stream) : gemm_single(gw2, nullptr, 0, nullptr, 0, stream))) return rc;
+    }
+    if (dx && dw1) {
+        if ((rc = launch_gemms(&gx, &gw1, split1 ? kPartReduceF32 : kPartWhole, acc1, nullptr, 0, stream))) return rc;
+    } else {
+        if (dx && (rc = gemm_single(gx, nullptr, 0, nullptr, 0, stream))) return rc;
+        if (dw1 && (rc = split1 ? launch_gemms(nullptr, &gw1, kPartReduceF32, acc1, nullptr, 0, stream) : gemm_single(gw1, nullptr, 0, nullptr, 0, stream))) return rc;
+    }
+    const long n = static_cast<long>(C) * H;
+    return launch_linear_finish(finish_job(acc1, dw1, n, part1, (M + 31) / 32, H, db1, db1_bf16), finish_job(acc2, dw2, n, part2, colsum_slabs(M, C), C, db2, db2_bf16),
+                                stream);
 }
 
 // ---- layer norm ----------------------------------------------------------------------
@@ -943,6 +1063,46 @@ int ib200_linear_bwd_ws(const void* x, const void* w, const void* dy, void* dx, 
     if (db_dtype != IB200_DTYPE_F32 && db_dtype != IB200_DTYPE_BF16) return IB200_ERR_INVALID_ARGUMENT;
     if (!workspace || !aligned16(workspace) || (M > 0 && K > 0 && N > 0 && workspace_bytes < linear_bwd_ws_bytes(K, N))) return IB200_ERR_WORKSPACE;
     return linear_bwd_core(x, w, dy, dx, dw, db, db_dtype == IB200_DTYPE_BF16, M, K, N, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t ib200_fused_linear_workspace_bytes(int M, int K, int N, int activation, int pass) {
+    if (M <= 0 || K <= 0 || N <= 0) return 0;
+    if (pass != IB200_PASS_BWD) return ib200_linear_workspace_bytes(M, K, N, pass);
+    const size_t base = linear_bwd_ws_bytes(K, N);
+    return activation == IB200_ACT_GELU ? round_up(base, 256) + static_cast<size_t>(M) * N * 2 : base;
+}
+
+int ib200_fused_linear_fwd(const void* x, const void* w, const void* bias, int bias_dtype, const void* residual, int activation, void* y, void* preact, int M, int K,
+                           int N, void* workspace, size_t workspace_bytes, ib200_stream_t stream) {
+    if (!valid_dtype(bias_dtype) || (activation != IB200_ACT_NONE && activation != IB200_ACT_GELU)) return IB200_ERR_INVALID_ARGUMENT;
+    if (preact && activation == IB200_ACT_NONE) return IB200_ERR_INVALID_ARGUMENT;
+    if (workspace && !aligned16(workspace)) return IB200_ERR_WORKSPACE;
+    return fused_linear_fwd_core(GemmDesc{x, w, y, M, N, K, 0, 1}, bias, bias_dtype == IB200_DTYPE_BF16, residual, preact, activation == IB200_ACT_GELU, workspace,
+                                 workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int ib200_fused_linear_bwd(const void* x, const void* w, const void* dy, const void* preact, int activation, void* dx, void* dw, void* db, int db_dtype, int M, int K,
+                           int N, void* workspace, size_t workspace_bytes, ib200_stream_t stream) {
+    if (!valid_dtype(db_dtype) || (activation != IB200_ACT_NONE && activation != IB200_ACT_GELU)) return IB200_ERR_INVALID_ARGUMENT;
+    if ((activation == IB200_ACT_GELU) != (preact != nullptr) || M <= 0 || K <= 0 || N <= 0) return IB200_ERR_INVALID_ARGUMENT;
+    if (!aligned16(preact)) return IB200_ERR_MISALIGNED;
+    if (!workspace || !aligned16(workspace) || workspace_bytes < ib200_fused_linear_workspace_bytes(M, K, N, activation, IB200_PASS_BWD)) return IB200_ERR_WORKSPACE;
+    if (!dx && !dw && !db) return IB200_OK;
+    if (N % 8) return IB200_ERR_UNSUPPORTED;
+    void* dz = preact ? static_cast<uint8_t*>(workspace) + round_up(linear_bwd_ws_bytes(K, N), 256) : nullptr;
+    return linear_bwd_core(x, w, dy, dx, dw, db, db_dtype == IB200_DTYPE_BF16, M, K, N, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream), preact, dz);
+}
+
+size_t ib200_feed_forward_workspace_bytes(int M, int C, int H) { return M <= 0 || C <= 0 || H <= 0 ? 0 : FfWorkspace(M, C, H).bytes; }
+
+int ib200_feed_forward_bwd(const void* x, const void* w1, const void* preact, const void* h, const void* w2, const void* dy, void* dx, void* dw1, void* db1,
+                           int db1_dtype, void* dw2, void* db2, int db2_dtype, int M, int C, int H, void* workspace, size_t workspace_bytes, ib200_stream_t stream) {
+    if (!x || !w1 || !preact || !h || !w2 || !dy || M <= 0 || C <= 0 || H <= 0 || !valid_dtype(db1_dtype) || !valid_dtype(db2_dtype)) return IB200_ERR_INVALID_ARGUMENT;
+    if (C % 8 || H % 8) return IB200_ERR_UNSUPPORTED;
+    if (!workspace || !aligned16(workspace) || workspace_bytes < ib200_feed_forward_workspace_bytes(M, C, H)) return IB200_ERR_WORKSPACE;
+    if (!dx && !dw1 && !db1 && !dw2 && !db2) return IB200_OK;
+    return ff_bwd_core(x, w1, preact, h, w2, dy, dx, dw1, db1, db1_dtype == IB200_DTYPE_BF16, dw2, db2, db2_dtype == IB200_DTYPE_BF16, M, C, H,
+                       static_cast<uint8_t*>(workspace), reinterpret_cast<cudaStream_t>(stream));
 }
 
 size_t ib200_layer_norm_workspace_bytes(int M, int C, int dtype) {

@@ -52,6 +52,11 @@ struct Abi {
     decltype(&ib200_linear_workspace_bytes) linear_workspace_bytes = nullptr;
     decltype(&ib200_linear_fwd_ws) linear_fwd = nullptr;
     decltype(&ib200_linear_bwd_ws) linear_bwd = nullptr;
+    decltype(&ib200_fused_linear_workspace_bytes) fused_linear_workspace_bytes = nullptr;
+    decltype(&ib200_fused_linear_fwd) fused_linear_fwd = nullptr;
+    decltype(&ib200_fused_linear_bwd) fused_linear_bwd = nullptr;
+    decltype(&ib200_feed_forward_workspace_bytes) feed_forward_workspace_bytes = nullptr;
+    decltype(&ib200_feed_forward_bwd) feed_forward_bwd = nullptr;
     decltype(&ib200_layer_norm_workspace_bytes) layer_norm_workspace_bytes = nullptr;
     decltype(&ib200_layer_norm_fwd) layer_norm_fwd = nullptr;
     decltype(&ib200_layer_norm_bwd) layer_norm_bwd = nullptr;
@@ -570,6 +575,256 @@ Tensor linear(const Tensor& x, const Tensor& w, const Tensor& bias) {
     return y;
 }
 
+// ---- projections with an activation and a residual, and the feed-forward block of two of them ----------------------------
+void* ptr_or_null(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+// What the kernels address: dense, on 16 bytes.
+Tensor dense16(const Tensor& t) {
+    if (!t.defined()) return t;
+    const Tensor d = t.contiguous();
+    return reinterpret_cast<uintptr_t>(d.data_ptr()) & 15u ? d.clone() : d;
+}
+int rows_of(const Tensor& x, int64_t K) {
+    const int64_t M = x.numel() / K;
+    TORCH_CHECK_VALUE(M <= 0x7fffffff, "linear: too many rows, x is ", x.sizes());
+    return static_cast<int>(M);
+}
+// A projection's weight and bias, the shapes ahead of devices and types; `like`: a tensor on the device they must be on.
+void check_weight_shapes(const Tensor& w, const Tensor& bias) {
+    const int64_t K = w.size(0), N = w.size(1);
+    TORCH_CHECK_VALUE(K > 0 && N > 0 && K <= 0x7fffffff && N <= 0x7fffffff, "linear: w must have rows and columns, w is ", w.sizes());
+    TORCH_CHECK_VALUE(!bias.defined() || (bias.dim() == 1 && bias.size(0) == N), "linear: the bias must be [", N, "]");
+}
+void check_weight_types(const Tensor& w, const Tensor& bias, const Tensor& like) {
+    check_bf16_cuda(w, "w");
+    check_same_device(w, like, "w");
+    if (!bias.defined()) return;
+    check_same_device(bias, like, "the bias");
+    TORCH_CHECK_TYPE(bias.scalar_type() == at::kFloat || bias.scalar_type() == at::kBFloat16, "linear: the bias must be float32 or bfloat16");
+}
+// A tensor of the output's shape: x's, with N columns.
+void check_output_like(const Tensor& t, const Tensor& x, int64_t N, const char* name) {
+    const bool ok = t.dim() == x.dim() && t.size(-1) == N && t.sizes().slice(0, t.dim() - 1) == x.sizes().slice(0, x.dim() - 1);
+    TORCH_CHECK_VALUE(ok, "linear: ", name, " must have the output's shape, x's with a last axis of ", N, "; it is ", t.sizes(), ", x is ", x.sizes());
+}
+void check_output_type(const Tensor& t, const Tensor& x, const char* name) {
+    check_same_device(t, x, name);
+    check_bf16_cuda(t, name);
+}
+void check_fused(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& residual) {
+    check_linear_shapes(x, w);
+    check_weight_shapes(w, bias);
+    if (residual.defined()) check_output_like(residual, x, w.size(1), "the residual");
+    rows_of(x, w.size(0));
+    check_bf16_cuda(x, "x");
+    check_weight_types(w, bias, x);
+    if (residual.defined()) check_output_type(residual, x, "the residual");
+}
+// Scratch of one call, held with the stream's lock until its launches are issued.
+struct Scratch {
+    std::unique_lock<std::mutex> lock;
+    Tensor buf;
+    Scratch(size_t bytes, c10::Device device, cudaStream_t stream) {
+        if (!bytes) return;
+        Workspace& ws = workspace_of(device.index(), stream);
+        lock = std::unique_lock<std::mutex>(ws.launching);
+        buf = linear_scratch(ws, bytes, device);
+    }
+    void* ptr() const { return ptr_or_null(buf); }
+};
+
+struct Fused {
+    Tensor y, pre;
+};
+// y = act(x w + bias) + residual; with `keep` (and an activation) z as fp16, for the backward.
+Fused fused_linear_forward(const Tensor& x_, const Tensor& w_, const Tensor& bias_, int act, const Tensor& residual_, bool keep) {
+    check_fused(x_, w_, bias_, residual_);
+    const c10::cuda::CUDAGuard guard(x_.device());
+    const int64_t K = w_.size(0), N = w_.size(1);
+    const int M = rows_of(x_, K);
+    auto shape = x_.sizes().vec();
+    shape.back() = N;
+    Fused r;
+    r.y = at::empty(shape, x_.options());
+    if (keep && act != IB200_ACT_NONE) r.pre = at::empty(shape, x_.options().dtype(at::kHalf));
+    if (M == 0) return r;
+    const Tensor x = dense16(x_), w = dense16(w_), b = dense16(bias_), res = dense16(residual_);
+    const int k = static_cast<int>(K), n = static_cast<int>(N);
+    cudaStream_t stream = c10::cuda::getCurrentCUDAStream(x.device().index()).stream();
+    const size_t bytes = g_abi.fused_linear_workspace_bytes(M, k, n, act, IB200_PASS_FWD);
+    const Scratch scratch(bytes, x.device(), stream);
+    check_status(g_abi.fused_linear_fwd(x.data_ptr(), w.data_ptr(), ptr_or_null(b), b.defined() ? dtype_code(b) : IB200_DTYPE_F32, ptr_or_null(res), act,
+                                        r.y.data_ptr(), ptr_or_null(r.pre), M, k, n, scratch.ptr(), bytes, reinterpret_cast<ib200_stream_t>(stream)),
+                 "ib200_fused_linear_fwd");
+    return r;
+}
+void check_preact(const Tensor& pre, const Tensor& x, int64_t N) {
+    TORCH_CHECK_VALUE(pre.defined() && pre.numel() == x.numel() / x.size(-1) * N && pre.device() == x.device() && pre.scalar_type() == at::kHalf,
+                      "linear: preact must be the float16 pre-activation that the forward kept");
+}
+LinearGrads fused_linear_backward(const Tensor& x_, const Tensor& w_, const Tensor& dy_, const Tensor& pre_, int act, bool need_dx, bool need_dw, bool need_db,
+                                  bool db_bf16) {
+    check_linear_shapes(x_, w_);
+    const int64_t K = w_.size(0), N = w_.size(1);
+    check_output_like(dy_, x_, N, "dy");
+    check_fused(x_, w_, Tensor(), Tensor());
+    check_output_type(dy_, x_, "dy");
+    if (act != IB200_ACT_NONE) check_preact(pre_, x_, N);
+    const c10::cuda::CUDAGuard guard(x_.device());
+    const int M = rows_of(x_, K);
+    LinearGrads g;
+    const auto db_type = x_.options().dtype(db_bf16 ? at::kBFloat16 : at::kFloat);
+    if (need_dx) g.dx = at::empty(x_.sizes(), x_.options());
+    if (need_dw) g.dw = M ? at::empty({K, N}, x_.options()) : at::zeros({K, N}, x_.options());
+    if (need_db) g.db = M ? at::empty({N}, db_type) : at::zeros({N}, db_type);
+    if (M == 0 || (!need_dx && !need_dw && !need_db)) return g;
+    const Tensor x = dense16(x_), w = dense16(w_), dy = dense16(dy_), pre = act != IB200_ACT_NONE ? dense16(pre_) : Tensor();
+    const int k = static_cast<int>(K), n = static_cast<int>(N);
+    cudaStream_t stream = c10::cuda::getCurrentCUDAStream(x.device().index()).stream();
+    const size_t bytes = g_abi.fused_linear_workspace_bytes(M, k, n, act, IB200_PASS_BWD);
+    const Scratch scratch(bytes, x.device(), stream);
+    check_status(g_abi.fused_linear_bwd(x.data_ptr(), w.data_ptr(), dy.data_ptr(), ptr_or_null(pre), act, ptr_or_null(g.dx), ptr_or_null(g.dw), ptr_or_null(g.db),
+                                        db_bf16 ? IB200_DTYPE_BF16 : IB200_DTYPE_F32, M, k, n, scratch.ptr(), bytes, reinterpret_cast<ib200_stream_t>(stream)),
+                 "ib200_fused_linear_bwd");
+    return g;
+}
+
+struct FusedLinearBackward : torch::autograd::Node {
+    SavedVariable x, w, pre;
+    int act = IB200_ACT_NONE;
+    at::ScalarType bias_type = at::kFloat;
+
+    variable_list apply(variable_list&& grads) override {
+        return in_node([&] { return backward(grads); });
+    }
+    variable_list backward(const variable_list& grads) {
+        variable_list out(4);
+        if (!grads[0].defined()) return out;
+        const Tensor tx = x.unpack(), tw = w.unpack(), tp = act != IB200_ACT_NONE ? pre.unpack() : Tensor();
+        at::AutoDispatchBelowADInplaceOrView below;
+        const LinearGrads g = fused_linear_backward(tx, tw, grads[0], tp, act, task_should_compute_output(0), task_should_compute_output(1),
+                                                    task_should_compute_output(2), bias_type == at::kBFloat16);
+        out = {g.dx, g.dw, g.db, task_should_compute_output(3) ? grads[0] : Tensor()};      // the residual's gradient is dy itself
+        return out;
+    }
+    void release_variables() override { x.reset_data(); w.reset_data(); pre.reset_data(); }
+    std::string name() const override { return "FusedLinearBackward"; }
+};
+
+Tensor fused_linear(const Tensor& x, const Tensor& w, const Tensor& bias, int act, const Tensor& residual) {
+    refuse_tangents({&x, &w, &bias, &residual}, "fused_linear");
+    const bool differentiable = torch::autograd::compute_requires_grad(x, w, bias, residual);
+    Fused r;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        r = fused_linear_forward(x, w, bias, act, residual, differentiable);
+    }
+    if (differentiable) {
+        auto node = std::shared_ptr<FusedLinearBackward>(new FusedLinearBackward(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(x, w, bias, residual));
+        node->x = SavedVariable(x, false);
+        node->w = SavedVariable(w, false);
+        node->act = act;
+        if (r.pre.defined()) node->pre = SavedVariable(r.pre, false);
+        if (bias.defined()) node->bias_type = bias.scalar_type();
+        torch::autograd::set_history(r.y, node);
+    }
+    return r.y;
+}
+
+// y = gelu(x w1 + b1) w2 + b2 (+ residual)
+void check_feed_forward(const Tensor& x, const Tensor& w1, const Tensor& b1, const Tensor& w2, const Tensor& b2, const Tensor& residual) {
+    check_linear_shapes(x, w1);
+    TORCH_CHECK_VALUE(w2.dim() == 2 && w2.size(0) == w1.size(1) && w2.size(1) == w1.size(0), "feed_forward: w2 must be w1's shape turned round, w1 is ", w1.sizes(),
+                      ", w2 is ", w2.sizes());
+    check_weight_shapes(w1, b1);
+    check_weight_shapes(w2, b2);
+    if (residual.defined()) check_output_like(residual, x, x.size(-1), "the residual");
+    rows_of(x, w1.size(0));
+    check_bf16_cuda(x, "x");
+    check_weight_types(w1, b1, x);
+    check_weight_types(w2, b2, x);
+    if (residual.defined()) check_output_type(residual, x, "the residual");
+}
+struct FeedForwardGrads {
+    Tensor dx, dw1, db1, dw2, db2;
+};
+FeedForwardGrads feed_forward_backward(const Tensor& x_, const Tensor& w1_, const Tensor& pre_, const Tensor& h_, const Tensor& w2_, const Tensor& dy_,
+                                       const bool (&need)[5], at::ScalarType b1_type, at::ScalarType b2_type) {
+    check_feed_forward(x_, w1_, Tensor(), w2_, Tensor(), Tensor());
+    const int64_t C = w1_.size(0), H = w1_.size(1);
+    check_output_like(dy_, x_, C, "dy");
+    check_output_type(dy_, x_, "dy");
+    check_preact(pre_, x_, H);
+    TORCH_CHECK_VALUE(h_.numel() == pre_.numel() && h_.device() == x_.device() && h_.scalar_type() == at::kBFloat16, "feed_forward: h must be the forward's hidden layer");
+    const c10::cuda::CUDAGuard guard(x_.device());
+    const int M = rows_of(x_, C);
+    auto output = [&](bool wanted, at::IntArrayRef shape, at::ScalarType type) {
+        if (!wanted) return Tensor();
+        return M ? at::empty(shape, x_.options().dtype(type)) : at::zeros(shape, x_.options().dtype(type));
+    };
+    FeedForwardGrads g{output(need[0], x_.sizes(), at::kBFloat16), output(need[1], {C, H}, at::kBFloat16), output(need[2], {H}, b1_type),
+                       output(need[3], {H, C}, at::kBFloat16), output(need[4], {C}, b2_type)};
+    if (M == 0) return g;
+    const Tensor x = dense16(x_), w1 = dense16(w1_), pre = dense16(pre_), h = dense16(h_), w2 = dense16(w2_), dy = dense16(dy_);
+    const int c = static_cast<int>(C), hh = static_cast<int>(H);
+    auto code = [](at::ScalarType t) { return t == at::kBFloat16 ? IB200_DTYPE_BF16 : IB200_DTYPE_F32; };
+    cudaStream_t stream = c10::cuda::getCurrentCUDAStream(x.device().index()).stream();
+    const size_t bytes = g_abi.feed_forward_workspace_bytes(M, c, hh);
+    const Scratch scratch(bytes, x.device(), stream);
+    check_status(g_abi.feed_forward_bwd(x.data_ptr(), w1.data_ptr(), pre.data_ptr(), h.data_ptr(), w2.data_ptr(), dy.data_ptr(), ptr_or_null(g.dx), ptr_or_null(g.dw1),
+                                        ptr_or_null(g.db1), code(b1_type), ptr_or_null(g.dw2), ptr_or_null(g.db2), code(b2_type), M, c, hh, scratch.ptr(), bytes,
+                                        reinterpret_cast<ib200_stream_t>(stream)),
+                 "ib200_feed_forward_bwd");
+    return g;
+}
+
+struct FeedForwardBackward : torch::autograd::Node {
+    SavedVariable x, w1, pre, h, w2;
+    at::ScalarType b1_type = at::kFloat, b2_type = at::kFloat;
+
+    variable_list apply(variable_list&& grads) override {
+        return in_node([&] { return backward(grads); });
+    }
+    variable_list backward(const variable_list& grads) {
+        if (!grads[0].defined()) return variable_list(6);
+        const Tensor tx = x.unpack(), t1 = w1.unpack(), tp = pre.unpack(), th = h.unpack(), t2 = w2.unpack();
+        at::AutoDispatchBelowADInplaceOrView below;
+        bool need[5];
+        for (int i = 0; i < 5; ++i) need[i] = task_should_compute_output(i);
+        const FeedForwardGrads g = feed_forward_backward(tx, t1, tp, th, t2, grads[0], need, b1_type, b2_type);
+        return {g.dx, g.dw1, g.db1, g.dw2, g.db2, task_should_compute_output(5) ? grads[0] : Tensor()};
+    }
+    void release_variables() override {
+        x.reset_data(); w1.reset_data(); pre.reset_data(); h.reset_data(); w2.reset_data();
+    }
+    std::string name() const override { return "FeedForwardBackward"; }
+};
+
+Tensor feed_forward(const Tensor& x, const Tensor& w1, const Tensor& b1, const Tensor& w2, const Tensor& b2, const Tensor& residual) {
+    refuse_tangents({&x, &w1, &b1, &w2, &b2, &residual}, "feed_forward");
+    check_feed_forward(x, w1, b1, w2, b2, residual);
+    const bool differentiable = torch::autograd::compute_requires_grad(x, w1, b1, w2, b2, residual);
+    Fused hidden, r;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        hidden = fused_linear_forward(x, w1, b1, IB200_ACT_GELU, Tensor(), differentiable);
+        r = fused_linear_forward(hidden.y, w2, b2, IB200_ACT_NONE, residual, false);
+    }
+    if (differentiable) {
+        auto node = std::shared_ptr<FeedForwardBackward>(new FeedForwardBackward(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(x, w1, b1, w2, b2, residual));
+        node->x = SavedVariable(x, false);
+        node->w1 = SavedVariable(w1, false);
+        node->pre = SavedVariable(hidden.pre, false);
+        node->h = SavedVariable(hidden.y, false);
+        node->w2 = SavedVariable(w2, false);
+        if (b1.defined()) node->b1_type = b1.scalar_type();
+        if (b2.defined()) node->b2_type = b2.scalar_type();
+        torch::autograd::set_history(r.y, node);
+    }
+    return r.y;
+}
+
 // ---- layer norm ----------------------------------------------------------------------
 int type_code(const Tensor& t, const char* op, const char* name) {
     TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16, op, ": ", name, " must be float32 or bfloat16");
@@ -632,10 +887,9 @@ Norm layer_norm_forward(const Tensor& x_, const Tensor& weight_, const Tensor& b
         r.rstd = at::empty(shape, x_.options().dtype(at::kFloat));
     }
     if (x_.numel() == 0) return r;
-    auto ptr = [](const Tensor& t) -> void* { return t.defined() ? t.data_ptr() : nullptr; };
     cudaStream_t stream = c10::cuda::getCurrentCUDAStream(x_.device().index()).stream();
-    check_status(g_abi.layer_norm_fwd(x.t.data_ptr(), x.pitch, ptr(w), ptr(b), param, r.y.data_ptr(), static_cast<float*>(ptr(r.mean)),
-                                      static_cast<float*>(ptr(r.rstd)), static_cast<int>(x_.numel() / C), static_cast<int>(C), static_cast<float>(eps), dtype_code(x_),
+    check_status(g_abi.layer_norm_fwd(x.t.data_ptr(), x.pitch, ptr_or_null(w), ptr_or_null(b), param, r.y.data_ptr(), static_cast<float*>(ptr_or_null(r.mean)),
+                                      static_cast<float*>(ptr_or_null(r.rstd)), static_cast<int>(x_.numel() / C), static_cast<int>(C), static_cast<float>(eps), dtype_code(x_),
                                       reinterpret_cast<ib200_stream_t>(stream)),
                  "ib200_layer_norm_fwd");
     return r;
@@ -665,15 +919,12 @@ NormGrads layer_norm_backward(const Tensor& x_, const Tensor& dy_, const Tensor&
     if (need_dw) g.dw = M ? at::empty({C}, param) : at::zeros({C}, param);
     if (need_db) g.db = M ? at::empty({C}, param) : at::zeros({C}, param);
     if (M == 0 || (!need_dx && !need_dw && !need_db)) return g;
-    auto ptr = [](const Tensor& t) -> void* { return t.defined() ? t.data_ptr() : nullptr; };
     const int m = static_cast<int>(M), c = static_cast<int>(C), dtype = dtype_code(x_);
     const size_t bytes = need_dw || need_db ? g_abi.layer_norm_workspace_bytes(m, c, dtype) : 0;
     cudaStream_t stream = c10::cuda::getCurrentCUDAStream(x_.device().index()).stream();
-    Workspace& ws = workspace_of(x_.device().index(), stream);
-    std::lock_guard<std::mutex> lock(ws.launching);
-    const Tensor scratch = bytes ? linear_scratch(ws, bytes, x_.device()) : Tensor();
-    check_status(g_abi.layer_norm_bwd(x.t.data_ptr(), x.pitch, ptr(w), dy.t.data_ptr(), dy.pitch, mean.data_ptr<float>(), rstd.data_ptr<float>(), ptr(g.dx), ptr(g.dw),
-                                      ptr(g.db), param_type == at::kBFloat16 ? IB200_DTYPE_BF16 : IB200_DTYPE_F32, m, c, dtype, ptr(scratch), bytes,
+    const Scratch scratch(bytes, x_.device(), stream);
+    check_status(g_abi.layer_norm_bwd(x.t.data_ptr(), x.pitch, ptr_or_null(w), dy.t.data_ptr(), dy.pitch, mean.data_ptr<float>(), rstd.data_ptr<float>(), ptr_or_null(g.dx), ptr_or_null(g.dw),
+                                      ptr_or_null(g.db), param_type == at::kBFloat16 ? IB200_DTYPE_BF16 : IB200_DTYPE_F32, m, c, dtype, scratch.ptr(), bytes,
                                       reinterpret_cast<ib200_stream_t>(stream)),
                  "ib200_layer_norm_bwd");
     return g;
@@ -751,6 +1002,13 @@ int arg_total_heads(PyObject* o) {
     TORCH_CHECK_VALUE(n > 0 && n <= 0x7fffffff, "causal_attention: total_heads must be a positive number of heads, got ", n);
     return static_cast<int>(n);
 }
+int arg_activation(PyObject* o) {
+    if (o == Py_None) return IB200_ACT_NONE;
+    const char* name = PyUnicode_Check(o) ? PyUnicode_AsUTF8(o) : nullptr;
+    if (!name && PyErr_Occurred()) throw python_error();
+    TORCH_CHECK_VALUE(name && std::string(name) == "gelu", "linear: activation must be None or \"gelu\"");
+    return IB200_ACT_GELU;
+}
 bool arg_bool(PyObject* o) {
     const int v = PyObject_IsTrue(o);
     if (v < 0) throw python_error();
@@ -801,6 +1059,11 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
         get(g_abi.linear_workspace_bytes, "ib200_linear_workspace_bytes");
         get(g_abi.linear_fwd, "ib200_linear_fwd_ws");
         get(g_abi.linear_bwd, "ib200_linear_bwd_ws");
+        get(g_abi.fused_linear_workspace_bytes, "ib200_fused_linear_workspace_bytes");
+        get(g_abi.fused_linear_fwd, "ib200_fused_linear_fwd");
+        get(g_abi.fused_linear_bwd, "ib200_fused_linear_bwd");
+        get(g_abi.feed_forward_workspace_bytes, "ib200_feed_forward_workspace_bytes");
+        get(g_abi.feed_forward_bwd, "ib200_feed_forward_bwd");
         get(g_abi.layer_norm_workspace_bytes, "ib200_layer_norm_workspace_bytes");
         get(g_abi.layer_norm_fwd, "ib200_layer_norm_fwd");
         get(g_abi.layer_norm_bwd, "ib200_layer_norm_bwd");
@@ -933,6 +1196,70 @@ PyObject* py_linear_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// (x, w, bias, activation, residual) -> y, differentiable
+PyObject* py_fused_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        want(n, 5);
+        const Tensor &x = arg_tensor(a[0]), &w = arg_tensor(a[1]);
+        const Tensor bias = arg_opt_tensor(a[2]), residual = arg_opt_tensor(a[4]);
+        const int act = arg_activation(a[3]);
+        Tensor y;
+        {
+            pybind11::gil_scoped_release nogil;
+            y = fused_linear(x, w, bias, act, residual);
+        }
+        return wrap(y);
+    });
+}
+// (x, w, bias, activation, residual, keep_preact) -> (y, preact)
+PyObject* py_fused_linear_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        want(n, 6);
+        const Tensor &x = arg_tensor(a[0]), &w = arg_tensor(a[1]);
+        const Tensor bias = arg_opt_tensor(a[2]), residual = arg_opt_tensor(a[4]);
+        const int act = arg_activation(a[3]);
+        const bool keep = arg_bool(a[5]);
+        Fused r;
+        {
+            pybind11::gil_scoped_release nogil;
+            at::AutoDispatchBelowADInplaceOrView below;
+            r = fused_linear_forward(x, w, bias, act, residual, keep);
+        }
+        return wrap_tuple({&r.y, &r.pre});
+    });
+}
+// (x, w, dy, preact, activation, need_dx, need_dw, need_db) -> (dx, dw, db)
+PyObject* py_fused_linear_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        want(n, 8);
+        const Tensor &x = arg_tensor(a[0]), &w = arg_tensor(a[1]), &dy = arg_tensor(a[2]);
+        const Tensor pre = arg_opt_tensor(a[3]);
+        const int act = arg_activation(a[4]);
+        const bool need_dx = arg_bool(a[5]), need_dw = arg_bool(a[6]), need_db = arg_bool(a[7]);
+        LinearGrads g;
+        {
+            pybind11::gil_scoped_release nogil;
+            at::AutoDispatchBelowADInplaceOrView below;
+            g = fused_linear_backward(x, w, dy, pre, act, need_dx, need_dw, need_db, false);
+        }
+        return wrap_tuple({&g.dx, &g.dw, &g.db});
+    });
+}
+// (x, w1, b1, w2, b2, residual) -> y, differentiable
+PyObject* py_feed_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        want(n, 6);
+        const Tensor &x = arg_tensor(a[0]), &w1 = arg_tensor(a[1]), &w2 = arg_tensor(a[3]);
+        const Tensor b1 = arg_opt_tensor(a[2]), b2 = arg_opt_tensor(a[4]), residual = arg_opt_tensor(a[5]);
+        Tensor y;
+        {
+            pybind11::gil_scoped_release nogil;
+            y = feed_forward(x, w1, b1, w2, b2, residual);
+        }
+        return wrap(y);
+    });
+}
+
 // (x, weight, bias, eps) -> y, differentiable
 PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
@@ -1044,6 +1371,10 @@ PyMethodDef g_methods[] = {IB200_PY(bind),
                            IB200_PY(linear),
                            IB200_PY(linear_forward),
                            IB200_PY(linear_backward),
+                           IB200_PY(fused_linear),
+                           IB200_PY(fused_linear_forward),
+                           IB200_PY(fused_linear_backward),
+                           IB200_PY(feed_forward),
                            IB200_PY(layer_norm),
                            IB200_PY(layer_norm_forward),
                            IB200_PY(layer_norm_backward),

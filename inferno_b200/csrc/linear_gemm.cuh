@@ -30,9 +30,20 @@
 //   bf16 output itself (one rounding per partial, at most eight).
 #pragma once
 
+#include <cuda_fp16.h>
+
 #include "sm100_ptx.cuh"
 
 namespace ib200 {
+
+// What the epilogue of task 0 does beyond adding the bias.  Each is a kernel of its own: a run-time branch would put every form's registers and
+// code into the plain one.
+enum : int {
+    kEpiBias = 0,          // c = acc + bias
+    kEpiResidual = 1,      // c = acc + bias + aux
+    kEpiGelu = 2,          // z = acc + bias;  c = gelu(z) (+ aux);  z kept as fp16 if it is wanted
+    kEpiSlope = 3,         // c = acc gelu'(z) with z = aux, and the column sums of c
+};
 
 struct GemmTraits {
     static constexpr int BM = 256, BN = 256, BK = 64;            // tile of a CTA pair
@@ -41,14 +52,22 @@ struct GemmTraits {
     static constexpr int A_BYTES = CM * BK * 2;                  // 16 KB
     static constexpr int B_BYTES = CN * BK * 2;                  // 16 KB
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-    static constexpr int OFF_OUT = STAGES * STAGE_BYTES;
     static constexpr int STAGING_BYTES = 32 * 128;               // epilogue staging of one warp
-    static constexpr int OFF_BAR = OFF_OUT + 8 * STAGING_BYTES;
-    static constexpr int SMEM_BYTES = OFF_BAR + 256 + 1024;
     static constexpr int EPI_WARPS = 8;                          // two per 32 rows of the tile, each with half of its columns
     static constexpr int THREADS = EPI_WARPS * 32 + 64;          // and the TMA warp and the MMA warp
     static constexpr uint32_t TM_COLS = 512;
-    static_assert(SMEM_BYTES <= 232448, "shared memory budget");
+};
+// Shared memory of a kernel form.  The fused epilogues bring a second 4 KB tile per epilogue warp (what is added or multiplied, or the second
+// output), which takes the place of one of the ring's six stages.
+template <int EPI>
+struct GemmSmem {
+    static constexpr int STAGES = EPI == kEpiBias ? GemmTraits::STAGES : 5;
+    static constexpr int OFF_OUT = STAGES * GemmTraits::STAGE_BYTES;
+    static constexpr int OFF_AUX = OFF_OUT + GemmTraits::EPI_WARPS * GemmTraits::STAGING_BYTES;
+    static constexpr int OFF_BAR = OFF_AUX + (EPI == kEpiBias ? 0 : GemmTraits::EPI_WARPS * GemmTraits::STAGING_BYTES);
+    static constexpr int BYTES = OFF_BAR + 256 + 1024;
+    static_assert(BYTES <= 232448, "shared memory budget");
+    static_assert((2 * STAGES + 4 + GemmTraits::EPI_WARPS) * 8 + 8 <= 256, "barriers");
 };
 
 struct GemmTask {
@@ -68,6 +87,9 @@ struct GemmParams {
     long long w_heavy, w_light, w_total;
     const void* bias;      // [N] of task 0 (task 1 when it is the only one), or null
     int bias_bf16;
+    int has_aux;           // kEpiGelu: a residual is added
+    int write_pre;         // kEpiGelu: z is kept
+    float* colsum;         // kEpiSlope: column sums of each 32 rows, [ceil(M / 32)][N], or null
     int* status;
 };
 
@@ -126,8 +148,9 @@ struct GemmWalk {
 
 // The tensor maps of a launch: operands and outputs of the two tasks, and what a split task 1 is added into (its bf16 output,
 // or the fp32 accumulation workspace).
+// aux: what a fused epilogue reads beside its tile; pre: where it keeps z.
 struct GemmMaps {
-    CUtensorMap a[2], b[2], c[2], sum;
+    CUtensorMap a[2], b[2], c[2], sum, aux, pre;
 };
 
 __device__ __forceinline__ float2 load_bias2(const GemmParams& p, int col) {      // col is even
@@ -135,19 +158,46 @@ __device__ __forceinline__ float2 load_bias2(const GemmParams& p, int col) {    
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(static_cast<const __nv_bfloat16*>(p.bias) + col));
 }
 
+// gelu in its tanh form is z s(2u) with the logistic function s and u = sqrt(2 / pi) (z + 0.044715 z^3): 0.5 (1 + tanh u) = s(2u).  As one exponential
+// and one reciprocal it keeps its relative precision where 1 + tanh u cancels, and both ends come out right without a branch (e^-2u is 0 or
+// infinite).  Constants: -2 sqrt(2 / pi) log2 e, and that times 0.044715.
+constexpr float kGeluExp1 = -2.302208198f, kGeluExp3 = kGeluExp1 * 0.044715f;
+constexpr float kGeluDu1 = 1.595769122f, kGeluDu3 = kGeluDu1 * 3.f * 0.044715f;      // d(2u)/dz = kGeluDu1 + kGeluDu3 z^2
+__device__ __forceinline__ float gelu_gate(float z) {                                // s(2u)
+    return __fdividef(1.f, 1.f + fast_exp2(z * fmaf(kGeluExp3, z * z, kGeluExp1)));
+}
+__device__ __forceinline__ float gelu(float z) { return z * gelu_gate(z); }
+__device__ __forceinline__ float gelu_slope(float z) {                               // |z| <= kPreactLimit
+    const float s = gelu_gate(z);
+    return fmaf(z * fmaf(kGeluDu3, z * z, kGeluDu1), s * (1.f - s), s);
+}
+// z is kept for the backward in fp16: beyond 16 the slope is 0 or 1 to the last bit of an fp32, so it is kept as +-16 (NaN stays NaN), and within that
+// fp16 has three bits more than bf16.  With z in bf16 the gradients would be half as far off again as their own rounding leaves them.
+constexpr float kPreactLimit = 16.f;
+__device__ __forceinline__ float preact_clamp(float z) { return z > kPreactLimit ? kPreactLimit : z < -kPreactLimit ? -kPreactLimit : z; }
+__device__ __forceinline__ uint32_t pack_preact2(float a, float b) {
+    const __half2 h = __floats2half2_rn(preact_clamp(a), preact_clamp(b));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack_half2(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+__device__ __forceinline__ float2 unpack_bf16x2(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+
+template <int EPI>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmTraits::THREADS, 1)
 gemm_bf16_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ GemmParams prm) {
     using TR = GemmTraits;
-    constexpr int BN = TR::BN, BK = TR::BK, NS = TR::STAGES, kTmaWarp = TR::EPI_WARPS, kMmaWarp = TR::EPI_WARPS + 1;
+    using SM = GemmSmem<EPI>;
+    constexpr int BN = TR::BN, BK = TR::BK, NS = SM::STAGES, kTmaWarp = TR::EPI_WARPS, kMmaWarp = TR::EPI_WARPS + 1;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    uint8_t* sOut = smem + TR::OFF_OUT;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + TR::OFF_BAR);
+    uint8_t* sOut = smem + SM::OFF_OUT;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SM::OFF_BAR);
     uint64_t* full = bars;                  // [NS]  TMA of both CTAs -> MMA (used in the even CTA)
     uint64_t* empty = full + NS;            // [NS]  MMA -> TMA (in both)
     uint64_t* acc_full = empty + NS;        // [2]   MMA -> epilogue (in both)
     uint64_t* acc_empty = acc_full + 2;     // [2]   the epilogues of both CTAs -> MMA (used in the even CTA)
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    uint64_t* aux_full = acc_empty + 2;     // [EPI_WARPS]  TMA -> that warp (fused epilogues)
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(aux_full + TR::EPI_WARPS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -159,6 +209,8 @@ gemm_bf16_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ 
         *abort_flag = 0;
         for (int s = 0; s < NS; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * TR::EPI_WARPS); }
+        if (EPI != kEpiBias)
+            for (int w = 0; w < TR::EPI_WARPS; ++w) mbar_init(&aux_full[w], 1);
         fence_mbar_init();
     }
     if (warp == kMmaWarp) { tmem_alloc_pair(tmem_slot, TR::TM_COLS); tmem_relinquish_pair(); }
@@ -269,60 +321,215 @@ gemm_bf16_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ 
                 tma_store_commit();
             }
         };
-        for (; walk.next(q); ++n) {
-            const GemmTask& k = prm.t[q.task];
-            const uint32_t buf = n & 1;
-            const int row = q.m0 + static_cast<int>(rank) * TR::CM + row0;
-            const bool with_bias = prm.bias && q.ks0 == 0;       // the part that starts the tile's K range brings the bias in
-            const bool f32_out = q.partial && prm.split == kPartReduceF32;
-            const CUtensorMap* mc = q.partial ? &maps.sum : &maps.c[q.task];
-            // two columns of bias per lane and 64-column step, fetched under the wait and handed round by shuffles (broadcast loads in
-            // the element loop queued behind the MMAs' operand reads for 2000 cycles and more)
-            float2 bias0 = make_float2(0.f, 0.f), bias1 = bias0;
-            if (with_bias) {
-                const int col = q.n0 + h * (BN / 2) + 2 * lane;
-                if (col < k.N) bias0 = load_bias2(prm, col);
-                if (col + 64 < k.N) bias1 = load_bias2(prm, col + 64);
+        auto pack_tile = [](const uint32_t (&v)[2][32], uint4 (&w)[8]) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                const uint32_t* x = &v[c >> 2][(c & 3) * 8];
+                w[c] = make_uint4(pack_bf16x2(__uint_as_float(x[0]), __uint_as_float(x[1])), pack_bf16x2(__uint_as_float(x[2]), __uint_as_float(x[3])),
+                                  pack_bf16x2(__uint_as_float(x[4]), __uint_as_float(x[5])), pack_bf16x2(__uint_as_float(x[6]), __uint_as_float(x[7])));
             }
-            mbar_wait(&acc_full[buf], (n >> 1) & 1, ab, 30);
-            tc_fence_after_sync();
-#pragma unroll 1
-            for (int c0 = h * (BN / 2); c0 < (h + 1) * (BN / 2); c0 += 64) {
-                const int col = q.n0 + c0;
-                uint32_t v[2][32];
-                tmem_ld_x32(tmem + buf * BN + c0 + lane_base, v[0]);
-                tmem_ld_x32(tmem + buf * BN + c0 + 32 + lane_base, v[1]);
-                tmem_wait_ld();
-                if (c0 + 64 == (h + 1) * (BN / 2)) {
-                    // every column of the accumulator is in registers: hand it back to the MMA warp
-                    tc_fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster_relaxed(free_bar[buf]);
-                }
-                if (row >= k.M || col >= k.N) continue;
+        };
+        if constexpr (EPI == kEpiBias) {
+            for (; walk.next(q); ++n) {
+                const GemmTask& k = prm.t[q.task];
+                const uint32_t buf = n & 1;
+                const int row = q.m0 + static_cast<int>(rank) * TR::CM + row0;
+                const bool with_bias = prm.bias && q.ks0 == 0;       // the part that starts the tile's K range brings the bias in
+                const bool f32_out = q.partial && prm.split == kPartReduceF32;
+                const CUtensorMap* mc = q.partial ? &maps.sum : &maps.c[q.task];
+                // two columns of bias per lane and 64-column step, fetched under the wait and handed round by shuffles (broadcast loads in
+                // the element loop queued behind the MMAs' operand reads for 2000 cycles and more)
+                float2 bias0 = make_float2(0.f, 0.f), bias1 = bias0;
                 if (with_bias) {
-                    const float2 bc = c0 & 64 ? bias1 : bias0;
-#pragma unroll
-                    for (int e = 0; e < 64; ++e)
-                        v[e >> 5][e & 31] = __float_as_uint(__uint_as_float(v[e >> 5][e & 31]) + __shfl_sync(0xffffffffu, e & 1 ? bc.y : bc.x, e >> 1));
+                    const int col = q.n0 + h * (BN / 2) + 2 * lane;
+                    if (col < k.N) bias0 = load_bias2(prm, col);
+                    if (col + 64 < k.N) bias1 = load_bias2(prm, col + 64);
                 }
-                uint4 w[8];
-                if (!f32_out) {
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        const uint32_t* x = &v[c >> 2][(c & 3) * 8];
-                        w[c] = make_uint4(pack_bf16x2(__uint_as_float(x[0]), __uint_as_float(x[1])), pack_bf16x2(__uint_as_float(x[2]), __uint_as_float(x[3])),
-                                          pack_bf16x2(__uint_as_float(x[4]), __uint_as_float(x[5])), pack_bf16x2(__uint_as_float(x[6]), __uint_as_float(x[7])));
+                mbar_wait(&acc_full[buf], (n >> 1) & 1, ab, 30);
+                tc_fence_after_sync();
+#pragma unroll 1
+                for (int c0 = h * (BN / 2); c0 < (h + 1) * (BN / 2); c0 += 64) {
+                    const int col = q.n0 + c0;
+                    uint32_t v[2][32];
+                    tmem_ld_x32(tmem + buf * BN + c0 + lane_base, v[0]);
+                    tmem_ld_x32(tmem + buf * BN + c0 + 32 + lane_base, v[1]);
+                    tmem_wait_ld();
+                    if (c0 + 64 == (h + 1) * (BN / 2)) {
+                        // every column of the accumulator is in registers: hand it back to the MMA warp
+                        tc_fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster_relaxed(free_bar[buf]);
                     }
-                    stage_out(mc, q.partial, col, row, w);
-                } else {
+                    if (row >= k.M || col >= k.N) continue;
+                    if (with_bias) {
+                        const float2 bc = c0 & 64 ? bias1 : bias0;
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
+                        for (int e = 0; e < 64; ++e)
+                            v[e >> 5][e & 31] = __float_as_uint(__uint_as_float(v[e >> 5][e & 31]) + __shfl_sync(0xffffffffu, e & 1 ? bc.y : bc.x, e >> 1));
+                    }
+                    uint4 w[8];
+                    if (!f32_out) {
 #pragma unroll
-                        for (int c = 0; c < 8; ++c) w[c] = make_uint4(v[half][4 * c], v[half][4 * c + 1], v[half][4 * c + 2], v[half][4 * c + 3]);
-                        if (col + 32 * half < k.N) stage_out(mc, true, col + 32 * half, row, w);
+                        for (int c = 0; c < 8; ++c) {
+                            const uint32_t* x = &v[c >> 2][(c & 3) * 8];
+                            w[c] = make_uint4(pack_bf16x2(__uint_as_float(x[0]), __uint_as_float(x[1])), pack_bf16x2(__uint_as_float(x[2]), __uint_as_float(x[3])),
+                                              pack_bf16x2(__uint_as_float(x[4]), __uint_as_float(x[5])), pack_bf16x2(__uint_as_float(x[6]), __uint_as_float(x[7])));
+                        }
+                        stage_out(mc, q.partial, col, row, w);
+                    } else {
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) w[c] = make_uint4(v[half][4 * c], v[half][4 * c + 1], v[half][4 * c + 2], v[half][4 * c + 3]);
+                            if (col + 32 * half < k.N) stage_out(mc, true, col + 32 * half, row, w);
+                        }
                     }
                 }
+            }
+        } else {
+            // Task 0 with its fused form, task 1 (if there is one) as above.  What the form reads beside the accumulator (aux: 32 rows x 64 columns
+            // at a time) is fetched by the TMA unit into the warp's second tile one step ahead: the first step's under the wait for the tile,
+            // or under the last step of the tile before.
+            uint8_t* aux = smem + SM::OFF_AUX + warp * TR::STAGING_BYTES;
+            const bool has_aux = EPI == kEpiResidual || EPI == kEpiSlope || prm.has_aux;
+            const int colf = h * (BN / 2);
+            uint32_t aux_n = 0;
+            auto request_aux = [&](const GemmPart& p, int c0) {
+                const int row = p.m0 + static_cast<int>(rank) * TR::CM + row0, col = p.n0 + c0;
+                if (has_aux && p.task == 0 && row < prm.t[0].M && col < prm.t[0].N && lane == 0) {
+                    mbar_arrive_expect_tx(&aux_full[warp], TR::STAGING_BYTES);
+                    tma_load_3d(aux, &maps.aux, &aux_full[warp], col, row, 0);
+                }
+            };
+            // a copy out of either tile: `pending` = 1 where the two tiles take turns (the other one's copy may still be reading)
+            auto stage_to = [&](uint8_t* tile, int pending, const CUtensorMap* m, int col, int row, const uint4 (&w)[8]) {
+                if (lane == 0) {
+                    if (pending) tma_store_wait_read<1>();
+                    else tma_store_wait_read_all();
+                }
+                __syncwarp();
+#pragma unroll
+                for (int c = 0; c < 8; ++c) st_shared_sw128(tile, lane, c, w[c]);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    tma_store_3d(m, tile, col, row, 0);
+                    tma_store_commit();
+                }
+            };
+            bool more = walk.next(q);
+            if (more) request_aux(q, colf);
+            for (; more; ++n) {
+                const GemmTask& k = prm.t[q.task];
+                const bool fused = q.task == 0;
+                const uint32_t buf = n & 1;
+                const int row = q.m0 + static_cast<int>(rank) * TR::CM + row0;
+                const bool with_bias = prm.bias && fused;
+                float2 bias0 = make_float2(0.f, 0.f), bias1 = bias0;
+                if (with_bias) {
+                    const int col = q.n0 + colf + 2 * lane;
+                    if (col < k.N) bias0 = load_bias2(prm, col);
+                    if (col + 64 < k.N) bias1 = load_bias2(prm, col + 64);
+                }
+                mbar_wait(&acc_full[buf], (n >> 1) & 1, ab, 30);
+                tc_fence_after_sync();
+                GemmPart ahead;
+                bool more_ahead = false;
+#pragma unroll 1
+                for (int c0 = colf; c0 < colf + BN / 2; c0 += 64) {
+                    const int col = q.n0 + c0;
+                    const bool inside = row < k.M && col < k.N, last = c0 != colf;
+                    uint4 a[8];
+                    if (has_aux && fused && inside) {
+                        mbar_wait(&aux_full[warp], aux_n & 1, ab, 31);
+                        ++aux_n;
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) a[c] = *reinterpret_cast<const uint4*>(aux + sw128_offset(lane, c));
+                    }
+                    uint32_t v[2][32];
+                    tmem_ld_x32(tmem + buf * BN + c0 + lane_base, v[0]);
+                    tmem_ld_x32(tmem + buf * BN + c0 + 32 + lane_base, v[1]);
+                    tmem_wait_ld();
+                    if (last) {
+                        tc_fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster_relaxed(free_bar[buf]);
+                        more_ahead = walk.next(ahead);
+                        if (more_ahead) request_aux(ahead, colf);
+                    } else {
+                        __syncwarp();          // every lane has read the aux tile
+                        request_aux(q, c0 + 64);
+                    }
+                    if (!inside) continue;
+                    uint4 w[8];
+                    if (!fused) {
+                        const bool f32_out = q.partial && prm.split == kPartReduceF32;
+                        const CUtensorMap* mc = q.partial ? &maps.sum : &maps.c[1];
+                        if (!f32_out) {
+                            pack_tile(v, w);
+                            stage_out(mc, q.partial, col, row, w);
+                        } else {
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                                for (int c = 0; c < 8; ++c) w[c] = make_uint4(v[half][4 * c], v[half][4 * c + 1], v[half][4 * c + 2], v[half][4 * c + 3]);
+                                if (col + 32 * half < k.N) stage_out(mc, true, col + 32 * half, row, w);
+                            }
+                        }
+                        continue;
+                    }
+                    if (with_bias) {
+                        const float2 bc = last ? bias1 : bias0;
+#pragma unroll
+                        for (int e = 0; e < 64; ++e)
+                            v[e >> 5][e & 31] = __float_as_uint(__uint_as_float(v[e >> 5][e & 31]) + __shfl_sync(0xffffffffu, e & 1 ? bc.y : bc.x, e >> 1));
+                    }
+                    if constexpr (EPI == kEpiGelu) {
+                        if (prm.write_pre) {
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) {
+                                const uint32_t* x = &v[c >> 2][(c & 3) * 8];
+                                w[c] = make_uint4(pack_preact2(__uint_as_float(x[0]), __uint_as_float(x[1])), pack_preact2(__uint_as_float(x[2]), __uint_as_float(x[3])),
+                                                  pack_preact2(__uint_as_float(x[4]), __uint_as_float(x[5])), pack_preact2(__uint_as_float(x[6]), __uint_as_float(x[7])));
+                            }
+                            stage_to(stage, !has_aux, &maps.pre, col, row, w);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 64; ++e) v[e >> 5][e & 31] = __float_as_uint(gelu(__uint_as_float(v[e >> 5][e & 31])));
+                    }
+                    if (EPI == kEpiSlope || has_aux) {
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) {
+                            const uint32_t aw[4] = {a[c].x, a[c].y, a[c].z, a[c].w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                uint32_t* x = &v[c >> 2][(c & 3) * 8 + 2 * e];
+                                const float2 f = EPI == kEpiSlope ? unpack_half2(aw[e]) : unpack_bf16x2(aw[e]);
+                                x[0] = __float_as_uint(EPI == kEpiSlope ? __uint_as_float(x[0]) * gelu_slope(f.x) : __uint_as_float(x[0]) + f.x);
+                                x[1] = __float_as_uint(EPI == kEpiSlope ? __uint_as_float(x[1]) * gelu_slope(f.y) : __uint_as_float(x[1]) + f.y);
+                            }
+                        }
+                    }
+                    pack_tile(v, w);
+                    // z and gelu(z) go out of a tile each, unless the second one holds the residual
+                    const bool two = EPI == kEpiGelu && !has_aux && prm.write_pre;
+                    stage_to(two ? aux : stage, two, &maps.c[0], col, row, w);
+                    if constexpr (EPI == kEpiSlope) {
+                        // two columns a lane, over the 32 rows of the staged tile (a row at a time: 128 bytes, no bank twice); rows past M are zeros
+                        if (prm.colsum) {
+                            float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+                            for (int r = 0; r < 32; ++r) {
+                                const float2 f = unpack_bf16x2(*reinterpret_cast<const uint32_t*>(stage + sw128_offset(r, lane >> 2) + (lane & 3) * 4));
+                                sum.x += f.x;
+                                sum.y += f.y;
+                            }
+                            if (col + 2 * lane < k.N) *reinterpret_cast<float2*>(prm.colsum + static_cast<long>(row >> 5) * k.N + col + 2 * lane) = sum;
+                        }
+                    }
+                }
+                more = more_ahead;
+                q = ahead;
             }
         }
         if (lane == 0) tma_store_wait_read_all();    // the CTA may leave once its shared memory has been read; the writes complete on their own
@@ -341,14 +548,18 @@ gemm_bf16_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ 
 // the broadcast add, src/inferno/core/broadcastops.cpp) as one row of partial sums per row slab, and the zeroing of the
 // fp32 accumulation workspace.  Block (x, y): 256 columns, rows y * rows_per_block ...; a warp reads 512 contiguous bytes
 // of a row (16 bytes a lane) and keeps four rows in flight.  HBM-bound: one read of dY.
+// GELU: x is dy, `pre` the kept z; dz = dy gelu'(z) is written for the two products that follow, and its columns, not dy's, are summed
+// (before they are rounded): two reads and a write.
 constexpr int kColsumCols = 256, kMaxColsumSlabs = 128;
-__global__ void __launch_bounds__(256) linear_prep_kernel(const __nv_bfloat16* __restrict__ x, float* __restrict__ part, int M, int N, int rows_per_block,
-                                                          int atomic, float4* __restrict__ zero, long zero4) {
+template <bool GELU>
+__global__ void __launch_bounds__(256) linear_prep_kernel(const __nv_bfloat16* __restrict__ x, const __half* __restrict__ pre, __nv_bfloat16* __restrict__ dz,
+                                                          float* __restrict__ part, int M, int N, int rows_per_block, int atomic, float4* __restrict__ zero,
+                                                          long zero4) {
     pdl_wait();
     pdl_trigger();
     const long zstep = static_cast<long>(gridDim.x) * gridDim.y * blockDim.x;
     for (long i = (static_cast<long>(blockIdx.y) * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x; i < zero4; i += zstep) zero[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (!part) return;
+    if (!GELU && !part) return;
     __shared__ float sums[8][kColsumCols + 4];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int col = blockIdx.x * kColsumCols + lane * 8;
@@ -362,7 +573,35 @@ __global__ void __launch_bounds__(256) linear_prep_kernel(const __nv_bfloat16* _
             acc[2 * e + 1] += __uint_as_float(w[e] & 0xffff0000u);
         }
     };
-    if (col < N) {
+    if (GELU && col < N) {
+        const uint4* src = reinterpret_cast<const uint4*>(x + col);
+        const uint4* zsrc = reinterpret_cast<const uint4*>(pre + col);
+        uint4* dst = reinterpret_cast<uint4*>(dz + col);
+        const long pitch = N / 8;
+        auto slopes = [&](long at, const uint4& g4, const uint4& z4) {
+            const uint32_t g[4] = {g4.x, g4.y, g4.z, g4.w}, z[4] = {z4.x, z4.y, z4.z, z4.w};
+            uint32_t o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = unpack_half2(z[e]), d = unpack_bf16x2(g[e]);
+                const float a = d.x * gelu_slope(f.x), b = d.y * gelu_slope(f.y);
+                acc[2 * e] += a;
+                acc[2 * e + 1] += b;
+                o[e] = pack_bf16x2(a, b);
+            }
+            dst[at] = make_uint4(o[0], o[1], o[2], o[3]);
+        };
+        int row = blockIdx.y * rows_per_block + warp;
+        for (; row + 8 < row1; row += 16) {
+            const long at = row * pitch, at1 = at + 8 * pitch;
+            const uint4 g0 = src[at], z0 = zsrc[at], g1 = src[at1], z1 = zsrc[at1];
+            slopes(at, g0, z0);
+            slopes(at1, g1, z1);
+        }
+        for (; row < row1; row += 8) slopes(row * pitch, src[row * pitch], zsrc[row * pitch]);
+    }
+    if (!part) return;
+    if (!GELU && col < N) {
         const uint4* src = reinterpret_cast<const uint4*>(x + col);
         const long pitch = N / 8;
         int row = blockIdx.y * rows_per_block + warp;
@@ -388,33 +627,97 @@ __global__ void __launch_bounds__(256) linear_prep_kernel(const __nv_bfloat16* _
     }
 }
 
-// The backward's helper behind the GEMMs: dW = bf16(fp32 accumulator), 8 elements per thread, and db = the sum of the row
-// slabs' partial sums, in a fixed order.  The first `db_blocks` blocks do db, 32 columns each (eight threads a column).
+// The backward's helper behind the GEMMs, for up to two projections: dW = bf16(fp32 accumulator), 8 elements per thread, and db = the sum
+// of the row slabs' partial sums, in a fixed order.  The first `db_blocks` blocks of a job do its db, 32 columns each (eight threads a column).
 constexpr int kFinishCols = 32;
-__global__ void __launch_bounds__(256) linear_finish_kernel(const float4* __restrict__ acc, uint4* __restrict__ out, long n8, const float* __restrict__ part,
-                                                            int slabs, int N, void* __restrict__ db, int db_bf16, int db_blocks) {
+struct FinishJob {
+    const float4* acc;     // or null
+    uint4* out;
+    long n8;
+    const float* part;     // [slabs][N]
+    int slabs, N;
+    void* db;              // or null
+    int db_bf16, db_blocks;
+};
+struct FinishJobs {
+    FinishJob j[2];
+};
+__global__ void __launch_bounds__(256) linear_finish_kernel(const __grid_constant__ FinishJobs jobs) {
     pdl_wait();
     pdl_trigger();
-    if (static_cast<int>(blockIdx.x) < db_blocks) {
+    const int all_db = jobs.j[0].db_blocks + jobs.j[1].db_blocks;
+    if (static_cast<int>(blockIdx.x) < all_db) {
+        const bool second = static_cast<int>(blockIdx.x) >= jobs.j[0].db_blocks;
+        const FinishJob& k = jobs.j[second];
         __shared__ float sums[8][kFinishCols];
-        const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5, c = blockIdx.x * kFinishCols + lane;
+        const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5, c = (blockIdx.x - (second ? jobs.j[0].db_blocks : 0)) * kFinishCols + lane;
         float s = 0.f;
-        if (c < N)
-            for (int j = grp; j < slabs; j += 8) s += part[static_cast<long>(j) * N + c];
+        if (c < k.N)
+#pragma unroll 4
+            for (int j = grp; j < k.slabs; j += 8) s += k.part[static_cast<long>(j) * k.N + c];
         sums[grp][lane] = s;
         __syncthreads();
-        if (grp == 0 && c < N) {
+        if (grp == 0 && c < k.N) {
 #pragma unroll
             for (int g = 1; g < 8; ++g) s += sums[g][lane];
-            if (db_bf16) static_cast<__nv_bfloat16*>(db)[c] = __float2bfloat16(s);
-            else static_cast<float*>(db)[c] = s;
+            if (k.db_bf16) static_cast<__nv_bfloat16*>(k.db)[c] = __float2bfloat16(s);
+            else static_cast<float*>(k.db)[c] = s;
         }
         return;
     }
-    const long step = static_cast<long>(gridDim.x - db_blocks) * blockDim.x;
-    for (long i = (static_cast<long>(blockIdx.x) - db_blocks) * blockDim.x + threadIdx.x; i < n8; i += step) {
-        const float4 a = acc[2 * i], b = acc[2 * i + 1];
-        out[i] = make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w), pack_bf16x2(b.x, b.y), pack_bf16x2(b.z, b.w));
+    const long step = static_cast<long>(gridDim.x - all_db) * blockDim.x;
+    const long first = (static_cast<long>(blockIdx.x) - all_db) * blockDim.x + threadIdx.x;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const FinishJob& k = jobs.j[q];
+        if (!k.acc) continue;
+        for (long i = first; i < k.n8; i += step) {
+            const float4 a = k.acc[2 * i], b = k.acc[2 * i + 1];
+            k.out[i] = make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w), pack_bf16x2(b.x, b.y), pack_bf16x2(b.z, b.w));
+        }
+    }
+}
+
+// Behind a forward product that was cut along K: the epilogue on its fp32 sums, 8 elements per thread.
+struct FusedFinish {
+    const float4* acc;
+    const void* bias;
+    int bias_bf16, gelu;
+    const uint4* residual;      // or null
+    uint4* pre;                 // fp16, or null
+    uint4* y;
+    long n8;
+    int N;
+};
+__global__ void __launch_bounds__(256) linear_fused_finish_kernel(const FusedFinish p) {
+    pdl_wait();
+    pdl_trigger();
+    const long step = static_cast<long>(gridDim.x) * blockDim.x;
+    for (long i = static_cast<long>(blockIdx.x) * blockDim.x + threadIdx.x; i < p.n8; i += step) {
+        const float4 a = p.acc[2 * i], b = p.acc[2 * i + 1];
+        float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        const int col = static_cast<int>(i * 8 % p.N);
+        if (p.bias) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                v[e] += p.bias_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[col + e]) : static_cast<const float*>(p.bias)[col + e];
+        }
+        if (p.pre) p.pre[i] = make_uint4(pack_preact2(v[0], v[1]), pack_preact2(v[2], v[3]), pack_preact2(v[4], v[5]), pack_preact2(v[6], v[7]));
+        if (p.gelu) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = gelu(v[e]);
+        }
+        if (p.residual) {
+            const uint4 r = p.residual[i];
+            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = unpack_bf16x2(w[e]);
+                v[2 * e] += f.x;
+                v[2 * e + 1] += f.y;
+            }
+        }
+        p.y[i] = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
     }
 }
 

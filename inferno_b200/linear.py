@@ -4,6 +4,10 @@
 (src/inferno/modules/linear.cpp:19-106); its backward is MMBackward + the bias' sum_to_shape
 (src/inferno/gradfn/mmbackward.cpp:36-98).  Here both directions run on the tcgen05 GEMM of
 ``csrc/linear_gemm.cuh`` through the C ABI (bf16 tensors, a bias of either type, fp32 accumulation).
+
+``fused_linear`` adds the activation and the residual that follow a projection in a transformer block to its epilogue, and
+``feed_forward`` joins two of them (InfernoApp/main.cpp:844-909: ff1 -> gelu -> ff2 -> + x; the reference's gelu is the tanh form,
+src/inferno/functional/gelu_kernels.h:6-14).
 """
 from __future__ import annotations
 
@@ -33,17 +37,63 @@ class LinearFunction:
         return _capi.host().linear(x, w, bias)
 
 
-class Linear(torch.nn.Module):
-    """``x @ W + b`` with W stored [in, out] like the reference's Linear; bf16 weight, fp32-accumulated GEMM."""
+def fused_linear_forward(x, w, bias=None, activation: str | None = None, residual=None, keep_preact: bool = False):
+    """(y, preact) with y = act(x @ w + bias) + residual; activation is None or "gelu" (the tanh form), residual has y's shape.
 
-    def __init__(self, in_features: int, out_features: int, bias: bool = True):
+    preact is what the backward needs of the pre-activation: fp16, limited to +-16, beyond which the derivative is 0 or 1.
+    None without an activation, or when it is not kept."""
+    return _capi.host().fused_linear_forward(x, w, bias, activation, residual, keep_preact)
+
+
+def fused_linear_backward(x, w, dy, preact=None, activation: str | None = None, need_dx=True, need_dw=True, need_db=True):
+    """(dx, dw, db) of ``fused_linear_forward``; db is fp32; what is not needed comes back as None.  The residual's gradient is dy.
+
+    dw is added up as in ``linear_backward``; dx and db repeat bit for bit."""
+    return _capi.host().fused_linear_backward(x, w, dy, preact, activation, need_dx, need_dw, need_db)
+
+
+def fused_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
+                 residual: torch.Tensor | None = None) -> torch.Tensor:
+    """``act(x @ w + bias) + residual`` in one kernel; differentiable (backward node in csrc/host_ops.cpp).  bf16 tensors, a bias of
+    either type; in_features and out_features are multiples of 8, the number of rows is free."""
+    return _capi.host().fused_linear(x, w, bias, activation, residual)
+
+
+def feed_forward(x: torch.Tensor, w1: torch.Tensor, b1: torch.Tensor | None, w2: torch.Tensor, b2: torch.Tensor | None,
+                 residual: torch.Tensor | None = None) -> torch.Tensor:
+    """``gelu(x @ w1 + b1) @ w2 + b2 + residual``; differentiable.  w1 [C, H], w2 [H, C]; biases and residual may be None.
+
+    Two kernels forward; backward the gradient of the hidden layer is multiplied by gelu' in the epilogue of the product that
+    makes it.  The hidden layer is rounded to bf16 between the products, and so is its gradient."""
+    return _capi.host().feed_forward(x, w1, b1, w2, b2, residual)
+
+
+class Linear(torch.nn.Module):
+    """``x @ W + b`` with W stored [in, out] like the reference's Linear; bf16 weight, fp32-accumulated GEMM.
+    With an activation ("gelu") or a residual given to forward, these are part of the kernel's epilogue."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, activation: str | None = None):
         super().__init__()
+        self.activation = activation
         self.weight = torch.nn.Parameter(torch.empty(in_features, out_features))
         self.bias = torch.nn.Parameter(torch.zeros(out_features)) if bias else None
         torch.nn.init.normal_(self.weight, 0.0, 0.02)
 
-    def forward(self, x):
-        return _capi.host().linear(x, self.weight, self.bias)
+    def forward(self, x, residual=None):
+        if self.activation is None and residual is None:
+            return _capi.host().linear(x, self.weight, self.bias)
+        return fused_linear(x, self.weight, self.bias, self.activation, residual)
+
+
+class FeedForward(torch.nn.Module):
+    """``feed_forward`` with its two projections as ``ff1`` and ``ff2``."""
+
+    def __init__(self, features: int, hidden: int, bias: bool = True):
+        super().__init__()
+        self.ff1, self.ff2 = Linear(features, hidden, bias), Linear(hidden, features, bias)
+
+    def forward(self, x, residual=None):
+        return feed_forward(x, self.ff1.weight, self.ff1.bias, self.ff2.weight, self.ff2.bias, residual)
 
 
 def _time_shape(M: int, K: int, N: int, iters: int = 20):
