@@ -750,7 +750,7 @@ constexpr int kLnMaxChunks = 4;        // 16-byte chunks of a row that a thread 
 // Threads per row: as few as hold the row in four chunks each.  0: the row is too long.
 int ln_threads_per_row(int C, int dtype) {
     const long bytes = static_cast<long>(C) * (dtype == IB200_DTYPE_F32 ? 4 : 2);
-    for (int tpr : {32, 128, 512})
+    for (int tpr : {32, 128, 256, 512})
         if (bytes <= 16L * kLnMaxChunks * tpr) return tpr;
     return 0;
 }
@@ -761,8 +761,9 @@ int ln_bwd_blocks(int M, int C, int dtype, int sms) {
 
 template <class S>
 int launch_ln(bool backward, const LnRows& p, int blocks, cudaStream_t stream) {
-    return backward ? launch_pdl<ln_bwd_kernel<S>>(blocks, S::THREADS, 0, stream, p)
-                    : launch_pdl<ln_fwd_kernel<S>>((p.M - 1) / S::ROWS + 1, S::THREADS, 0, stream, p);
+    if (!allow_smem<ln_bwd_kernel<S>>(S::BWD_SMEM) || !allow_smem<ln_fwd_kernel<S>>(S::FWD_SMEM)) return IB200_ERR_CUDA;
+    return backward ? launch_pdl<ln_bwd_kernel<S>>(blocks, S::THREADS, S::BWD_SMEM, stream, p)
+                    : launch_pdl<ln_fwd_kernel<S>>(std::min((p.M - 1) / S::ROWS + 1, S::FWD_BLOCKS * device_info()->sms), S::THREADS, S::FWD_SMEM, stream, p);
 }
 template <class T, int TPR>
 int launch_ln_row(bool aligned, bool backward, const LnRows& p, int blocks, cudaStream_t stream) {
@@ -782,6 +783,7 @@ int launch_ln_type(int dtype, bool backward, const LnRows& p, int blocks, cudaSt
     switch (ln_threads_per_row(p.C, dtype)) {
         case 32: return launch_ln_row<T, 32>(aligned, backward, p, blocks, stream);
         case 128: return launch_ln_row<T, 128>(aligned, backward, p, blocks, stream);
+        case 256: return launch_ln_row<T, 256>(aligned, backward, p, blocks, stream);
         default: return launch_ln_row<T, 512>(aligned, backward, p, blocks, stream);
     }
 }

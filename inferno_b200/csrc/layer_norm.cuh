@@ -10,7 +10,7 @@
 // (src/inferno/cuda/cudalayernorm.cu:16-160, 212-400; modules: src/inferno/modules/layernorm.cpp:25-98).
 //
 // Memory-bound: a row is read once into registers, and everything is computed from there, so the variance is the sum of squared
-// differences from the mean and not a difference of two sums.  A row belongs to 32, 128 or 512 threads (LnShape), each of which holds
+// differences from the mean and not a difference of two sums.  A row belongs to 32, 128, 256 or 512 threads (LnShape), each of which holds
 // up to four 16-byte chunks of it: a row of one warp needs no barrier.  The backward's threads keep their columns from row to row and
 // sum dw and db in registers; a block's sums meet in the workspace, which ln_finish_kernel adds up in a fixed order.  All sums are
 // fp32; the only rounding to fewer bits is that of the results.
@@ -49,7 +49,10 @@ struct LnShape {
     static constexpr bool ALIGNED = ALIGNED_;
     static constexpr int THREADS = TPR_ == 32 ? 256 : TPR_, ROWS = THREADS / TPR_;      // per block
     static constexpr int CHUNK_COLS = TPR_ * VEC;                                       // columns of one chunk of all threads
-    static constexpr int BWD_BLOCKS = 512 / THREADS;                                    // of the backward, resident per SM
+    static constexpr int FWD_BLOCKS = TPR_ == 512 ? 1 : (NV_ < 4 ? 768 : 512) / THREADS, BWD_BLOCKS = 512 / THREADS;      // resident per SM
+    static constexpr int FWD_STAGES = 4, BWD_STAGES = 3;                                // rows of a thread's ring
+    static constexpr int FWD_SMEM = ALIGNED_ ? FWD_STAGES * NV_ * THREADS * 16 : 0;
+    static constexpr int BWD_SMEM = ALIGNED_ ? BWD_STAGES * 2 * NV_ * THREADS * 16 : 0;
 };
 
 __device__ __forceinline__ float ln_to_float(float v) { return v; }
@@ -62,81 +65,69 @@ template <class S>
 __device__ __forceinline__ int ln_col(int v, int e, int t) {
     return S::ALIGNED ? (v * S::TPR + t) * S::VEC + e : v * S::CHUNK_COLS + e * S::TPR + t;
 }
-__device__ __forceinline__ void ln_unpack(const uint4& u, float (&f)[8]) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        f[2 * e] = __uint_as_float(w[e] << 16);
-        f[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-    }
-}
-__device__ __forceinline__ void ln_unpack(const uint4& u, float (&f)[4]) {
-    f[0] = __uint_as_float(u.x);
-    f[1] = __uint_as_float(u.y);
-    f[2] = __uint_as_float(u.z);
-    f[3] = __uint_as_float(u.w);
-}
-// One chunk of a row; zeros past its end.
+// A chunk in registers: pairs of fp32, for the packed arithmetic (two lanes an instruction: with single ones the issue slots, not the memory, bound
+// the forward).
 template <class S>
-__device__ __forceinline__ void ln_load(const typename S::T* row, int v, int t, int C, float (&f)[S::VEC]) {
-    if constexpr (S::ALIGNED) {
-        const int c = ln_col<S>(v, 0, t);
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (c < C) u = *reinterpret_cast<const uint4*>(row + c);
-        ln_unpack(u, f);
-    } else {
+struct LnChunk {
+    uint64_t f[S::VEC / 2];
+};
+__device__ __forceinline__ uint64_t ln_pair_bf16(uint32_t w) { return pack_f32x2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+__device__ __forceinline__ void ln_unpack(const uint4& u, uint64_t (&f)[4]) {
+    f[0] = ln_pair_bf16(u.x);
+    f[1] = ln_pair_bf16(u.y);
+    f[2] = ln_pair_bf16(u.z);
+    f[3] = ln_pair_bf16(u.w);
+}
+__device__ __forceinline__ void ln_unpack(const uint4& u, uint64_t (&f)[2]) {
+    f[0] = pack_f32x2(__uint_as_float(u.x), __uint_as_float(u.y));
+    f[1] = pack_f32x2(__uint_as_float(u.z), __uint_as_float(u.w));
+}
+// Elements of p one by one, `none` past the row's end (rows that do not begin on 16 bytes).
+template <class S, class P>
+__device__ __forceinline__ void ln_gather(const P* p, float none, int v, int t, int C, LnChunk<S>& k) {
 #pragma unroll
-        for (int e = 0; e < S::VEC; ++e) {
-            const int c = ln_col<S>(v, e, t);
-            f[e] = c < C ? ln_to_float(row[c]) : 0.f;
-        }
+    for (int e = 0; e < S::VEC; e += 2) {
+        const int c0 = ln_col<S>(v, e, t), c1 = ln_col<S>(v, e + 1, t);
+        k.f[e / 2] = pack_f32x2(c0 < C ? ln_to_float(p[c0]) : none, c1 < C ? ln_to_float(p[c1]) : none);
     }
 }
-// The same columns of weight or bias.
-template <class S, class P>
-__device__ __forceinline__ void ln_load_param_as(const P* p, int v, int t, int C, float (&f)[S::VEC]) {
+// The same columns of weight or bias: after the first row they come from L1.
+template <class S>
+__device__ __forceinline__ void ln_load_param(const void* p, int bf16, float none, int v, int t, int C, LnChunk<S>& k) {
     if constexpr (S::ALIGNED) {
         const int c = ln_col<S>(v, 0, t);
+        if (!p || c >= C) {
 #pragma unroll
-        for (int e = 0; e < S::VEC; ++e) f[e] = 0.f;
-        if (c >= C) return;
-        if constexpr (sizeof(P) == 4) {
+            for (int i = 0; i < S::VEC / 2; ++i) k.f[i] = pack_f32x2(none, none);
+        } else if (bf16) {
 #pragma unroll
             for (int q = 0; q < S::VEC / 4; ++q) {
-                const float4 u = *reinterpret_cast<const float4*>(p + c + 4 * q);
-                f[4 * q] = u.x; f[4 * q + 1] = u.y; f[4 * q + 2] = u.z; f[4 * q + 3] = u.w;
+                const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p) + c + 4 * q);
+                k.f[2 * q] = ln_pair_bf16(u.x);
+                k.f[2 * q + 1] = ln_pair_bf16(u.y);
             }
         } else {
 #pragma unroll
             for (int q = 0; q < S::VEC / 4; ++q) {
-                const uint2 u = *reinterpret_cast<const uint2*>(p + c + 4 * q);
-                f[4 * q] = __uint_as_float(u.x << 16);
-                f[4 * q + 1] = __uint_as_float(u.x & 0xffff0000u);
-                f[4 * q + 2] = __uint_as_float(u.y << 16);
-                f[4 * q + 3] = __uint_as_float(u.y & 0xffff0000u);
+                const float4 u = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + c + 4 * q);
+                k.f[2 * q] = pack_f32x2(u.x, u.y);
+                k.f[2 * q + 1] = pack_f32x2(u.z, u.w);
             }
         }
-    } else {
+    } else if (!p) {
 #pragma unroll
-        for (int e = 0; e < S::VEC; ++e) {
-            const int c = ln_col<S>(v, e, t);
-            f[e] = c < C ? ln_to_float(p[c]) : 0.f;
-        }
-    }
-}
-template <class S>
-__device__ __forceinline__ void ln_load_param(const void* p, int bf16, float none, int v, int t, int C, float (&f)[S::VEC]) {
-    if (!p) {
-#pragma unroll
-        for (int e = 0; e < S::VEC; ++e) f[e] = none;
+        for (int i = 0; i < S::VEC / 2; ++i) k.f[i] = pack_f32x2(none, none);
     } else if (bf16) {
-        ln_load_param_as<S>(static_cast<const __nv_bfloat16*>(p), v, t, C, f);
+        ln_gather<S>(static_cast<const __nv_bfloat16*>(p), none, v, t, C, k);
     } else {
-        ln_load_param_as<S>(static_cast<const float*>(p), v, t, C, f);
+        ln_gather<S>(static_cast<const float*>(p), none, v, t, C, k);
     }
 }
 template <class S>
-__device__ __forceinline__ void ln_store(typename S::T* row, int v, int t, int C, const float (&f)[S::VEC]) {
+__device__ __forceinline__ void ln_store(typename S::T* row, int v, int t, int C, const LnChunk<S>& k) {
+    float f[S::VEC];
+#pragma unroll
+    for (int i = 0; i < S::VEC / 2; ++i) unpack_f32x2(k.f[i], f[2 * i], f[2 * i + 1]);
     if constexpr (S::ALIGNED) {
         const int c = ln_col<S>(v, 0, t);
         if (c >= C) return;
@@ -152,15 +143,20 @@ __device__ __forceinline__ void ln_store(typename S::T* row, int v, int t, int C
         }
     }
 }
+__device__ __forceinline__ float ln_pair_sum(uint64_t p) {
+    float a, b;
+    unpack_f32x2(p, a, b);
+    return a + b;
+}
 
-// Sums of a and b over the threads of a row.  `turn` alternates between two sets of slots, so that one barrier per sum is enough: a slot
+// Sums of a (and b) over the threads of a row.  `turn` alternates between two sets of slots, so that one barrier per sum is enough: a slot
 // is written again only after the next sum's barrier, which every thread reaches after it has read.
-template <class S>
+template <class S, bool BOTH>
 __device__ __forceinline__ float2 ln_row_sum(float a, float b, float2 (*slots)[16], int turn) {
 #pragma unroll
     for (int m = 16; m > 0; m >>= 1) {
         a += __shfl_xor_sync(0xffffffffu, a, m);
-        b += __shfl_xor_sync(0xffffffffu, b, m);
+        if (BOTH) b += __shfl_xor_sync(0xffffffffu, b, m);
     }
     if constexpr (S::WARPS > 1) {
         float2* s = slots[turn & 1];
@@ -170,116 +166,220 @@ __device__ __forceinline__ float2 ln_row_sum(float a, float b, float2 (*slots)[1
 #pragma unroll
         for (int w = 0; w < S::WARPS; ++w) {
             a += s[w].x;
-            b += s[w].y;
+            if (BOTH) b += s[w].y;
         }
     }
     return make_float2(a, b);
 }
 
+// ---- a thread's ring in shared memory: its own chunks of the rows to come ----
+// Filled by 16-byte asynchronous copies and read by the thread that asked for them, so that waiting for the thread's own copies is all the
+// synchronisation there is.  [stage][chunk][thread]: a warp's accesses run together.
+__device__ __forceinline__ void ln_copy_async(uint4* dst, const void* src, bool inside) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(inside ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void ln_copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void ln_copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
 template <class S>
-__global__ void __launch_bounds__(S::THREADS) ln_fwd_kernel(const LnRows p) {
+__device__ __forceinline__ void ln_request(uint4* slots, const typename S::T* row, int t, int C) {
+#pragma unroll
+    for (int v = 0; v < S::NV; ++v) {
+        const int c = ln_col<S>(v, 0, t);
+        ln_copy_async(slots + v * S::THREADS + threadIdx.x, row + (c < C ? c : 0), c < C);
+    }
+}
+
+template <class S>
+__global__ void __launch_bounds__(S::THREADS, S::FWD_BLOCKS) ln_fwd_kernel(const LnRows p) {
     using T = typename S::T;
+    constexpr int ST = S::FWD_STAGES;
+    extern __shared__ uint4 ring[];
     __shared__ float2 slots[2][16];
     pdl_wait();
     pdl_trigger();
     const int t = threadIdx.x % S::TPR;
-    const int r = blockIdx.x * S::ROWS + threadIdx.x / S::TPR;
-    if (r >= p.M) return;                  // a whole row's threads
-    const T* row = static_cast<const T*>(p.x) + static_cast<long>(r) * p.x_pitch;
-    float x[S::NV][S::VEC];
-    float s = 0.f;
+    const long first = static_cast<long>(blockIdx.x) * S::ROWS + threadIdx.x / S::TPR, step = static_cast<long>(gridDim.x) * S::ROWS;
+    const T* x0 = static_cast<const T*>(p.x);
+    if constexpr (S::ALIGNED) {
 #pragma unroll
-    for (int v = 0; v < S::NV; ++v) {
-        ln_load<S>(row, v, t, p.C, x[v]);
-#pragma unroll
-        for (int e = 0; e < S::VEC; ++e) s += x[v][e];
+        for (int s = 0; s < ST - 1; ++s) {
+            const long r = first + s * step;
+            if (r < p.M) ln_request<S>(ring + s * S::NV * S::THREADS, x0 + r * p.x_pitch, t, p.C);
+            ln_copy_commit();
+        }
     }
     const float inv = 1.f / static_cast<float>(p.C);
-    const float mean = ln_row_sum<S>(s, 0.f, slots, 0).x * inv;
-    float q = 0.f, left = 0.f;
+    int stage = 0;
+    for (long r = first; r < p.M; r += step) {
+        LnChunk<S> x[S::NV];
+        if constexpr (S::ALIGNED) {
+            const long ra = r + (ST - 1) * step;
+            const int sa = stage == 0 ? ST - 1 : stage - 1;          // the slot that was read last
+            if (ra < p.M) ln_request<S>(ring + sa * S::NV * S::THREADS, x0 + ra * p.x_pitch, t, p.C);
+            ln_copy_commit();
+            ln_copy_wait<ST - 1>();
 #pragma unroll
-    for (int v = 0; v < S::NV; ++v)
+            for (int v = 0; v < S::NV; ++v) ln_unpack(ring[(stage * S::NV + v) * S::THREADS + threadIdx.x], x[v].f);
+            if (++stage == ST) stage = 0;
+        } else {
 #pragma unroll
-        for (int e = 0; e < S::VEC; ++e) {
-            x[v][e] -= mean;
-            if (ln_col<S>(v, e, t) < p.C) {
-                q += x[v][e] * x[v][e];
-                left += x[v][e];
+            for (int v = 0; v < S::NV; ++v) ln_gather<S>(x0 + r * p.x_pitch, 0.f, v, t, p.C, x[v]);
+        }
+        uint64_t s = 0;
+#pragma unroll
+        for (int v = 0; v < S::NV; ++v)
+#pragma unroll
+            for (int i = 0; i < S::VEC / 2; ++i) s = fadd2(s, x[v].f[i]);
+        const float mean = ln_row_sum<S, false>(ln_pair_sum(s), 0.f, slots, 0).x * inv;
+        const uint64_t minus = pack_f32x2(-mean, -mean);
+        uint64_t q = 0, left = 0;
+#pragma unroll
+        for (int v = 0; v < S::NV; ++v) {
+#pragma unroll
+            for (int i = 0; i < S::VEC / 2; ++i) x[v].f[i] = fadd2(x[v].f[i], minus);
+            if constexpr (S::ALIGNED) {
+                if (ln_col<S>(v, 0, t) >= p.C) continue;
+            } else {
+#pragma unroll
+                for (int e = 0; e < S::VEC; e += 2) {
+                    float a, b;
+                    unpack_f32x2(x[v].f[e / 2], a, b);
+                    x[v].f[e / 2] = pack_f32x2(ln_col<S>(v, e, t) < p.C ? a : 0.f, ln_col<S>(v, e + 1, t) < p.C ? b : 0.f);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < S::VEC / 2; ++i) {
+                q = ffma2(x[v].f[i], x[v].f[i], q);
+                left = fadd2(left, x[v].f[i]);
             }
         }
-    // what rounding has left of the mean: it counts where a row's mean is much larger than its spread
-    const float2 s2 = ln_row_sum<S>(q, left, slots, 1);
-    const float dm = s2.y * inv;
-    const float rstd = rsqrtf(fmaxf(s2.x * inv - dm * dm, 0.f) + p.eps);
-    if (t == 0 && p.mean) {
-        p.mean[r] = mean + dm;
-        p.rstd[r] = rstd;
-    }
-    const float shift = -dm * rstd;
-    T* out = static_cast<T*>(p.out) + static_cast<long>(r) * p.C;
+        // what rounding has left of the mean: it counts where a row's mean is much larger than its spread
+        const float2 s2 = ln_row_sum<S, true>(ln_pair_sum(q), ln_pair_sum(left), slots, 1);
+        const float dm = s2.y * inv;
+        const float rstd = rsqrtf(fmaxf(s2.x * inv - dm * dm, 0.f) + p.eps);
+        if (t == 0 && p.mean) {
+            p.mean[r] = mean + dm;
+            p.rstd[r] = rstd;
+        }
+        const uint64_t scale = pack_f32x2(rstd, rstd), shift = pack_f32x2(-dm * rstd, -dm * rstd);
+        T* out = static_cast<T*>(p.out) + r * p.C;
 #pragma unroll
-    for (int v = 0; v < S::NV; ++v) {
-        float w[S::VEC], b[S::VEC];
-        ln_load_param<S>(p.w, p.param_bf16, 1.f, v, t, p.C, w);
-        ln_load_param<S>(p.b, p.param_bf16, 0.f, v, t, p.C, b);
+        for (int v = 0; v < S::NV; ++v) {
+            LnChunk<S> w, b;
+            ln_load_param<S>(p.w, p.param_bf16, 1.f, v, t, p.C, w);
+            ln_load_param<S>(p.b, p.param_bf16, 0.f, v, t, p.C, b);
 #pragma unroll
-        for (int e = 0; e < S::VEC; ++e) x[v][e] = (x[v][e] * rstd + shift) * w[e] + b[e];
-        ln_store<S>(out, v, t, p.C, x[v]);
+            for (int i = 0; i < S::VEC / 2; ++i) x[v].f[i] = ffma2(ffma2(x[v].f[i], scale, shift), w.f[i], b.f[i]);
+            ln_store<S>(out, v, t, p.C, x[v]);
+        }
     }
 }
 
 template <class S>
 __global__ void __launch_bounds__(S::THREADS, S::BWD_BLOCKS) ln_bwd_kernel(const LnRows p) {
     using T = typename S::T;
+    constexpr int ST = S::BWD_STAGES, ROW = 2 * S::NV * S::THREADS;
+    extern __shared__ uint4 ring[];
     __shared__ float2 slots[2][16];
     pdl_wait();
     pdl_trigger();
     const int t = threadIdx.x % S::TPR;
+    const long first = static_cast<long>(blockIdx.x) * S::ROWS + threadIdx.x / S::TPR, step = static_cast<long>(gridDim.x) * S::ROWS;
+    const T *x0 = static_cast<const T*>(p.x), *g0 = static_cast<const T*>(p.dy);
+    auto request = [&](int s, long r) {
+        ln_request<S>(ring + s * ROW, x0 + r * p.x_pitch, t, p.C);
+        ln_request<S>(ring + s * ROW + S::NV * S::THREADS, g0 + r * p.dy_pitch, t, p.C);
+    };
+    float mean = 0.f, rstd = 0.f;
+    if (first < p.M) {
+        mean = p.mean[first];
+        rstd = p.rstd[first];
+    }
+    if constexpr (S::ALIGNED) {
+#pragma unroll
+        for (int s = 0; s < ST - 1; ++s) {
+            const long r = first + s * step;
+            if (r < p.M) request(s, r);
+            ln_copy_commit();
+        }
+    }
     const float inv = 1.f / static_cast<float>(p.C);
+    LnChunk<S> dw2[S::NV], db2[S::NV];
+#pragma unroll
+    for (int v = 0; v < S::NV; ++v)
+#pragma unroll
+        for (int i = 0; i < S::VEC / 2; ++i) dw2[v].f[i] = db2[v].f[i] = 0;
+    int turn = 0, stage = 0;
+    for (long r = first; r < p.M; r += step, ++turn) {
+        float next_mean = 0.f, next_rstd = 0.f;
+        if (r + step < p.M) {
+            next_mean = p.mean[r + step];
+            next_rstd = p.rstd[r + step];
+        }
+        if constexpr (S::ALIGNED) {
+            const long ra = r + (ST - 1) * step;
+            if (ra < p.M) request(stage == 0 ? ST - 1 : stage - 1, ra);          // the slot that was read last
+            ln_copy_commit();
+            ln_copy_wait<ST - 1>();
+        }
+        // One chunk of both rows, xh and g: read again for the second pass rather than held, which would cost the registers that the sums are in.
+        const uint64_t scale = pack_f32x2(rstd, rstd), minus = pack_f32x2(-mean, -mean);
+        auto chunk = [&](int v, LnChunk<S>& x, LnChunk<S>& g) {
+            if constexpr (S::ALIGNED) {
+                ln_unpack(ring[stage * ROW + v * S::THREADS + threadIdx.x], x.f);
+                ln_unpack(ring[stage * ROW + (S::NV + v) * S::THREADS + threadIdx.x], g.f);
+            } else {
+                ln_gather<S>(x0 + r * p.x_pitch, 0.f, v, t, p.C, x);
+                ln_gather<S>(g0 + r * p.dy_pitch, 0.f, v, t, p.C, g);
+            }
+#pragma unroll
+            for (int i = 0; i < S::VEC / 2; ++i) x.f[i] = fmul2(fadd2(x.f[i], minus), scale);      // past the row's end: something finite, and g is zero there
+        };
+        uint64_t s1 = 0, s2 = 0;
+#pragma unroll
+        for (int v = 0; v < S::NV; ++v) {
+            LnChunk<S> x, g, w;
+            chunk(v, x, g);
+            ln_load_param<S>(p.w, p.param_bf16, 1.f, v, t, p.C, w);
+#pragma unroll
+            for (int i = 0; i < S::VEC / 2; ++i) {
+                dw2[v].f[i] = ffma2(g.f[i], x.f[i], dw2[v].f[i]);
+                db2[v].f[i] = fadd2(db2[v].f[i], g.f[i]);
+                const uint64_t gw = fmul2(g.f[i], w.f[i]);
+                s1 = fadd2(s1, gw);
+                s2 = ffma2(gw, x.f[i], s2);
+            }
+        }
+        const float2 s = ln_row_sum<S, true>(ln_pair_sum(s1), ln_pair_sum(s2), slots, turn);
+        if (p.out) {
+            // dx = rstd g - rstd c1 - xh rstd c2
+            const float c1 = -s.x * inv * rstd, c2 = -s.y * inv * rstd;
+            const uint64_t add = pack_f32x2(c1, c1), slope = pack_f32x2(c2, c2);
+            T* out = static_cast<T*>(p.out) + r * p.C;
+#pragma unroll
+            for (int v = 0; v < S::NV; ++v) {
+                LnChunk<S> x, g, w;
+                chunk(v, x, g);
+                ln_load_param<S>(p.w, p.param_bf16, 1.f, v, t, p.C, w);
+#pragma unroll
+                for (int i = 0; i < S::VEC / 2; ++i) g.f[i] = ffma2(fmul2(g.f[i], w.f[i]), scale, ffma2(x.f[i], slope, add));
+                ln_store<S>(out, v, t, p.C, g);
+            }
+        }
+        mean = next_mean;
+        rstd = next_rstd;
+        if (++stage == ST) stage = 0;
+    }
+    if (!p.part) return;
     float dw[S::NV][S::VEC], db[S::NV][S::VEC];
 #pragma unroll
     for (int v = 0; v < S::NV; ++v)
 #pragma unroll
-        for (int e = 0; e < S::VEC; ++e) dw[v][e] = db[v][e] = 0.f;
-    int turn = 0;
-    for (long r = static_cast<long>(blockIdx.x) * S::ROWS + threadIdx.x / S::TPR; r < p.M; r += static_cast<long>(gridDim.x) * S::ROWS, ++turn) {
-        const T* xr = static_cast<const T*>(p.x) + r * p.x_pitch;
-        const T* gr = static_cast<const T*>(p.dy) + r * p.dy_pitch;
-        const float mean = p.mean[r], rstd = p.rstd[r];
-        float xh[S::NV][S::VEC], g[S::NV][S::VEC];
-        float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-        for (int v = 0; v < S::NV; ++v) {
-            ln_load<S>(xr, v, t, p.C, xh[v]);
-            ln_load<S>(gr, v, t, p.C, g[v]);
+        for (int i = 0; i < S::VEC / 2; ++i) {
+            unpack_f32x2(dw2[v].f[i], dw[v][2 * i], dw[v][2 * i + 1]);
+            unpack_f32x2(db2[v].f[i], db[v][2 * i], db[v][2 * i + 1]);
         }
-#pragma unroll
-        for (int v = 0; v < S::NV; ++v) {
-            float w[S::VEC];
-            ln_load_param<S>(p.w, p.param_bf16, 1.f, v, t, p.C, w);
-#pragma unroll
-            for (int e = 0; e < S::VEC; ++e) {
-                xh[v][e] = (xh[v][e] - mean) * rstd;      // past the row's end: something finite, and g is zero there
-                dw[v][e] += g[v][e] * xh[v][e];
-                db[v][e] += g[v][e];
-                g[v][e] *= w[e];
-                s1 += g[v][e];
-                s2 += g[v][e] * xh[v][e];
-            }
-        }
-        const float2 s = ln_row_sum<S>(s1, s2, slots, turn);
-        const float c1 = s.x * inv, c2 = s.y * inv;
-        if (p.out) {
-            T* out = static_cast<T*>(p.out) + r * p.C;
-#pragma unroll
-            for (int v = 0; v < S::NV; ++v) {
-#pragma unroll
-                for (int e = 0; e < S::VEC; ++e) g[v][e] = rstd * (g[v][e] - c1 - xh[v][e] * c2);
-                ln_store<S>(out, v, t, p.C, g[v]);
-            }
-        }
-    }
-    if (!p.part) return;
     float* part = p.part + static_cast<long>(blockIdx.x) * 2 * p.C;
     if constexpr (S::ROWS == 1) {
 #pragma unroll

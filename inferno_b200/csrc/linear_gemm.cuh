@@ -153,9 +153,13 @@ struct GemmMaps {
     CUtensorMap a[2], b[2], c[2], sum, aux, pre;
 };
 
-__device__ __forceinline__ float2 load_bias2(const GemmParams& p, int col) {      // col is even
-    if (!p.bias_bf16) return *reinterpret_cast<const float2*>(static_cast<const float*>(p.bias) + col);
-    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(static_cast<const __nv_bfloat16*>(p.bias) + col));
+// Two columns of bias (col is even) as they are stored, converted where they are used: the load then waits for nobody.
+__device__ __forceinline__ uint2 load_bias2(const GemmParams& p, int col) {
+    if (!p.bias_bf16) return *reinterpret_cast<const uint2*>(static_cast<const float*>(p.bias) + col);
+    return make_uint2(*reinterpret_cast<const uint32_t*>(static_cast<const __nv_bfloat16*>(p.bias) + col), 0u);
+}
+__device__ __forceinline__ uint64_t bias_pair(const GemmParams& p, uint2 b) {
+    return p.bias_bf16 ? pack_f32x2(__uint_as_float(b.x << 16), __uint_as_float(b.x & 0xffff0000u)) : pack_f32x2(__uint_as_float(b.x), __uint_as_float(b.y));
 }
 
 // gelu in its tanh form is z s(2u) with the logistic function s and u = sqrt(2 / pi) (z + 0.044715 z^3): 0.5 (1 + tanh u) = s(2u).  As one exponential
@@ -163,24 +167,39 @@ __device__ __forceinline__ float2 load_bias2(const GemmParams& p, int col) {    
 // infinite).  Constants: -2 sqrt(2 / pi) log2 e, and that times 0.044715.
 constexpr float kGeluExp1 = -2.302208198f, kGeluExp3 = kGeluExp1 * 0.044715f;
 constexpr float kGeluDu1 = 1.595769122f, kGeluDu3 = kGeluDu1 * 3.f * 0.044715f;      // d(2u)/dz = kGeluDu1 + kGeluDu3 z^2
-__device__ __forceinline__ float gelu_gate(float z) {                                // s(2u)
-    return __fdividef(1.f, 1.f + fast_exp2(z * fmaf(kGeluExp3, z * z, kGeluExp1)));
+// Two at a time: the polynomials in packed fp32, an exponential and a reciprocal each (gelu of 64 elements a thread: 290 issue slots, 510 one by one).
+__device__ __forceinline__ uint64_t splat2(float a) { return pack_f32x2(a, a); }
+__device__ __forceinline__ uint64_t gelu_gate2(uint64_t z, uint64_t zz) {            // s(2u)
+    float a, b;
+    unpack_f32x2(fmul2(z, ffma2(splat2(kGeluExp3), zz, splat2(kGeluExp1))), a, b);
+    unpack_f32x2(fadd2(pack_f32x2(fast_exp2(a), fast_exp2(b)), splat2(1.f)), a, b);
+    return pack_f32x2(fast_rcp(a), fast_rcp(b));
 }
-__device__ __forceinline__ float gelu(float z) { return z * gelu_gate(z); }
-__device__ __forceinline__ float gelu_slope(float z) {                               // |z| <= kPreactLimit
-    const float s = gelu_gate(z);
-    return fmaf(z * fmaf(kGeluDu3, z * z, kGeluDu1), s * (1.f - s), s);
+__device__ __forceinline__ uint64_t gelu2(uint64_t z) { return fmul2(z, gelu_gate2(z, fmul2(z, z))); }
+__device__ __forceinline__ uint64_t gelu_slope2(uint64_t z) {                        // |z| <= kPreactLimit
+    const uint64_t zz = fmul2(z, z), s = gelu_gate2(z, zz);
+    return ffma2(fmul2(z, ffma2(splat2(kGeluDu3), zz, splat2(kGeluDu1))), fmul2(s, ffma2(s, splat2(-1.f), splat2(1.f))), s);
 }
 // z is kept for the backward in fp16: beyond 16 the slope is 0 or 1 to the last bit of an fp32, so it is kept as +-16 (NaN stays NaN), and within that
 // fp16 has three bits more than bf16.  With z in bf16 the gradients would be half as far off again as their own rounding leaves them.
 constexpr float kPreactLimit = 16.f;
-__device__ __forceinline__ float preact_clamp(float z) { return z > kPreactLimit ? kPreactLimit : z < -kPreactLimit ? -kPreactLimit : z; }
-__device__ __forceinline__ uint32_t pack_preact2(float a, float b) {
-    const __half2 h = __floats2half2_rn(preact_clamp(a), preact_clamp(b));
+__device__ __forceinline__ uint32_t pack_preact2(uint64_t z) {
+    float a, b;
+    unpack_f32x2(z, a, b);
+    const __half2 lim = __float2half2_rn(kPreactLimit);
+    const __half2 h = __hmax2_nan(__hmin2_nan(__floats2half2_rn(a, b), lim), __hneg2(lim));
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ float2 unpack_half2(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
-__device__ __forceinline__ float2 unpack_bf16x2(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+__device__ __forceinline__ uint64_t unpack_half2(uint32_t w) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return pack_f32x2(f.x, f.y);
+}
+__device__ __forceinline__ uint64_t unpack_bf16x2(uint32_t w) { return pack_f32x2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+__device__ __forceinline__ uint32_t pack_bf16_pair(uint64_t p) {
+    float a, b;
+    unpack_f32x2(p, a, b);
+    return pack_bf16x2(a, b);
+}
 
 template <int EPI>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmTraits::THREADS, 1)
@@ -298,239 +317,196 @@ gemm_bf16_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ 
             }
         }
     } else {
-        // ------------------------------ epilogue (two threads per output row of this CTA, half of the columns each) ------------------------------
-        // Every warp works for itself: it stages 32 rows x 128 bytes in its own 4 KB and has the TMA unit store them (or add them
-        // to the other parts of the tile), so no barrier ties the warps together.  Registers straight to global memory (a 32-byte
-        // sector per thread) took 6200 cycles a tile, at three cycles per sector, and 2800 more in the release of the accumulator, which
-        // had to wait for the stores; four warps that shared staging panels under named barriers took 7300.
+        // ------------------------------ epilogue (32 rows a warp, half of the tile's columns) ------------------------------
+        // Every warp works for itself: it stages 32 rows x 64 columns in its own 4 KB and has the TMA unit store them (or add them to the other parts
+        // of the tile), so no barrier ties the warps together.  Registers straight to global memory (a 32-byte sector per thread) took 6200
+        // cycles a tile, at three cycles per sector, and 2800 more in the release of the accumulator, which had to wait for the stores; four
+        // warps that shared staging panels under named barriers took 7300.
+        // A thread holds pairs of columns of four rows (tmem_ld_16x256b_x8), the same columns in each, so the bias is eight pairs in registers, and the
+        // arithmetic is packed.  With a row per thread each element's bias came by a shuffle, and two warps a scheduler could not hide it
+        // all: 15000 cycles a 256 x 256 tile with GELU and z, 10800 with a residual (8192 x 1024 x 4096: 69.7 and 56.8 us).
         const int h = warp >> 2, row0 = (warp & 3) * 32;
         const uint32_t lane_base = static_cast<uint32_t>(row0) << 16;
         uint8_t* stage = sOut + warp * TR::STAGING_BYTES;
+        uint8_t* second = smem + SM::OFF_AUX + warp * TR::STAGING_BYTES;      // fused forms: what is read beside the accumulator, or a second output
         const uint32_t free_bar[2] = {mapa_u32(smem_u32(&acc_empty[0]), 0), mapa_u32(smem_u32(&acc_empty[1]), 0)};
+        const bool has_aux = EPI == kEpiResidual || EPI == kEpiSlope || (EPI == kEpiGelu && prm.has_aux);
+        const int colf = h * (BN / 2), pair_col = 2 * (lane & 3);
+        uint32_t aux_n = 0;
+        auto request_aux = [&](const GemmPart& p, int c0) {      // the step's 32 x 64 tile; one at a time is on its way or being read
+            const int row = p.m0 + static_cast<int>(rank) * TR::CM + row0, col = p.n0 + c0;
+            if (has_aux && p.task == 0 && row < prm.t[0].M && col < prm.t[0].N && lane == 0) {
+                mbar_arrive_expect_tx(&aux_full[warp], TR::STAGING_BYTES);
+                tma_load_3d(second, &maps.aux, &aux_full[warp], col, row, 0);
+            }
+        };
+        uint2 bias[8];
+        auto request_bias = [&](const GemmPart& p, int c0) {
+            if (!prm.bias) return;
+            const int col = p.n0 + c0, N = prm.t[p.task].N;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (col + 8 * j < N) bias[j] = load_bias2(prm, col + 8 * j + pair_col);
+        };
+        auto tile_free = [&] {                                   // the last copies have read the staging tiles
+            if (lane == 0) tma_store_wait_read_all();
+            __syncwarp();
+        };
         uint32_t n = 0;
-        auto stage_out = [&](const CUtensorMap* m, bool add, int col, int row, const uint4 (&w)[8]) {
-            if (lane == 0) tma_store_wait_read_all();            // the previous copy has read the staging rows
-            __syncwarp();
-#pragma unroll
-            for (int c = 0; c < 8; ++c) st_shared_sw128(stage, lane, c, w[c]);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-                if (add) tma_reduce_add_3d(m, stage, col, row, 0);       // rows / columns past M / N are clipped by the copy
-                else tma_store_3d(m, stage, col, row, 0);
-                tma_store_commit();
-            }
-        };
-        auto pack_tile = [](const uint32_t (&v)[2][32], uint4 (&w)[8]) {
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                const uint32_t* x = &v[c >> 2][(c & 3) * 8];
-                w[c] = make_uint4(pack_bf16x2(__uint_as_float(x[0]), __uint_as_float(x[1])), pack_bf16x2(__uint_as_float(x[2]), __uint_as_float(x[3])),
-                                  pack_bf16x2(__uint_as_float(x[4]), __uint_as_float(x[5])), pack_bf16x2(__uint_as_float(x[6]), __uint_as_float(x[7])));
-            }
-        };
-        if constexpr (EPI == kEpiBias) {
-            for (; walk.next(q); ++n) {
-                const GemmTask& k = prm.t[q.task];
-                const uint32_t buf = n & 1;
-                const int row = q.m0 + static_cast<int>(rank) * TR::CM + row0;
-                const bool with_bias = prm.bias && q.ks0 == 0;       // the part that starts the tile's K range brings the bias in
-                const bool f32_out = q.partial && prm.split == kPartReduceF32;
-                const CUtensorMap* mc = q.partial ? &maps.sum : &maps.c[q.task];
-                // two columns of bias per lane and 64-column step, fetched under the wait and handed round by shuffles (broadcast loads in
-                // the element loop queued behind the MMAs' operand reads for 2000 cycles and more)
-                float2 bias0 = make_float2(0.f, 0.f), bias1 = bias0;
-                if (with_bias) {
-                    const int col = q.n0 + h * (BN / 2) + 2 * lane;
-                    if (col < k.N) bias0 = load_bias2(prm, col);
-                    if (col + 64 < k.N) bias1 = load_bias2(prm, col + 64);
-                }
-                mbar_wait(&acc_full[buf], (n >> 1) & 1, ab, 30);
-                tc_fence_after_sync();
+        bool more = walk.next(q);
+        if (more) {
+            request_aux(q, colf);
+            request_bias(q, colf);
+        }
+        for (; more; ++n) {
+            const GemmTask& k = prm.t[q.task];
+            const bool fused = EPI != kEpiBias && q.task == 0;
+            const uint32_t buf = n & 1;
+            const int row = q.m0 + static_cast<int>(rank) * TR::CM + row0;
+            const bool with_bias = prm.bias && q.ks0 == 0;       // the part that starts the tile's K range brings the bias in
+            mbar_wait(&acc_full[buf], (n >> 1) & 1, ab, 30);
+            tc_fence_after_sync();
+            GemmPart ahead;
+            bool more_ahead = false;
 #pragma unroll 1
-                for (int c0 = h * (BN / 2); c0 < (h + 1) * (BN / 2); c0 += 64) {
-                    const int col = q.n0 + c0;
-                    uint32_t v[2][32];
-                    tmem_ld_x32(tmem + buf * BN + c0 + lane_base, v[0]);
-                    tmem_ld_x32(tmem + buf * BN + c0 + 32 + lane_base, v[1]);
-                    tmem_wait_ld();
-                    if (c0 + 64 == (h + 1) * (BN / 2)) {
-                        // every column of the accumulator is in registers: hand it back to the MMA warp
-                        tc_fence_before_sync();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster_relaxed(free_bar[buf]);
-                    }
-                    if (row >= k.M || col >= k.N) continue;
-                    if (with_bias) {
-                        const float2 bc = c0 & 64 ? bias1 : bias0;
+            for (int c0 = colf; c0 < colf + BN / 2; c0 += 64) {
+                const int col = q.n0 + c0;
+                const bool inside = row < k.M && col < k.N, last = c0 != colf;
+                uint32_t a[8][4];
+                if (EPI != kEpiBias && has_aux && fused && inside) {
+                    mbar_wait(&aux_full[warp], aux_n & 1, ab, 31);
+                    ++aux_n;
 #pragma unroll
-                        for (int e = 0; e < 64; ++e)
-                            v[e >> 5][e & 31] = __float_as_uint(__uint_as_float(v[e >> 5][e & 31]) + __shfl_sync(0xffffffffu, e & 1 ? bc.y : bc.x, e >> 1));
-                    }
-                    uint4 w[8];
-                    if (!f32_out) {
+                    for (int j = 0; j < 8; ++j) ld_matrix_sw128(second, lane, j, a[j]);
+                }
+                uint32_t r[2][32];
+                tmem_ld_16x256b_x8(tmem + buf * BN + c0 + lane_base, r[0]);
+                tmem_ld_16x256b_x8(tmem + buf * BN + c0 + lane_base + (16u << 16), r[1]);
+                tmem_wait_ld();
+                // rows 8i + lane / 4, columns 8j + pair_col
+                uint64_t v[4][8];
 #pragma unroll
-                        for (int c = 0; c < 8; ++c) {
-                            const uint32_t* x = &v[c >> 2][(c & 3) * 8];
-                            w[c] = make_uint4(pack_bf16x2(__uint_as_float(x[0]), __uint_as_float(x[1])), pack_bf16x2(__uint_as_float(x[2]), __uint_as_float(x[3])),
-                                              pack_bf16x2(__uint_as_float(x[4]), __uint_as_float(x[5])), pack_bf16x2(__uint_as_float(x[6]), __uint_as_float(x[7])));
-                        }
-                        stage_out(mc, q.partial, col, row, w);
-                    } else {
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const uint32_t* x = &r[i >> 1][4 * j + 2 * (i & 1)];
+                        v[i][j] = pack_f32x2(__uint_as_float(x[0]), __uint_as_float(x[1]));
+                    }
+                if (with_bias) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const uint64_t b = bias_pair(prm, bias[j]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[i][j] = fadd2(v[i][j], b);
+                    }
+                }
+                if (last) {
+                    // every column of the accumulator is in registers: hand it back to the MMA warp
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster_relaxed(free_bar[buf]);
+                    more_ahead = walk.next(ahead);
+                    if (more_ahead) {
+                        request_aux(ahead, colf);
+                        request_bias(ahead, colf);
+                    }
+                } else {
+                    __syncwarp();                                // every lane has read the aux tile
+                    request_aux(q, c0 + 64);
+                    request_bias(q, c0 + 64);
+                }
+                if (!inside) continue;
+                tile_free();
+                if (!fused) {
+                    const CUtensorMap* mc = q.partial ? &maps.sum : &maps.c[q.task];
+                    if (q.partial && prm.split == kPartReduceF32) {
 #pragma unroll
                         for (int half = 0; half < 2; ++half) {
+                            if (half) tile_free();
 #pragma unroll
-                            for (int c = 0; c < 8; ++c) w[c] = make_uint4(v[half][4 * c], v[half][4 * c + 1], v[half][4 * c + 2], v[half][4 * c + 3]);
-                            if (col + 32 * half < k.N) stage_out(mc, true, col + 32 * half, row, w);
+                            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)      // 32 columns of fp32: a pair is half a 16-byte chunk
+                                    *reinterpret_cast<uint64_t*>(stage + sw128_offset(8 * i + (lane >> 2), 2 * j + ((lane & 3) >> 1)) + (lane & 1) * 8) = v[i][4 * half + j];
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                            if (lane == 0 && col + 32 * half < k.N) {
+                                tma_reduce_add_3d(mc, stage, col + 32 * half, row, 0);       // rows / columns past M / N are clipped by the copy
+                                tma_store_commit();
+                            }
                         }
-                    }
-                }
-            }
-        } else {
-            // Task 0 with its fused form, task 1 (if there is one) as above.  What the form reads beside the accumulator (aux: 32 rows x 64 columns
-            // at a time) is fetched by the TMA unit into the warp's second tile one step ahead: the first step's under the wait for the tile,
-            // or under the last step of the tile before.
-            uint8_t* aux = smem + SM::OFF_AUX + warp * TR::STAGING_BYTES;
-            const bool has_aux = EPI == kEpiResidual || EPI == kEpiSlope || prm.has_aux;
-            const int colf = h * (BN / 2);
-            uint32_t aux_n = 0;
-            auto request_aux = [&](const GemmPart& p, int c0) {
-                const int row = p.m0 + static_cast<int>(rank) * TR::CM + row0, col = p.n0 + c0;
-                if (has_aux && p.task == 0 && row < prm.t[0].M && col < prm.t[0].N && lane == 0) {
-                    mbar_arrive_expect_tx(&aux_full[warp], TR::STAGING_BYTES);
-                    tma_load_3d(aux, &maps.aux, &aux_full[warp], col, row, 0);
-                }
-            };
-            // a copy out of either tile: `pending` = 1 where the two tiles take turns (the other one's copy may still be reading)
-            auto stage_to = [&](uint8_t* tile, int pending, const CUtensorMap* m, int col, int row, const uint4 (&w)[8]) {
-                if (lane == 0) {
-                    if (pending) tma_store_wait_read<1>();
-                    else tma_store_wait_read_all();
-                }
-                __syncwarp();
-#pragma unroll
-                for (int c = 0; c < 8; ++c) st_shared_sw128(tile, lane, c, w[c]);
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                    tma_store_3d(m, tile, col, row, 0);
-                    tma_store_commit();
-                }
-            };
-            bool more = walk.next(q);
-            if (more) request_aux(q, colf);
-            for (; more; ++n) {
-                const GemmTask& k = prm.t[q.task];
-                const bool fused = q.task == 0;
-                const uint32_t buf = n & 1;
-                const int row = q.m0 + static_cast<int>(rank) * TR::CM + row0;
-                const bool with_bias = prm.bias && fused;
-                float2 bias0 = make_float2(0.f, 0.f), bias1 = bias0;
-                if (with_bias) {
-                    const int col = q.n0 + colf + 2 * lane;
-                    if (col < k.N) bias0 = load_bias2(prm, col);
-                    if (col + 64 < k.N) bias1 = load_bias2(prm, col + 64);
-                }
-                mbar_wait(&acc_full[buf], (n >> 1) & 1, ab, 30);
-                tc_fence_after_sync();
-                GemmPart ahead;
-                bool more_ahead = false;
-#pragma unroll 1
-                for (int c0 = colf; c0 < colf + BN / 2; c0 += 64) {
-                    const int col = q.n0 + c0;
-                    const bool inside = row < k.M && col < k.N, last = c0 != colf;
-                    uint4 a[8];
-                    if (has_aux && fused && inside) {
-                        mbar_wait(&aux_full[warp], aux_n & 1, ab, 31);
-                        ++aux_n;
-#pragma unroll
-                        for (int c = 0; c < 8; ++c) a[c] = *reinterpret_cast<const uint4*>(aux + sw128_offset(lane, c));
-                    }
-                    uint32_t v[2][32];
-                    tmem_ld_x32(tmem + buf * BN + c0 + lane_base, v[0]);
-                    tmem_ld_x32(tmem + buf * BN + c0 + 32 + lane_base, v[1]);
-                    tmem_wait_ld();
-                    if (last) {
-                        tc_fence_before_sync();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster_relaxed(free_bar[buf]);
-                        more_ahead = walk.next(ahead);
-                        if (more_ahead) request_aux(ahead, colf);
                     } else {
-                        __syncwarp();          // every lane has read the aux tile
-                        request_aux(q, c0 + 64);
-                    }
-                    if (!inside) continue;
-                    uint4 w[8];
-                    if (!fused) {
-                        const bool f32_out = q.partial && prm.split == kPartReduceF32;
-                        const CUtensorMap* mc = q.partial ? &maps.sum : &maps.c[1];
-                        if (!f32_out) {
-                            pack_tile(v, w);
-                            stage_out(mc, q.partial, col, row, w);
-                        } else {
 #pragma unroll
-                            for (int half = 0; half < 2; ++half) {
-#pragma unroll
-                                for (int c = 0; c < 8; ++c) w[c] = make_uint4(v[half][4 * c], v[half][4 * c + 1], v[half][4 * c + 2], v[half][4 * c + 3]);
-                                if (col + 32 * half < k.N) stage_out(mc, true, col + 32 * half, row, w);
-                            }
+                        for (int j = 0; j < 8; ++j) {
+                            const uint32_t w[4] = {pack_bf16_pair(v[0][j]), pack_bf16_pair(v[1][j]), pack_bf16_pair(v[2][j]), pack_bf16_pair(v[3][j])};
+                            st_matrix_sw128(stage, lane, j, w);
                         }
-                        continue;
-                    }
-                    if (with_bias) {
-                        const float2 bc = last ? bias1 : bias0;
-#pragma unroll
-                        for (int e = 0; e < 64; ++e)
-                            v[e >> 5][e & 31] = __float_as_uint(__uint_as_float(v[e >> 5][e & 31]) + __shfl_sync(0xffffffffu, e & 1 ? bc.y : bc.x, e >> 1));
-                    }
-                    if constexpr (EPI == kEpiGelu) {
-                        if (prm.write_pre) {
-#pragma unroll
-                            for (int c = 0; c < 8; ++c) {
-                                const uint32_t* x = &v[c >> 2][(c & 3) * 8];
-                                w[c] = make_uint4(pack_preact2(__uint_as_float(x[0]), __uint_as_float(x[1])), pack_preact2(__uint_as_float(x[2]), __uint_as_float(x[3])),
-                                                  pack_preact2(__uint_as_float(x[4]), __uint_as_float(x[5])), pack_preact2(__uint_as_float(x[6]), __uint_as_float(x[7])));
-                            }
-                            stage_to(stage, !has_aux, &maps.pre, col, row, w);
-                        }
-#pragma unroll
-                        for (int e = 0; e < 64; ++e) v[e >> 5][e & 31] = __float_as_uint(gelu(__uint_as_float(v[e >> 5][e & 31])));
-                    }
-                    if (EPI == kEpiSlope || has_aux) {
-#pragma unroll
-                        for (int c = 0; c < 8; ++c) {
-                            const uint32_t aw[4] = {a[c].x, a[c].y, a[c].z, a[c].w};
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                uint32_t* x = &v[c >> 2][(c & 3) * 8 + 2 * e];
-                                const float2 f = EPI == kEpiSlope ? unpack_half2(aw[e]) : unpack_bf16x2(aw[e]);
-                                x[0] = __float_as_uint(EPI == kEpiSlope ? __uint_as_float(x[0]) * gelu_slope(f.x) : __uint_as_float(x[0]) + f.x);
-                                x[1] = __float_as_uint(EPI == kEpiSlope ? __uint_as_float(x[1]) * gelu_slope(f.y) : __uint_as_float(x[1]) + f.y);
-                            }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (q.partial) tma_reduce_add_3d(mc, stage, col, row, 0);
+                            else tma_store_3d(mc, stage, col, row, 0);
+                            tma_store_commit();
                         }
                     }
-                    pack_tile(v, w);
-                    // z and gelu(z) go out of a tile each, unless the second one holds the residual
-                    const bool two = EPI == kEpiGelu && !has_aux && prm.write_pre;
-                    stage_to(two ? aux : stage, two, &maps.c[0], col, row, w);
-                    if constexpr (EPI == kEpiSlope) {
-                        // two columns a lane, over the 32 rows of the staged tile (a row at a time: 128 bytes, no bank twice); rows past M are zeros
-                        if (prm.colsum) {
-                            float2 sum = make_float2(0.f, 0.f);
+                    continue;
+                }
+                if constexpr (EPI != kEpiBias) {
+                    uint8_t* out = stage;
+                    if (EPI == kEpiGelu && prm.write_pre) {
 #pragma unroll
-                            for (int r = 0; r < 32; ++r) {
-                                const float2 f = unpack_bf16x2(*reinterpret_cast<const uint32_t*>(stage + sw128_offset(r, lane >> 2) + (lane & 3) * 4));
-                                sum.x += f.x;
-                                sum.y += f.y;
-                            }
-                            if (col + 2 * lane < k.N) *reinterpret_cast<float2*>(prm.colsum + static_cast<long>(row >> 5) * k.N + col + 2 * lane) = sum;
+                        for (int j = 0; j < 8; ++j) {
+                            const uint32_t w[4] = {pack_preact2(v[0][j]), pack_preact2(v[1][j]), pack_preact2(v[2][j]), pack_preact2(v[3][j])};
+                            st_matrix_sw128(stage, lane, j, w);
                         }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tma_store_3d(&maps.pre, stage, col, row, 0);
+                            tma_store_commit();
+                        }
+                        // gelu(z) goes out of the second tile, or, where that one is the residual's, out of the first again
+                        if (has_aux) tile_free();
+                        else out = second;
+                    }
+                    uint64_t sum[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if (EPI == kEpiGelu) v[i][j] = gelu2(v[i][j]);
+                            if (EPI == kEpiSlope) v[i][j] = fmul2(v[i][j], gelu_slope2(unpack_half2(a[j][i])));
+                            else if (has_aux) v[i][j] = fadd2(v[i][j], unpack_bf16x2(a[j][i]));
+                            w[i] = pack_bf16_pair(v[i][j]);
+                        }
+                        if (EPI == kEpiSlope) sum[j] = fadd2(fadd2(v[0][j], v[1][j]), fadd2(v[2][j], v[3][j]));
+                        st_matrix_sw128(out, lane, j, w);
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_3d(&maps.c[0], out, col, row, 0);
+                        tma_store_commit();
+                    }
+                    if (EPI == kEpiSlope && prm.colsum) {
+                        // the eight lanes that share columns add up their rows' sums, each ending with one of the eight pairs (rows past M are zeros)
+#pragma unroll
+                        for (int half = 4; half > 0; half >>= 1) {
+                            const bool upper = lane & (4 * half);
+#pragma unroll
+                            for (int j = 0; j < half; ++j) {
+                                const uint64_t send = upper ? sum[j] : sum[j + half], keep = upper ? sum[j + half] : sum[j];
+                                sum[j] = fadd2(keep, __shfl_xor_sync(0xffffffffu, static_cast<unsigned long long>(send), 4 * half));
+                            }
+                        }
+                        const int at = col + 8 * (lane >> 2) + pair_col;
+                        if (at < k.N) *reinterpret_cast<uint64_t*>(prm.colsum + static_cast<long>(row >> 5) * k.N + at) = sum[0];
                     }
                 }
-                more = more_ahead;
-                q = ahead;
             }
+            more = more_ahead;
+            q = ahead;
         }
         if (lane == 0) tma_store_wait_read_all();    // the CTA may leave once its shared memory has been read; the writes complete on their own
     }
@@ -583,8 +559,8 @@ __global__ void __launch_bounds__(256) linear_prep_kernel(const __nv_bfloat16* _
             uint32_t o[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float2 f = unpack_half2(z[e]), d = unpack_bf16x2(g[e]);
-                const float a = d.x * gelu_slope(f.x), b = d.y * gelu_slope(f.y);
+                float a, b;
+                unpack_f32x2(fmul2(unpack_bf16x2(g[e]), gelu_slope2(unpack_half2(z[e]))), a, b);
                 acc[2 * e] += a;
                 acc[2 * e + 1] += b;
                 o[e] = pack_bf16x2(a, b);
@@ -695,29 +671,26 @@ __global__ void __launch_bounds__(256) linear_fused_finish_kernel(const FusedFin
     const long step = static_cast<long>(gridDim.x) * blockDim.x;
     for (long i = static_cast<long>(blockIdx.x) * blockDim.x + threadIdx.x; i < p.n8; i += step) {
         const float4 a = p.acc[2 * i], b = p.acc[2 * i + 1];
-        float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        uint64_t v[4] = {pack_f32x2(a.x, a.y), pack_f32x2(a.z, a.w), pack_f32x2(b.x, b.y), pack_f32x2(b.z, b.w)};
         const int col = static_cast<int>(i * 8 % p.N);
-        if (p.bias) {
+        uint32_t o[4];
+        const uint4 r4 = p.residual ? p.residual[i] : make_uint4(0, 0, 0, 0);
+        const uint32_t r[4] = {r4.x, r4.y, r4.z, r4.w};
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                v[e] += p.bias_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[col + e]) : static_cast<const float*>(p.bias)[col + e];
+        for (int e = 0; e < 4; ++e) {
+            if (p.bias)
+                v[e] = fadd2(v[e], p.bias_bf16 ? unpack_bf16x2(reinterpret_cast<const uint32_t*>(static_cast<const __nv_bfloat16*>(p.bias) + col)[e])
+                                               : reinterpret_cast<const uint64_t*>(static_cast<const float*>(p.bias) + col)[e]);
+            o[e] = pack_preact2(v[e]);
         }
-        if (p.pre) p.pre[i] = make_uint4(pack_preact2(v[0], v[1]), pack_preact2(v[2], v[3]), pack_preact2(v[4], v[5]), pack_preact2(v[6], v[7]));
-        if (p.gelu) {
+        if (p.pre) p.pre[i] = make_uint4(o[0], o[1], o[2], o[3]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = gelu(v[e]);
+        for (int e = 0; e < 4; ++e) {
+            if (p.gelu) v[e] = gelu2(v[e]);
+            if (p.residual) v[e] = fadd2(v[e], unpack_bf16x2(r[e]));
+            o[e] = pack_bf16_pair(v[e]);
         }
-        if (p.residual) {
-            const uint4 r = p.residual[i];
-            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 f = unpack_bf16x2(w[e]);
-                v[2 * e] += f.x;
-                v[2 * e + 1] += f.y;
-            }
-        }
-        p.y[i] = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+        p.y[i] = make_uint4(o[0], o[1], o[2], o[3]);
     }
 }
 

@@ -384,8 +384,6 @@ __device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk
 __device__ __forceinline__ void tma_store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void tma_store_wait_read_all() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 
-template <int PENDING>      // all but the last PENDING copies of this thread
-__device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(PENDING) : "memory"); }
 
 // ---- TMEM ----------------------------------------------------------------------
 // One full warp allocates; the base address (lane 0, first column) lands in smem.
@@ -537,6 +535,21 @@ __device__ __forceinline__ void st_shared_sw128(uint8_t* panel, uint32_t row, ui
     *reinterpret_cast<uint4*>(panel + sw128_offset(row, chunk16)) = v;
 }
 
+// Four 8x8 matrices of 16-bit elements between registers and a 128B-swizzled panel of 32 rows, stacked: chunk `chunk16` of rows 0 .. 31.  Thread t holds
+// elements 2 (t % 4), +1 of row 8i + t / 4 in w[i].  No bank is met twice.
+__device__ __forceinline__ void st_matrix_sw128(uint8_t* panel, uint32_t lane, uint32_t chunk16, const uint32_t (&w)[4]) {
+    IB200_CHECKED(lane < 32u && chunk16 < 8u && smem_addr_ok(smem_u32(panel), 1024), kBndSwizzle);
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(panel + sw128_offset(lane, chunk16))), "r"(w[0]), "r"(w[1]),
+                 "r"(w[2]), "r"(w[3])
+                 : "memory");
+}
+__device__ __forceinline__ void ld_matrix_sw128(const uint8_t* panel, uint32_t lane, uint32_t chunk16, uint32_t (&w)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "r"(smem_u32(panel + sw128_offset(lane, chunk16)))
+                 : "memory");
+}
+
 // ---- TMEM <-> registers --------------------------------------------------------
 // 32x32b shape: the warp reads 32 lanes (its quarter: lanes 32*(warp%4)..+31),
 // thread i gets lane i, N consecutive 32-bit columns.
@@ -550,6 +563,27 @@ __device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t (&r)[32]) {
 #endif
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+// 16x256b shape, 64 columns: 16 lanes (`taddr` names the first: the warp's quarter, or 16 past it).  Thread t holds, of each 8 columns j, the pair of
+// columns 8j + 2 (t % 4) of row t / 4 in r[4j], r[4j + 1] and of row t / 4 + 8 in r[4j + 2], r[4j + 3]: the layout that stmatrix and ldmatrix speak.
+__device__ __forceinline__ void tmem_ld_16x256b_x8(uint32_t taddr, uint32_t (&r)[32]) {
+#ifdef IB200_BOUNDS
+    if (!bounds_ok(tmem_addr_ok(taddr, 64), kBndTmemLd)) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) r[e] = 0u;
+        return;
+    }
+#endif
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
         "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
         "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
@@ -591,18 +625,23 @@ __device__ __forceinline__ float fast_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float fast_rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// Packed fp32x2 arithmetic (one instruction for two lanes of fp32 math).
 // three-input maximum (one instruction on sm_100)
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
+// Packed fp32x2 arithmetic (one instruction for two lanes of fp32 math).
 __device__ __forceinline__ uint64_t pack_f32x2(float lo, float hi) {
     uint64_t r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
