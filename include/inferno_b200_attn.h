@@ -146,28 +146,27 @@ int ib200_linear_bwd_ws(const void* x, const void* w, const void* dy, void* dx, 
 
 /* y[M,N] = act(x[M,K] w[K,N] + bias[N]) + residual[M,N], all but the product in its epilogue.  activation IB200_ACT_GELU is the reference's
  * tanh form, gelu(z) = z / (1 + exp(-2u)) with u = sqrt(2 / pi) (z + 0.044715 z^3).  bias (of type bias_dtype) and residual (bf16, dense) may be
- * NULL.  preact: if not NULL (activation GELU only), z = x w + bias is kept there for the backward as fp16, [M, N], limited to +-16,
- * beyond which gelu' is 0 or 1.  K and N multiples of 8, any M; bases 16-byte aligned.  The workspace is used by products that are cut along K
- * (ib200_fused_linear_workspace_bytes, 0: none); without one they are not cut.  y and preact must not overlap the operands, y not preact.
+ * NULL.  slope: if not NULL (activation GELU only), gelu'(x w + bias) is kept there for the backward as fp16, [M, N].  K and N multiples of 8, any M; bases 16-byte aligned.  The workspace is used by products that are cut along K
+ * (ib200_fused_linear_workspace_bytes, 0: none); without one they are not cut.  y and slope must not overlap the operands, y not slope.
  * Replaces Linear::forward, the gelu op and the residual addition behind them (src/inferno/modules/linear.cpp:99-106,
  * src/inferno/cuda/cudagelu.cu:40-66, src/inferno/cuda/cudaadd.cu:20-142). */
 enum { IB200_ACT_NONE = 0, IB200_ACT_GELU = 1 };
 size_t ib200_fused_linear_workspace_bytes(int M, int K, int N, int activation, int pass);
 int ib200_fused_linear_fwd(const void* x, const void* w, const void* bias, int bias_dtype, const void* residual, int activation,
-                           void* y, void* preact, int M, int K, int N, void* workspace, size_t workspace_bytes, ib200_stream_t stream);
+                           void* y, void* slope, int M, int K, int N, void* workspace, size_t workspace_bytes, ib200_stream_t stream);
 
-/* Its backward: dz = dy gelu'(preact) (activation GELU; dz = dy without one, preact NULL), dx = dz w^T, dw = x^T dz, db = column sums of dz (of
+/* Its backward: dz = dy slope (activation GELU; dz = dy without one, slope NULL), dx = dz w^T, dw = x^T dz, db = column sums of dz (of
  * type db_dtype); any of dx / dw / db may be NULL.  The gradient of the residual is dy itself.  The workspace is always needed.  dw is
  * added up as in ib200_linear_bwd_ws; dx and db repeat bit for bit.  Replaces MMBackward and GeluBackward
  * (src/inferno/gradfn/mmbackward.cpp:36-98; kernel src/inferno/cuda/cudagelu.cu:138-202). */
-int ib200_fused_linear_bwd(const void* x, const void* w, const void* dy, const void* preact, int activation, void* dx, void* dw,
+int ib200_fused_linear_bwd(const void* x, const void* w, const void* dy, const void* slope, int activation, void* dx, void* dw,
                            void* db, int db_dtype, int M, int K, int N, void* workspace, size_t workspace_bytes, ib200_stream_t stream);
 
 /* Backward of the feed-forward block y[M,C] = h w2 + b2 (+ residual), h = gelu(x[M,C] w1[C,H] + b1): two ib200_fused_linear_fwd calls, which leave
- * preact (fp16) and h [M,H].  dz = (dy w2^T) gelu'(preact) is formed in the epilogue of that product and its columns are summed there (db1), dw2 =
+ * slope (fp16) and h [M,H].  dz = (dy w2^T) slope is formed in the epilogue of that product and its columns are summed there (db1), dw2 =
  * h^T dy, db2 = column sums of dy, dx = dz w1^T, dw1 = x^T dz; any output may be NULL.  C and H multiples of 8, any M. */
 size_t ib200_feed_forward_workspace_bytes(int M, int C, int H);
-int ib200_feed_forward_bwd(const void* x, const void* w1, const void* preact, const void* h, const void* w2, const void* dy, void* dx,
+int ib200_feed_forward_bwd(const void* x, const void* w1, const void* slope, const void* h, const void* w2, const void* dy, void* dx,
                            void* dw1, void* db1, int db1_dtype, void* dw2, void* db2, int db2_dtype, int M, int C, int H,
                            void* workspace, size_t workspace_bytes, ib200_stream_t stream);
 

@@ -15,6 +15,7 @@
 #include "attn_fwd.cuh"
 #include "attn_fwd_persist.cuh"
 #include "layer_norm.cuh"
+#include "linear_few.cuh"
 #include "linear_gemm.cuh"
 
 namespace {
@@ -77,12 +78,12 @@ bool make_tmap(CUtensorMap* m, const void* base, bool f32, int D, int T, const R
     return r == CUDA_SUCCESS;
 }
 
-// Tensor map over a row-major matrix [rows, cols] of bf16 or fp32; box = [box_rows x 128 bytes], 128B swizzle.
-bool make_tmap_2d(CUtensorMap* m, const void* base, long rows, long cols, int box_rows, bool f32 = false) {
+// Tensor map over a row-major matrix [rows, cols] of bf16 or fp32 (or several, one behind the other); box = [box_rows x 128 bytes], 128B swizzle.
+bool make_tmap_2d(CUtensorMap* m, const void* base, long rows, long cols, int box_rows, bool f32 = false, int matrices = 1) {
     EncodeTiledFn enc = encode_fn();
     if (!enc) return false;
     const cuuint64_t es = f32 ? 4 : 2;
-    cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), 1};
+    cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(matrices)};
     cuuint64_t strides[2] = {static_cast<cuuint64_t>(cols) * es, static_cast<cuuint64_t>(rows) * static_cast<cuuint64_t>(cols) * es};
     cuuint32_t box[3] = {static_cast<cuuint32_t>(128 / es), static_cast<cuuint32_t>(box_rows), 1};
     cuuint32_t estr[3] = {1, 1, 1};
@@ -471,7 +472,8 @@ struct GemmDesc {
 
 bool gemm_set_task(GemmParams& p, GemmMaps& m, int i, const GemmDesc& d) {
     using TR = GemmTraits;
-    p.t[i] = GemmTask{d.M, d.N, (d.M + TR::BM - 1) / TR::BM, d.tiles(), d.k_slices(), d.a_mn, d.b_mn};
+    const int band = kBandRows * ((d.N + TR::BN - 1) / TR::BN);
+    p.t[i] = GemmTask{d.M, d.N, (d.M + TR::BM - 1) / TR::BM, d.tiles(), d.k_slices(), d.a_mn, d.b_mn, band, 1.f / static_cast<float>(band)};
     // A: [M, K] (box 128 rows) or stored [K, M] (box 64 k-rows); B: stored [K, N] (box 64 k-rows) or [N, K] (box 128 rows)
     return (d.a_mn ? make_tmap_2d(&m.a[i], d.a, d.K, d.M, TR::BK) : make_tmap_2d(&m.a[i], d.a, d.M, d.K, TR::CM)) &&
            (d.b_mn ? make_tmap_2d(&m.b[i], d.b, d.K, d.N, TR::BK) : make_tmap_2d(&m.b[i], d.b, d.N, d.K, TR::CN)) &&
@@ -487,14 +489,23 @@ bool gemm_wants_split_beside(const GemmDesc& d, int pairs) { return d.tiles() <=
 // A fused epilogue of the `whole` product (kEpi*): what it reads beside its accumulator, and what it writes beside c.
 struct GemmEpi {
     int mode = kEpiBias;
-    const void* aux = nullptr;      // residual (bf16) or z (fp16), [M, N]
-    void* pre = nullptr;            // z, fp16 [M, N]
+    const void* aux = nullptr;      // residual (bf16) or gelu'(z) (fp16), [M, N]
+    void* keep = nullptr;           // where gelu'(z) goes, fp16 [M, N]
     float* colsum = nullptr;        // [ceil(M / 32)][N]
 };
 template <int EPI>
 int launch_gemm_form(int pairs, const GemmMaps& maps, const GemmParams& p, cudaStream_t stream) {
     if (!allow_smem<gemm_bf16_kernel<EPI>>(GemmSmem<EPI>::BYTES)) return IB200_ERR_CUDA;
     return launch_pdl<gemm_bf16_kernel<EPI>>(2 * pairs, GemmTraits::THREADS, GemmSmem<EPI>::BYTES, stream, maps, p);
+}
+
+// Parts of a forward with a fused epilogue that is cut along K (1: it is not).  Cutting costs a launch behind it and the parts' traffic, about 5 us
+// together, and saves the slices that other pairs take over, 0.3 us each.  Whole against cut, us: 777 x 1000 x 2008 (saves 8 slices) 15.1 and 16.3,
+// 17 x 1024 x 4096 (8) 12.2 and 10.9, 512 x 2048 x 512 (24) 17.0 and 13.0, 1023 x 4096 x 1024 (48) 27.0 and 19.1, 64 x 4096 x 1024 (56) 25.7 and 12.2.
+constexpr int kMinSavedSlices = 12;
+int gemm_slabs(const GemmDesc& d, int pairs) {
+    const int parts = std::min(std::min(8, pairs / d.tiles()), d.k_slices() / kMinPartSlices);
+    return parts > 1 && d.k_slices() - (d.k_slices() + parts - 1) / parts > kMinSavedSlices ? parts : 1;
 }
 
 // One launch: `whole` cut into whole tiles (may be null), `other` cut into whole tiles or, with split != kPartWhole, along K.
@@ -510,11 +521,12 @@ int launch_gemms(const GemmDesc* whole, const GemmDesc* other, int split, float*
     if (!whole) { maps.a[0] = maps.a[1]; maps.b[0] = maps.b[1]; maps.c[0] = maps.c[1]; }
     if (!other) { maps.a[1] = maps.a[0]; maps.b[1] = maps.b[0]; maps.c[1] = maps.c[0]; }
     maps.sum = maps.c[1];
-    if (split == kPartReduceF32 && !make_tmap_2d(&maps.sum, acc, other->M, other->N, 32, true)) return IB200_ERR_CUDA;
-    maps.aux = maps.pre = maps.c[0];
-    if ((epi.aux && !make_tmap_2d(&maps.aux, epi.aux, whole->M, whole->N, 32)) || (epi.pre && !make_tmap_2d(&maps.pre, epi.pre, whole->M, whole->N, 32))) return IB200_ERR_CUDA;
+    p.slabs = split == kPartSlab ? gemm_slabs(*other, max_pairs) : 1;
+    if (split >= kPartReduceF32 && !make_tmap_2d(&maps.sum, acc, other->M, other->N, 32, true, p.slabs)) return IB200_ERR_CUDA;
+    maps.aux = maps.keep = maps.c[0];
+    if ((epi.aux && !make_tmap_2d(&maps.aux, epi.aux, whole->M, whole->N, 32)) || (epi.keep && !make_tmap_2d(&maps.keep, epi.keep, whole->M, whole->N, 32))) return IB200_ERR_CUDA;
     p.has_aux = epi.aux != nullptr;
-    p.write_pre = epi.pre != nullptr;
+    p.keep_slope = epi.keep != nullptr;
     p.colsum = epi.colsum;
     p.split = split;
     p.bias = bias;
@@ -524,10 +536,10 @@ int launch_gemms(const GemmDesc* whole, const GemmDesc* other, int split, float*
     if (split == kPartWhole) {
         tiles += p.t[1].tiles;
         pairs = static_cast<int>(tiles < max_pairs ? tiles : max_pairs);
-    } else if (split == kPartReduceBf16) {
+    } else if (split == kPartReduceBf16 || split == kPartSlab) {
         // Every part is rounded to bf16 as it is added, so a tile is cut into as few equal parts as keep the pairs busy.  Two parts give the same
         // bits in either order.  (Runs of equal length over all tiles, the rule below, meet in three or four parts of some tiles.)
-        int splits = std::min(8, max_pairs / p.t[1].tiles);
+        int splits = split == kPartSlab ? p.slabs : std::min(8, max_pairs / p.t[1].tiles);
         while (splits > 1 && p.t[1].k_slices / splits < kMinPartSlices) --splits;
         pairs = p.t[1].tiles * splits;
         p.heavy = 0;
@@ -605,27 +617,60 @@ int gemm_single(const GemmDesc& d, const void* bias, int bias_bf16, void* ws, si
 
 bool valid_dtype(int dtype) { return dtype == IB200_DTYPE_F32 || dtype == IB200_DTYPE_BF16; }
 
+// Up to 16 rows.  Blocks of a cluster split K until two blocks per SM are there, as long as every warp keeps two steps of 16 rows.
+template <int SPLIT>
+int launch_few(const FewRows& p, int strips, cudaStream_t stream) {
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = SPLIT;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(strips * SPLIT);
+    cfg.blockDim = dim3(kFewWarps * 32);
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = SPLIT > 1 ? 2 : 1;
+    return cuda_ok(cudaLaunchKernelEx(&cfg, linear_few_kernel<SPLIT>, p)) ? IB200_OK : IB200_ERR_CUDA;
+}
+int linear_few(FewRows p, int sms, cudaStream_t stream) {
+    const int strips = (p.N + kFewCols - 1) / kFewCols, steps = (p.K + 15) / 16;
+    int split = 1;
+    while (split < 8 && strips * split * 2 <= 2 * sms && steps >= split * 2 * 2 * kFewWarps) split *= 2;
+    p.steps = (steps + split - 1) / split;
+    switch (split) {
+        case 1: return launch_few<1>(p, strips, stream);
+        case 2: return launch_few<2>(p, strips, stream);
+        case 4: return launch_few<4>(p, strips, stream);
+        default: return launch_few<8>(p, strips, stream);
+    }
+}
+
 // y = act(x w + bias) + residual.
-int fused_linear_fwd_core(const GemmDesc& d, const void* bias, int bias_bf16, const void* residual, void* pre, bool gelu, void* ws, size_t ws_bytes,
+int fused_linear_fwd_core(const GemmDesc& d, const void* bias, int bias_bf16, const void* residual, void* slope, bool gelu, void* ws, size_t ws_bytes,
                           cudaStream_t stream) {
-    if (!gelu && !residual) return gemm_single(d, bias, bias_bf16, ws, ws_bytes, stream);
-    if (!aligned16(bias) || !aligned16(residual) || !aligned16(pre)) return IB200_ERR_MISALIGNED;
+    if (!aligned16(bias) || !aligned16(residual) || !aligned16(slope)) return IB200_ERR_MISALIGNED;
     int rc = gemm_check(d);
     if (rc != IB200_OK) return rc;
     const DeviceInfo* dev = device_info();
     if (!dev) return IB200_ERR_CUDA;
+    if (d.M <= kFewMaxRows)
+        return linear_few(FewRows{static_cast<const __nv_bfloat16*>(d.a), static_cast<const __nv_bfloat16*>(d.b), bias, bias_bf16, gelu,
+                                  static_cast<const __nv_bfloat16*>(residual), static_cast<__half*>(slope), static_cast<__nv_bfloat16*>(d.c), d.M, d.N, d.K, 0},
+                          dev->sms, stream);
     const size_t n = static_cast<size_t>(d.M) * d.N;
-    if (gemm_wants_split(d, dev->sms / 2) && ws && ws_bytes >= n * 4) {
-        if (!cuda_ok(cudaMemsetAsync(ws, 0, n * 4, stream))) return IB200_ERR_CUDA;
-        if ((rc = launch_gemms(nullptr, &d, kPartReduceF32, static_cast<float*>(ws), nullptr, 0, stream))) return rc;
-        const FusedFinish p{static_cast<const float4*>(ws), bias, bias_bf16, gelu, static_cast<const uint4*>(residual), static_cast<uint4*>(pre), static_cast<uint4*>(d.c),
+    const int slabs = gemm_slabs(d, dev->sms / 2);
+    if (slabs > 1 && ws && ws_bytes >= slabs * n * 4) {
+        if ((rc = launch_gemms(nullptr, &d, kPartSlab, static_cast<float*>(ws), nullptr, 0, stream))) return rc;
+        const FusedFinish p{static_cast<const float4*>(ws), slabs, bias, bias_bf16, gelu, static_cast<const uint4*>(residual), static_cast<uint4*>(slope), static_cast<uint4*>(d.c),
                             static_cast<long>(n / 8), d.N};
         return launch_pdl<linear_fused_finish_kernel>(static_cast<int>(std::min<long>((p.n8 + 255) / 256, 148 * 8)), 256, 0, stream, p);
     }
     GemmEpi epi;
-    epi.mode = gelu ? kEpiGelu : kEpiResidual;
+    epi.mode = gelu ? kEpiGelu : residual ? kEpiResidual : kEpiBias;
     epi.aux = residual;
-    epi.pre = pre;
+    epi.keep = slope;
     return launch_gemms(&d, nullptr, kPartWhole, nullptr, bias, bias_bf16, stream, epi);
 }
 
@@ -637,24 +682,24 @@ int colsum_slabs(int M, int N) {
 }
 size_t linear_bwd_ws_bytes(int K, int N) { return round_up(static_cast<size_t>(K) * N * 4, 256) + static_cast<size_t>(kMaxColsumSlabs) * N * 4; }
 
-// The helper ahead of a backward's products: column sums of dy (`part`), zeroing of the accumulators, and with `pre` dz = dy gelu'(z).
-int launch_linear_prep(const void* dy, const void* pre, void* dz, float* part, int M, int N, bool atomic, float* zero, size_t zero_floats, cudaStream_t stream) {
+// The helper ahead of a backward's products: column sums of dy (`part`), zeroing of the accumulators, and with `slope` dz = dy slope.
+int launch_linear_prep(const void* dy, const void* slope, void* dz, float* part, int M, int N, bool atomic, float* zero, size_t zero_floats, cudaStream_t stream) {
     const int slabs = colsum_slabs(M, N), rows = (M + slabs - 1) / slabs;
-    const dim3 grid((N + kColsumCols - 1) / kColsumCols, part || pre ? slabs : 64);
+    const dim3 grid((N + kColsumCols - 1) / kColsumCols, part || slope ? slabs : 64);
     float4* z4 = reinterpret_cast<float4*>(zero);
     const long n4 = static_cast<long>(zero_floats / 4);
     const auto* g = static_cast<const __nv_bfloat16*>(dy);
-    return pre ? launch_pdl<linear_prep_kernel<true>>(grid, 256, 0, stream, g, static_cast<const __half*>(pre), static_cast<__nv_bfloat16*>(dz), part, M, N, rows,
+    return slope ? launch_pdl<linear_prep_kernel<true>>(grid, 256, 0, stream, g, static_cast<const __half*>(slope), static_cast<__nv_bfloat16*>(dz), part, M, N, rows,
                                                       static_cast<int>(atomic), z4, n4)
                : launch_pdl<linear_prep_kernel<false>>(grid, 256, 0, stream, g, static_cast<const __half*>(nullptr), static_cast<__nv_bfloat16*>(nullptr), part, M, N,
                                                        rows, static_cast<int>(atomic), z4, n4);
 }
 
-// With `pre` (and a workspace) dy is first multiplied by gelu'(pre), into `dz`.
+// With `slope` (and a workspace) dy is first multiplied by it, into `dz`.
 int linear_bwd_core(const void* x, const void* w, const void* dy, void* dx, void* dw, void* db, int db_bf16, int M, int K, int N, void* ws, size_t ws_bytes,
-                    cudaStream_t stream, const void* pre = nullptr, void* dz = nullptr) {
+                    cudaStream_t stream, const void* slope = nullptr, void* dz = nullptr) {
     if (!x || !w || !dy) return IB200_ERR_INVALID_ARGUMENT;
-    const void* g = pre ? dz : dy;
+    const void* g = slope ? dz : dy;
     // dx[M,K] = g[M,N] w^T: w is stored [K, N], i.e. the "B" of this product stored [N_out = K rows, contraction N contiguous]
     const GemmDesc gx{g, w, dx, M, K, N, 0, 0};
     // dw[K,N] = x^T g: x is stored [M, K], i.e. the "A" of this product stored [contraction M rows, K contiguous]
@@ -677,8 +722,8 @@ int linear_bwd_core(const void* x, const void* w, const void* dy, void* dx, void
         part = have_ws ? reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + round_up(static_cast<size_t>(K) * N * 4, 256)) : static_cast<float*>(db);
         if (!have_ws && !cuda_ok(cudaMemsetAsync(db, 0, static_cast<size_t>(N) * 4, stream))) return IB200_ERR_CUDA;
     }
-    if (db || split || pre) {
-        if ((rc = launch_linear_prep(dy, pre, dz, part, M, N, !have_ws, acc, split ? static_cast<size_t>(K) * N : 0, stream))) return rc;
+    if (db || split || slope) {
+        if ((rc = launch_linear_prep(dy, slope, dz, part, M, N, !have_ws, acc, split ? static_cast<size_t>(K) * N : 0, stream))) return rc;
     }
     if (have_ws && dx && dw) {
         if ((rc = launch_gemms(&gx, &gw, split ? kPartReduceF32 : kPartWhole, acc, nullptr, 0, stream))) return rc;
@@ -690,7 +735,7 @@ int linear_bwd_core(const void* x, const void* w, const void* dy, void* dx, void
     return launch_linear_finish(finish_job(acc, dw, static_cast<long>(K) * N, part, colsum_slabs(M, N), N, have_ws ? db : nullptr, db_bf16), stream);
 }
 
-// The feed-forward block's backward: dz = (dy w2^T) gelu'(z) with the columns' sums in the epilogue of that product, which shares its launch with
+// The feed-forward block's backward: dz = (dy w2^T) slope with the columns' sums in the epilogue of that product, which shares its launch with
 // dw2 = h^T dy; then dx = dz w1^T and dw1 = x^T dz in another.  Workspace: [acc1 | acc2 | dy's column sums | dz's column sums | dz].
 struct FfWorkspace {
     size_t acc1, acc2, part2, part1, dz, bytes;
@@ -704,7 +749,7 @@ struct FfWorkspace {
         bytes = dz + round_up(static_cast<size_t>(M) * H * 2, 256);
     }
 };
-int ff_bwd_core(const void* x, const void* w1, const void* pre, const void* h, const void* w2, const void* dy, void* dx, void* dw1, void* db1, int db1_bf16,
+int ff_bwd_core(const void* x, const void* w1, const void* kept, const void* h, const void* w2, const void* dy, void* dx, void* dw1, void* db1, int db1_bf16,
                 void* dw2, void* db2, int db2_bf16, int M, int C, int H, uint8_t* ws, cudaStream_t stream) {
     const FfWorkspace L(M, C, H);
     const bool inner = dx || dw1 || db1;
@@ -712,7 +757,7 @@ int ff_bwd_core(const void* x, const void* w1, const void* pre, const void* h, c
     const GemmDesc gz{dy, w2, dz, M, H, C, 0, 0}, gw2{h, dy, dw2, H, C, M, 1, 1}, gx{dz, w1, dx, M, C, H, 0, 0}, gw1{x, dz, dw1, C, H, M, 1, 1};
     int rc;
     if ((inner && (rc = gemm_check(gz))) || (dw2 && (rc = gemm_check(gw2))) || (dx && (rc = gemm_check(gx))) || (dw1 && (rc = gemm_check(gw1)))) return rc;
-    if (!aligned16(dy) || !aligned16(pre)) return IB200_ERR_MISALIGNED;
+    if (!aligned16(dy) || !aligned16(kept)) return IB200_ERR_MISALIGNED;
     const DeviceInfo* dev = device_info();
     if (!dev) return IB200_ERR_NO_DEVICE;
     const int pairs = dev->sms / 2;
@@ -726,7 +771,7 @@ int ff_bwd_core(const void* x, const void* w1, const void* pre, const void* h, c
     }
     GemmEpi slope;
     slope.mode = kEpiSlope;
-    slope.aux = pre;
+    slope.aux = kept;
     slope.colsum = part1;
     if (inner) {
         if ((rc = launch_gemms(&gz, dw2 ? &gw2 : nullptr, split2 ? kPartReduceF32 : kPartWhole, acc2, nullptr, 0, stream, slope))) return rc;
@@ -745,47 +790,60 @@ int ff_bwd_core(const void* x, const void* w1, const void* pre, const void* h, c
 }
 
 // ---- layer norm ----------------------------------------------------------------------
-constexpr int kLnMaxChunks = 4;        // 16-byte chunks of a row that a thread holds
-
-// Threads per row: as few as hold the row in four chunks each.  0: the row is too long.
+// Threads per row, by its 16-byte chunks.  A thread holds two to four of them where it can: with one (128 threads for 16384 x 1024 bf16) what is done per
+// row and not per element takes over, 22 us forward and 36 backward.  0: the row is too long.
 int ln_threads_per_row(int C, int dtype) {
-    const long bytes = static_cast<long>(C) * (dtype == IB200_DTYPE_F32 ? 4 : 2);
-    for (int tpr : {32, 128, 256, 512})
-        if (bytes <= 16L * kLnMaxChunks * tpr) return tpr;
+    const long chunks = (static_cast<long>(C) * (dtype == IB200_DTYPE_F32 ? 4 : 2) + 15) / 16;
+    if (chunks <= 3 * 32) return 32;
+    for (int tpr : {64, 128, 256, 512})
+        if (chunks <= 4L * tpr) return tpr;
     return 0;
 }
-int ln_bwd_blocks(int M, int C, int dtype, int sms) {
-    const int tpr = ln_threads_per_row(C, dtype), rows = tpr == 32 ? 8 : 1, per_sm = tpr == 32 ? 2 : 512 / tpr;
-    return std::min((M - 1) / rows + 1, per_sm * sms);
-}
+int ln_bwd_blocks(int M, int C, int dtype, int sms) { return std::min((M - 1) / (kLnBwdThreads / ln_threads_per_row(C, dtype)) + 1, sms); }
 
 template <class S>
 int launch_ln(bool backward, const LnRows& p, int blocks, cudaStream_t stream) {
     if (!allow_smem<ln_bwd_kernel<S>>(S::BWD_SMEM) || !allow_smem<ln_fwd_kernel<S>>(S::FWD_SMEM)) return IB200_ERR_CUDA;
-    return backward ? launch_pdl<ln_bwd_kernel<S>>(blocks, S::THREADS, S::BWD_SMEM, stream, p)
-                    : launch_pdl<ln_fwd_kernel<S>>(std::min((p.M - 1) / S::ROWS + 1, S::FWD_BLOCKS * device_info()->sms), S::THREADS, S::FWD_SMEM, stream, p);
+    return backward ? launch_pdl<ln_bwd_kernel<S>>(blocks, kLnBwdThreads, S::BWD_SMEM, stream, p)
+                    : launch_pdl<ln_fwd_kernel<S>>(std::min((p.M - 1) / S::FWD_ROWS + 1, S::FWD_BLOCKS * device_info()->sms), S::FWD_THREADS, S::FWD_SMEM, stream, p);
 }
-template <class T, int TPR>
-int launch_ln_row(bool aligned, bool backward, const LnRows& p, int blocks, cudaStream_t stream) {
-    if (!aligned) return launch_ln<LnShape<T, TPR, kLnMaxChunks, false>>(backward, p, blocks, stream);
-    switch ((p.C - 1) / LnShape<T, TPR, 1, true>::CHUNK_COLS) {
-        case 0: return launch_ln<LnShape<T, TPR, 1, true>>(backward, p, blocks, stream);
-        case 1: return launch_ln<LnShape<T, TPR, 2, true>>(backward, p, blocks, stream);
-        case 2: return launch_ln<LnShape<T, TPR, 3, true>>(backward, p, blocks, stream);
-        default: return launch_ln<LnShape<T, TPR, 4, true>>(backward, p, blocks, stream);
+template <class T, class PT, int TPR, bool ALIGNED>
+int launch_ln_row(bool backward, const LnRows& p, int blocks, cudaStream_t stream) {
+    const int nv = (p.C - 1) / LnShape<T, PT, TPR, 1, true>::CHUNK_COLS + 1;
+    if constexpr (TPR == 32) {
+        if (nv == 1) return launch_ln<LnShape<T, PT, TPR, 1, ALIGNED>>(backward, p, blocks, stream);
+    }
+    if constexpr (TPR <= 64) {
+        if (nv == 2) return launch_ln<LnShape<T, PT, TPR, 2, ALIGNED>>(backward, p, blocks, stream);
+    }
+    if (TPR == 32 || nv == 3) return launch_ln<LnShape<T, PT, TPR, 3, ALIGNED>>(backward, p, blocks, stream);
+    if constexpr (TPR > 32) return launch_ln<LnShape<T, PT, TPR, 4, ALIGNED>>(backward, p, blocks, stream);
+    return IB200_ERR_UNSUPPORTED;
+}
+template <class T, class PT, bool ALIGNED>
+int launch_ln_shape(int dtype, bool backward, const LnRows& p, int blocks, cudaStream_t stream) {
+    switch (ln_threads_per_row(p.C, dtype)) {
+        case 32: return launch_ln_row<T, PT, 32, ALIGNED>(backward, p, blocks, stream);
+        case 64: return launch_ln_row<T, PT, 64, ALIGNED>(backward, p, blocks, stream);
+        case 128: return launch_ln_row<T, PT, 128, ALIGNED>(backward, p, blocks, stream);
+        case 256: return launch_ln_row<T, PT, 256, ALIGNED>(backward, p, blocks, stream);
+        default: return launch_ln_row<T, PT, 512, ALIGNED>(backward, p, blocks, stream);
     }
 }
-template <class T>
+// PT: type of weight and bias in the kernels for aligned rows.
+template <class T, class PT>
 int launch_ln_type(int dtype, bool backward, const LnRows& p, int blocks, cudaStream_t stream) {
     constexpr int kVec = 16 / sizeof(T);
-    const bool aligned = p.C % kVec == 0 && p.x_pitch % kVec == 0 && p.dy_pitch % kVec == 0 && aligned16(p.x) && aligned16(p.dy) && aligned16(p.w) &&
+    const bool typed = (!p.w && !p.b) || p.param_bf16 == (sizeof(PT) == 2);
+    const bool aligned = typed && p.C % kVec == 0 && p.x_pitch % kVec == 0 && p.dy_pitch % kVec == 0 && aligned16(p.x) && aligned16(p.dy) && aligned16(p.w) &&
                          aligned16(p.b) && aligned16(p.out);
-    switch (ln_threads_per_row(p.C, dtype)) {
-        case 32: return launch_ln_row<T, 32>(aligned, backward, p, blocks, stream);
-        case 128: return launch_ln_row<T, 128>(aligned, backward, p, blocks, stream);
-        case 256: return launch_ln_row<T, 256>(aligned, backward, p, blocks, stream);
-        default: return launch_ln_row<T, 512>(aligned, backward, p, blocks, stream);
-    }
+    return aligned ? launch_ln_shape<T, PT, true>(dtype, backward, p, blocks, stream) : launch_ln_shape<T, float, false>(dtype, backward, p, blocks, stream);
+}
+// fp32 rows with bf16 weights, which nobody keeps, share the kernels for rows that do not begin on 16 bytes.
+int launch_ln_any(int dtype, bool backward, const LnRows& p, int blocks, cudaStream_t stream) {
+    if (dtype == IB200_DTYPE_F32) return launch_ln_type<float, float>(dtype, backward, p, blocks, stream);
+    return p.param_bf16 ? launch_ln_type<__nv_bfloat16, __nv_bfloat16>(dtype, backward, p, blocks, stream)
+                        : launch_ln_type<__nv_bfloat16, float>(dtype, backward, p, blocks, stream);
 }
 
 int ln_check(const void* x, long x_pitch, int M, int C, int dtype, int param_dtype) {
@@ -1069,41 +1127,46 @@ int ib200_linear_bwd_ws(const void* x, const void* w, const void* dy, void* dx, 
 
 size_t ib200_fused_linear_workspace_bytes(int M, int K, int N, int activation, int pass) {
     if (M <= 0 || K <= 0 || N <= 0) return 0;
-    if (pass != IB200_PASS_BWD) return ib200_linear_workspace_bytes(M, K, N, pass);
+    if (pass != IB200_PASS_BWD) {
+        const DeviceInfo* dev = device_info();
+        if (!dev || M <= kFewMaxRows) return 0;
+        const int slabs = gemm_slabs(GemmDesc{nullptr, nullptr, nullptr, M, N, K, 0, 1}, dev->sms / 2);
+        return slabs > 1 ? static_cast<size_t>(slabs) * M * N * 4 : 0;
+    }
     const size_t base = linear_bwd_ws_bytes(K, N);
     return activation == IB200_ACT_GELU ? round_up(base, 256) + static_cast<size_t>(M) * N * 2 : base;
 }
 
-int ib200_fused_linear_fwd(const void* x, const void* w, const void* bias, int bias_dtype, const void* residual, int activation, void* y, void* preact, int M, int K,
+int ib200_fused_linear_fwd(const void* x, const void* w, const void* bias, int bias_dtype, const void* residual, int activation, void* y, void* slope, int M, int K,
                            int N, void* workspace, size_t workspace_bytes, ib200_stream_t stream) {
     if (!valid_dtype(bias_dtype) || (activation != IB200_ACT_NONE && activation != IB200_ACT_GELU)) return IB200_ERR_INVALID_ARGUMENT;
-    if (preact && activation == IB200_ACT_NONE) return IB200_ERR_INVALID_ARGUMENT;
+    if (slope && activation == IB200_ACT_NONE) return IB200_ERR_INVALID_ARGUMENT;
     if (workspace && !aligned16(workspace)) return IB200_ERR_WORKSPACE;
-    return fused_linear_fwd_core(GemmDesc{x, w, y, M, N, K, 0, 1}, bias, bias_dtype == IB200_DTYPE_BF16, residual, preact, activation == IB200_ACT_GELU, workspace,
+    return fused_linear_fwd_core(GemmDesc{x, w, y, M, N, K, 0, 1}, bias, bias_dtype == IB200_DTYPE_BF16, residual, slope, activation == IB200_ACT_GELU, workspace,
                                  workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
 }
 
-int ib200_fused_linear_bwd(const void* x, const void* w, const void* dy, const void* preact, int activation, void* dx, void* dw, void* db, int db_dtype, int M, int K,
+int ib200_fused_linear_bwd(const void* x, const void* w, const void* dy, const void* slope, int activation, void* dx, void* dw, void* db, int db_dtype, int M, int K,
                            int N, void* workspace, size_t workspace_bytes, ib200_stream_t stream) {
     if (!valid_dtype(db_dtype) || (activation != IB200_ACT_NONE && activation != IB200_ACT_GELU)) return IB200_ERR_INVALID_ARGUMENT;
-    if ((activation == IB200_ACT_GELU) != (preact != nullptr) || M <= 0 || K <= 0 || N <= 0) return IB200_ERR_INVALID_ARGUMENT;
-    if (!aligned16(preact)) return IB200_ERR_MISALIGNED;
+    if ((activation == IB200_ACT_GELU) != (slope != nullptr) || M <= 0 || K <= 0 || N <= 0) return IB200_ERR_INVALID_ARGUMENT;
+    if (!aligned16(slope)) return IB200_ERR_MISALIGNED;
     if (!workspace || !aligned16(workspace) || workspace_bytes < ib200_fused_linear_workspace_bytes(M, K, N, activation, IB200_PASS_BWD)) return IB200_ERR_WORKSPACE;
     if (!dx && !dw && !db) return IB200_OK;
     if (N % 8) return IB200_ERR_UNSUPPORTED;
-    void* dz = preact ? static_cast<uint8_t*>(workspace) + round_up(linear_bwd_ws_bytes(K, N), 256) : nullptr;
-    return linear_bwd_core(x, w, dy, dx, dw, db, db_dtype == IB200_DTYPE_BF16, M, K, N, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream), preact, dz);
+    void* dz = slope ? static_cast<uint8_t*>(workspace) + round_up(linear_bwd_ws_bytes(K, N), 256) : nullptr;
+    return linear_bwd_core(x, w, dy, dx, dw, db, db_dtype == IB200_DTYPE_BF16, M, K, N, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream), slope, dz);
 }
 
 size_t ib200_feed_forward_workspace_bytes(int M, int C, int H) { return M <= 0 || C <= 0 || H <= 0 ? 0 : FfWorkspace(M, C, H).bytes; }
 
-int ib200_feed_forward_bwd(const void* x, const void* w1, const void* preact, const void* h, const void* w2, const void* dy, void* dx, void* dw1, void* db1,
+int ib200_feed_forward_bwd(const void* x, const void* w1, const void* slope, const void* h, const void* w2, const void* dy, void* dx, void* dw1, void* db1,
                            int db1_dtype, void* dw2, void* db2, int db2_dtype, int M, int C, int H, void* workspace, size_t workspace_bytes, ib200_stream_t stream) {
-    if (!x || !w1 || !preact || !h || !w2 || !dy || M <= 0 || C <= 0 || H <= 0 || !valid_dtype(db1_dtype) || !valid_dtype(db2_dtype)) return IB200_ERR_INVALID_ARGUMENT;
+    if (!x || !w1 || !slope || !h || !w2 || !dy || M <= 0 || C <= 0 || H <= 0 || !valid_dtype(db1_dtype) || !valid_dtype(db2_dtype)) return IB200_ERR_INVALID_ARGUMENT;
     if (C % 8 || H % 8) return IB200_ERR_UNSUPPORTED;
     if (!workspace || !aligned16(workspace) || workspace_bytes < ib200_feed_forward_workspace_bytes(M, C, H)) return IB200_ERR_WORKSPACE;
     if (!dx && !dw1 && !db1 && !dw2 && !db2) return IB200_OK;
-    return ff_bwd_core(x, w1, preact, h, w2, dy, dx, dw1, db1, db1_dtype == IB200_DTYPE_BF16, dw2, db2, db2_dtype == IB200_DTYPE_BF16, M, C, H,
+    return ff_bwd_core(x, w1, slope, h, w2, dy, dx, dw1, db1, db1_dtype == IB200_DTYPE_BF16, dw2, db2, db2_dtype == IB200_DTYPE_BF16, M, C, H,
                        static_cast<uint8_t*>(workspace), reinterpret_cast<cudaStream_t>(stream));
 }
 
@@ -1123,8 +1186,7 @@ int ib200_layer_norm_fwd(const void* x, int64_t x_pitch, const void* weight, con
         return IB200_ERR_MISALIGNED;
     if ((rc = device_ok()) != IB200_OK) return rc;
     const LnRows p{x, static_cast<long>(x_pitch), nullptr, 0, weight, bias, param_dtype == IB200_DTYPE_BF16, y, mean, rstd, nullptr, M, C, eps};
-    return dtype == IB200_DTYPE_F32 ? launch_ln_type<float>(dtype, false, p, 0, reinterpret_cast<cudaStream_t>(stream))
-                                    : launch_ln_type<__nv_bfloat16>(dtype, false, p, 0, reinterpret_cast<cudaStream_t>(stream));
+    return launch_ln_any(dtype, false, p, 0, reinterpret_cast<cudaStream_t>(stream));
 }
 
 int ib200_layer_norm_bwd(const void* x, int64_t x_pitch, const void* weight, const void* dy, int64_t dy_pitch, const float* mean, const float* rstd, void* dx,
@@ -1146,9 +1208,9 @@ int ib200_layer_norm_bwd(const void* x, int64_t x_pitch, const void* weight, con
     float* part = params ? static_cast<float*>(workspace) : nullptr;
     const LnRows p{x, static_cast<long>(x_pitch), dy, static_cast<long>(dy_pitch), weight, nullptr, param_dtype == IB200_DTYPE_BF16, dx, const_cast<float*>(mean),
                    const_cast<float*>(rstd), part, M, C, 0.f};
-    rc = dtype == IB200_DTYPE_F32 ? launch_ln_type<float>(dtype, true, p, blocks, stream) : launch_ln_type<__nv_bfloat16>(dtype, true, p, blocks, stream);
+    rc = launch_ln_any(dtype, true, p, blocks, stream);
     if (rc != IB200_OK || !params) return rc;
-    return launch_pdl<ln_finish_kernel>(dim3((C + kLnFinishCols - 1) / kLnFinishCols, 2), 256, 0, stream, part, blocks, C, dw, db,
+    return launch_pdl<ln_finish_kernel>(dim3((C + kLnFinishCols - 1) / kLnFinishCols, 2), 512, 0, stream, part, blocks, C, dw, db,
                                         static_cast<int>(param_dtype == IB200_DTYPE_BF16));
 }
 

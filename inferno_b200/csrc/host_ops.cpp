@@ -633,9 +633,9 @@ struct Scratch {
 };
 
 struct Fused {
-    Tensor y, pre;
+    Tensor y, slope;
 };
-// y = act(x w + bias) + residual; with `keep` (and an activation) z as fp16, for the backward.
+// y = act(x w + bias) + residual; with `keep` (and an activation) act'(x w + bias) as fp16, for the backward.
 Fused fused_linear_forward(const Tensor& x_, const Tensor& w_, const Tensor& bias_, int act, const Tensor& residual_, bool keep) {
     check_fused(x_, w_, bias_, residual_);
     const c10::cuda::CUDAGuard guard(x_.device());
@@ -645,7 +645,7 @@ Fused fused_linear_forward(const Tensor& x_, const Tensor& w_, const Tensor& bia
     shape.back() = N;
     Fused r;
     r.y = at::empty(shape, x_.options());
-    if (keep && act != IB200_ACT_NONE) r.pre = at::empty(shape, x_.options().dtype(at::kHalf));
+    if (keep && act != IB200_ACT_NONE) r.slope = at::empty(shape, x_.options().dtype(at::kHalf));
     if (M == 0) return r;
     const Tensor x = dense16(x_), w = dense16(w_), b = dense16(bias_), res = dense16(residual_);
     const int k = static_cast<int>(K), n = static_cast<int>(N);
@@ -653,22 +653,22 @@ Fused fused_linear_forward(const Tensor& x_, const Tensor& w_, const Tensor& bia
     const size_t bytes = g_abi.fused_linear_workspace_bytes(M, k, n, act, IB200_PASS_FWD);
     const Scratch scratch(bytes, x.device(), stream);
     check_status(g_abi.fused_linear_fwd(x.data_ptr(), w.data_ptr(), ptr_or_null(b), b.defined() ? dtype_code(b) : IB200_DTYPE_F32, ptr_or_null(res), act,
-                                        r.y.data_ptr(), ptr_or_null(r.pre), M, k, n, scratch.ptr(), bytes, reinterpret_cast<ib200_stream_t>(stream)),
+                                        r.y.data_ptr(), ptr_or_null(r.slope), M, k, n, scratch.ptr(), bytes, reinterpret_cast<ib200_stream_t>(stream)),
                  "ib200_fused_linear_fwd");
     return r;
 }
-void check_preact(const Tensor& pre, const Tensor& x, int64_t N) {
-    TORCH_CHECK_VALUE(pre.defined() && pre.numel() == x.numel() / x.size(-1) * N && pre.device() == x.device() && pre.scalar_type() == at::kHalf,
-                      "linear: preact must be the float16 pre-activation that the forward kept");
+void check_slope(const Tensor& slope, const Tensor& x, int64_t N) {
+    TORCH_CHECK_VALUE(slope.defined() && slope.numel() == x.numel() / x.size(-1) * N && slope.device() == x.device() && slope.scalar_type() == at::kHalf,
+                      "linear: slope must be the float16 tensor that the forward kept");
 }
-LinearGrads fused_linear_backward(const Tensor& x_, const Tensor& w_, const Tensor& dy_, const Tensor& pre_, int act, bool need_dx, bool need_dw, bool need_db,
+LinearGrads fused_linear_backward(const Tensor& x_, const Tensor& w_, const Tensor& dy_, const Tensor& slope_, int act, bool need_dx, bool need_dw, bool need_db,
                                   bool db_bf16) {
     check_linear_shapes(x_, w_);
     const int64_t K = w_.size(0), N = w_.size(1);
     check_output_like(dy_, x_, N, "dy");
     check_fused(x_, w_, Tensor(), Tensor());
     check_output_type(dy_, x_, "dy");
-    if (act != IB200_ACT_NONE) check_preact(pre_, x_, N);
+    if (act != IB200_ACT_NONE) check_slope(slope_, x_, N);
     const c10::cuda::CUDAGuard guard(x_.device());
     const int M = rows_of(x_, K);
     LinearGrads g;
@@ -677,19 +677,19 @@ LinearGrads fused_linear_backward(const Tensor& x_, const Tensor& w_, const Tens
     if (need_dw) g.dw = M ? at::empty({K, N}, x_.options()) : at::zeros({K, N}, x_.options());
     if (need_db) g.db = M ? at::empty({N}, db_type) : at::zeros({N}, db_type);
     if (M == 0 || (!need_dx && !need_dw && !need_db)) return g;
-    const Tensor x = dense16(x_), w = dense16(w_), dy = dense16(dy_), pre = act != IB200_ACT_NONE ? dense16(pre_) : Tensor();
+    const Tensor x = dense16(x_), w = dense16(w_), dy = dense16(dy_), slope = act != IB200_ACT_NONE ? dense16(slope_) : Tensor();
     const int k = static_cast<int>(K), n = static_cast<int>(N);
     cudaStream_t stream = c10::cuda::getCurrentCUDAStream(x.device().index()).stream();
     const size_t bytes = g_abi.fused_linear_workspace_bytes(M, k, n, act, IB200_PASS_BWD);
     const Scratch scratch(bytes, x.device(), stream);
-    check_status(g_abi.fused_linear_bwd(x.data_ptr(), w.data_ptr(), dy.data_ptr(), ptr_or_null(pre), act, ptr_or_null(g.dx), ptr_or_null(g.dw), ptr_or_null(g.db),
+    check_status(g_abi.fused_linear_bwd(x.data_ptr(), w.data_ptr(), dy.data_ptr(), ptr_or_null(slope), act, ptr_or_null(g.dx), ptr_or_null(g.dw), ptr_or_null(g.db),
                                         db_bf16 ? IB200_DTYPE_BF16 : IB200_DTYPE_F32, M, k, n, scratch.ptr(), bytes, reinterpret_cast<ib200_stream_t>(stream)),
                  "ib200_fused_linear_bwd");
     return g;
 }
 
 struct FusedLinearBackward : torch::autograd::Node {
-    SavedVariable x, w, pre;
+    SavedVariable x, w, slope;
     int act = IB200_ACT_NONE;
     at::ScalarType bias_type = at::kFloat;
 
@@ -699,14 +699,14 @@ struct FusedLinearBackward : torch::autograd::Node {
     variable_list backward(const variable_list& grads) {
         variable_list out(4);
         if (!grads[0].defined()) return out;
-        const Tensor tx = x.unpack(), tw = w.unpack(), tp = act != IB200_ACT_NONE ? pre.unpack() : Tensor();
+        const Tensor tx = x.unpack(), tw = w.unpack(), tp = act != IB200_ACT_NONE ? slope.unpack() : Tensor();
         at::AutoDispatchBelowADInplaceOrView below;
         const LinearGrads g = fused_linear_backward(tx, tw, grads[0], tp, act, task_should_compute_output(0), task_should_compute_output(1),
                                                     task_should_compute_output(2), bias_type == at::kBFloat16);
         out = {g.dx, g.dw, g.db, task_should_compute_output(3) ? grads[0] : Tensor()};      // the residual's gradient is dy itself
         return out;
     }
-    void release_variables() override { x.reset_data(); w.reset_data(); pre.reset_data(); }
+    void release_variables() override { x.reset_data(); w.reset_data(); slope.reset_data(); }
     std::string name() const override { return "FusedLinearBackward"; }
 };
 
@@ -724,7 +724,7 @@ Tensor fused_linear(const Tensor& x, const Tensor& w, const Tensor& bias, int ac
         node->x = SavedVariable(x, false);
         node->w = SavedVariable(w, false);
         node->act = act;
-        if (r.pre.defined()) node->pre = SavedVariable(r.pre, false);
+        if (r.slope.defined()) node->slope = SavedVariable(r.slope, false);
         if (bias.defined()) node->bias_type = bias.scalar_type();
         torch::autograd::set_history(r.y, node);
     }
@@ -748,14 +748,14 @@ void check_feed_forward(const Tensor& x, const Tensor& w1, const Tensor& b1, con
 struct FeedForwardGrads {
     Tensor dx, dw1, db1, dw2, db2;
 };
-FeedForwardGrads feed_forward_backward(const Tensor& x_, const Tensor& w1_, const Tensor& pre_, const Tensor& h_, const Tensor& w2_, const Tensor& dy_,
+FeedForwardGrads feed_forward_backward(const Tensor& x_, const Tensor& w1_, const Tensor& slope_, const Tensor& h_, const Tensor& w2_, const Tensor& dy_,
                                        const bool (&need)[5], at::ScalarType b1_type, at::ScalarType b2_type) {
     check_feed_forward(x_, w1_, Tensor(), w2_, Tensor(), Tensor());
     const int64_t C = w1_.size(0), H = w1_.size(1);
     check_output_like(dy_, x_, C, "dy");
     check_output_type(dy_, x_, "dy");
-    check_preact(pre_, x_, H);
-    TORCH_CHECK_VALUE(h_.numel() == pre_.numel() && h_.device() == x_.device() && h_.scalar_type() == at::kBFloat16, "feed_forward: h must be the forward's hidden layer");
+    check_slope(slope_, x_, H);
+    TORCH_CHECK_VALUE(h_.numel() == slope_.numel() && h_.device() == x_.device() && h_.scalar_type() == at::kBFloat16, "feed_forward: h must be the forward's hidden layer");
     const c10::cuda::CUDAGuard guard(x_.device());
     const int M = rows_of(x_, C);
     auto output = [&](bool wanted, at::IntArrayRef shape, at::ScalarType type) {
@@ -765,13 +765,13 @@ FeedForwardGrads feed_forward_backward(const Tensor& x_, const Tensor& w1_, cons
     FeedForwardGrads g{output(need[0], x_.sizes(), at::kBFloat16), output(need[1], {C, H}, at::kBFloat16), output(need[2], {H}, b1_type),
                        output(need[3], {H, C}, at::kBFloat16), output(need[4], {C}, b2_type)};
     if (M == 0) return g;
-    const Tensor x = dense16(x_), w1 = dense16(w1_), pre = dense16(pre_), h = dense16(h_), w2 = dense16(w2_), dy = dense16(dy_);
+    const Tensor x = dense16(x_), w1 = dense16(w1_), slope = dense16(slope_), h = dense16(h_), w2 = dense16(w2_), dy = dense16(dy_);
     const int c = static_cast<int>(C), hh = static_cast<int>(H);
     auto code = [](at::ScalarType t) { return t == at::kBFloat16 ? IB200_DTYPE_BF16 : IB200_DTYPE_F32; };
     cudaStream_t stream = c10::cuda::getCurrentCUDAStream(x.device().index()).stream();
     const size_t bytes = g_abi.feed_forward_workspace_bytes(M, c, hh);
     const Scratch scratch(bytes, x.device(), stream);
-    check_status(g_abi.feed_forward_bwd(x.data_ptr(), w1.data_ptr(), pre.data_ptr(), h.data_ptr(), w2.data_ptr(), dy.data_ptr(), ptr_or_null(g.dx), ptr_or_null(g.dw1),
+    check_status(g_abi.feed_forward_bwd(x.data_ptr(), w1.data_ptr(), slope.data_ptr(), h.data_ptr(), w2.data_ptr(), dy.data_ptr(), ptr_or_null(g.dx), ptr_or_null(g.dw1),
                                         ptr_or_null(g.db1), code(b1_type), ptr_or_null(g.dw2), ptr_or_null(g.db2), code(b2_type), M, c, hh, scratch.ptr(), bytes,
                                         reinterpret_cast<ib200_stream_t>(stream)),
                  "ib200_feed_forward_bwd");
@@ -779,7 +779,7 @@ FeedForwardGrads feed_forward_backward(const Tensor& x_, const Tensor& w1_, cons
 }
 
 struct FeedForwardBackward : torch::autograd::Node {
-    SavedVariable x, w1, pre, h, w2;
+    SavedVariable x, w1, slope, h, w2;
     at::ScalarType b1_type = at::kFloat, b2_type = at::kFloat;
 
     variable_list apply(variable_list&& grads) override {
@@ -787,7 +787,7 @@ struct FeedForwardBackward : torch::autograd::Node {
     }
     variable_list backward(const variable_list& grads) {
         if (!grads[0].defined()) return variable_list(6);
-        const Tensor tx = x.unpack(), t1 = w1.unpack(), tp = pre.unpack(), th = h.unpack(), t2 = w2.unpack();
+        const Tensor tx = x.unpack(), t1 = w1.unpack(), tp = slope.unpack(), th = h.unpack(), t2 = w2.unpack();
         at::AutoDispatchBelowADInplaceOrView below;
         bool need[5];
         for (int i = 0; i < 5; ++i) need[i] = task_should_compute_output(i);
@@ -795,7 +795,7 @@ struct FeedForwardBackward : torch::autograd::Node {
         return {g.dx, g.dw1, g.db1, g.dw2, g.db2, task_should_compute_output(5) ? grads[0] : Tensor()};
     }
     void release_variables() override {
-        x.reset_data(); w1.reset_data(); pre.reset_data(); h.reset_data(); w2.reset_data();
+        x.reset_data(); w1.reset_data(); slope.reset_data(); h.reset_data(); w2.reset_data();
     }
     std::string name() const override { return "FeedForwardBackward"; }
 };
@@ -815,7 +815,7 @@ Tensor feed_forward(const Tensor& x, const Tensor& w1, const Tensor& b1, const T
         node->set_next_edges(torch::autograd::collect_next_edges(x, w1, b1, w2, b2, residual));
         node->x = SavedVariable(x, false);
         node->w1 = SavedVariable(w1, false);
-        node->pre = SavedVariable(hidden.pre, false);
+        node->slope = SavedVariable(hidden.slope, false);
         node->h = SavedVariable(hidden.y, false);
         node->w2 = SavedVariable(w2, false);
         if (b1.defined()) node->b1_type = b1.scalar_type();
@@ -1211,7 +1211,7 @@ PyObject* py_fused_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
         return wrap(y);
     });
 }
-// (x, w, bias, activation, residual, keep_preact) -> (y, preact)
+// (x, w, bias, activation, residual, keep_slope) -> (y, slope)
 PyObject* py_fused_linear_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         want(n, 6);
@@ -1225,22 +1225,22 @@ PyObject* py_fused_linear_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
             at::AutoDispatchBelowADInplaceOrView below;
             r = fused_linear_forward(x, w, bias, act, residual, keep);
         }
-        return wrap_tuple({&r.y, &r.pre});
+        return wrap_tuple({&r.y, &r.slope});
     });
 }
-// (x, w, dy, preact, activation, need_dx, need_dw, need_db) -> (dx, dw, db)
+// (x, w, dy, slope, activation, need_dx, need_dw, need_db) -> (dx, dw, db)
 PyObject* py_fused_linear_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         want(n, 8);
         const Tensor &x = arg_tensor(a[0]), &w = arg_tensor(a[1]), &dy = arg_tensor(a[2]);
-        const Tensor pre = arg_opt_tensor(a[3]);
+        const Tensor slope = arg_opt_tensor(a[3]);
         const int act = arg_activation(a[4]);
         const bool need_dx = arg_bool(a[5]), need_dw = arg_bool(a[6]), need_db = arg_bool(a[7]);
         LinearGrads g;
         {
             pybind11::gil_scoped_release nogil;
             at::AutoDispatchBelowADInplaceOrView below;
-            g = fused_linear_backward(x, w, dy, pre, act, need_dx, need_dw, need_db, false);
+            g = fused_linear_backward(x, w, dy, slope, act, need_dx, need_dw, need_db, false);
         }
         return wrap_tuple({&g.dx, &g.dw, &g.db});
     });

@@ -9,10 +9,10 @@
 // layernorm_input_grad_kernel and its layernorm_param_grad_kernel, which reads x and dy a second time
 // (src/inferno/cuda/cudalayernorm.cu:16-160, 212-400; modules: src/inferno/modules/layernorm.cpp:25-98).
 //
-// Memory-bound: a row is read once into registers, and everything is computed from there, so the variance is the sum of squared
-// differences from the mean and not a difference of two sums.  A row belongs to 32, 128, 256 or 512 threads (LnShape), each of which holds
-// up to four 16-byte chunks of it: a row of one warp needs no barrier.  The backward's threads keep their columns from row to row and
-// sum dw and db in registers; a block's sums meet in the workspace, which ln_finish_kernel adds up in a fixed order.  All sums are
+// Memory-bound: a row is read from global memory once, into the ring, and everything is computed from there, so the variance is the sum of
+// squared differences from the mean and not a difference of two sums.  A row belongs to 32, 64, 128, 256 or 512 threads (LnShape), each of
+// which has up to four 16-byte chunks of it: a row of one warp needs no barrier.  The backward's threads keep their columns from row to row
+// and sum dw and db in registers; a block's sums meet in the workspace, which ln_finish_kernel adds up in a fixed order.  All sums are
 // fp32; the only rounding to fewer bits is that of the results.
 #pragma once
 
@@ -40,19 +40,25 @@ struct LnRows {
     float eps;
 };
 
-// TPR threads per row, chunks of 16 bytes, NV of them per thread.  ALIGNED: rows begin on 16 bytes and hold whole chunks; a thread's chunk
-// is then 16 contiguous bytes.  Otherwise the same columns are dealt out element by element, so that a warp's loads still run together.
-template <class T_, int TPR_, int NV_, bool ALIGNED_>
+// TPR threads per row, chunks of 16 bytes, NV of them per thread.  PT: type of weight and bias.  ALIGNED: rows begin on 16 bytes and hold whole
+// chunks, and so do weight and bias; a thread's chunk is then 16 contiguous bytes.  Otherwise the same columns are dealt out element by
+// element, so that a warp's loads still run together, and the type of weight and bias is looked up.
+constexpr int kLnBwdThreads = 512;      // a block of the backward, one per SM: as few blocks' sums as there can be
+template <class T_, class PT_, int TPR_, int NV_, bool ALIGNED_>
 struct LnShape {
     using T = T_;
+    using PT = PT_;
     static constexpr int TPR = TPR_, NV = NV_, VEC = 16 / sizeof(T_), WARPS = TPR_ / 32;
     static constexpr bool ALIGNED = ALIGNED_;
-    static constexpr int THREADS = TPR_ == 32 ? 256 : TPR_, ROWS = THREADS / TPR_;      // per block
+    static constexpr int FWD_THREADS = TPR_ < 256 ? 256 : TPR_, FWD_ROWS = FWD_THREADS / TPR_, FWD_BLOCKS = 1024 / FWD_THREADS;      // blocks resident per SM
+    static constexpr int BWD_ROWS = kLnBwdThreads / TPR_;
     static constexpr int CHUNK_COLS = TPR_ * VEC;                                       // columns of one chunk of all threads
-    static constexpr int FWD_BLOCKS = TPR_ == 512 ? 1 : (NV_ < 4 ? 768 : 512) / THREADS, BWD_BLOCKS = 512 / THREADS;      // resident per SM
-    static constexpr int FWD_STAGES = 4, BWD_STAGES = 3;                                // rows of a thread's ring
-    static constexpr int FWD_SMEM = ALIGNED_ ? FWD_STAGES * NV_ * THREADS * 16 : 0;
-    static constexpr int BWD_SMEM = ALIGNED_ ? BWD_STAGES * 2 * NV_ * THREADS * 16 : 0;
+    static constexpr int STAGES = 2;                                                    // rows of a thread's ring: this one and the next
+    static constexpr int PARAM_UNITS = sizeof(PT_) * VEC / 16 ? sizeof(PT_) * VEC / 16 : 1;      // 16-byte units of a chunk's weights
+    static constexpr int FWD_SMEM = ALIGNED_ ? STAGES * NV_ * FWD_THREADS * 16 : 0;
+    static constexpr int BWD_RING = ALIGNED_ ? (STAGES * 2 + PARAM_UNITS) * NV_ * kLnBwdThreads * 16 : 0;
+    static constexpr int BWD_SUMS = kLnBwdThreads * VEC * 4;                            // one chunk's columns of every row at work, in the ring's place
+    static constexpr int BWD_SMEM = BWD_RING > BWD_SUMS ? BWD_RING : BWD_SUMS;
 };
 
 __device__ __forceinline__ float ln_to_float(float v) { return v; }
@@ -91,28 +97,34 @@ __device__ __forceinline__ void ln_gather(const P* p, float none, int v, int t, 
         k.f[e / 2] = pack_f32x2(c0 < C ? ln_to_float(p[c0]) : none, c1 < C ? ln_to_float(p[c1]) : none);
     }
 }
-// The same columns of weight or bias: after the first row they come from L1.
+// The same columns of weight or bias, `none` where there is none.
+template <class S>
+__device__ __forceinline__ void ln_unpack_param(const uint4 (&u)[S::PARAM_UNITS], LnChunk<S>& k) {
+    if constexpr (sizeof(typename S::PT) == 4) {
+#pragma unroll
+        for (int q = 0; q < S::VEC / 4; ++q) {
+            k.f[2 * q] = pack_f32x2(__uint_as_float(u[q].x), __uint_as_float(u[q].y));
+            k.f[2 * q + 1] = pack_f32x2(__uint_as_float(u[q].z), __uint_as_float(u[q].w));
+        }
+    } else {
+        const uint32_t w[4] = {u[0].x, u[0].y, u[0].z, u[0].w};
+#pragma unroll
+        for (int i = 0; i < S::VEC / 2; ++i) k.f[i] = ln_pair_bf16(w[i]);
+    }
+}
 template <class S>
 __device__ __forceinline__ void ln_load_param(const void* p, int bf16, float none, int v, int t, int C, LnChunk<S>& k) {
     if constexpr (S::ALIGNED) {
         const int c = ln_col<S>(v, 0, t);
-        if (!p || c >= C) {
+        if (p && c < C) {
+            const uint4* src = reinterpret_cast<const uint4*>(static_cast<const typename S::PT*>(p) + c);
+            uint4 u[S::PARAM_UNITS];
 #pragma unroll
-            for (int i = 0; i < S::VEC / 2; ++i) k.f[i] = pack_f32x2(none, none);
-        } else if (bf16) {
-#pragma unroll
-            for (int q = 0; q < S::VEC / 4; ++q) {
-                const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p) + c + 4 * q);
-                k.f[2 * q] = ln_pair_bf16(u.x);
-                k.f[2 * q + 1] = ln_pair_bf16(u.y);
-            }
+            for (int q = 0; q < S::PARAM_UNITS; ++q) u[q] = src[q];
+            ln_unpack_param<S>(u, k);
         } else {
 #pragma unroll
-            for (int q = 0; q < S::VEC / 4; ++q) {
-                const float4 u = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + c + 4 * q);
-                k.f[2 * q] = pack_f32x2(u.x, u.y);
-                k.f[2 * q + 1] = pack_f32x2(u.z, u.w);
-            }
+            for (int i = 0; i < S::VEC / 2; ++i) k.f[i] = pack_f32x2(none, none);
         }
     } else if (!p) {
 #pragma unroll
@@ -150,7 +162,7 @@ __device__ __forceinline__ float ln_pair_sum(uint64_t p) {
 }
 
 // Sums of a (and b) over the threads of a row.  `turn` alternates between two sets of slots, so that one barrier per sum is enough: a slot
-// is written again only after the next sum's barrier, which every thread reaches after it has read.
+// is written again only after the next sum's barrier, which every thread reaches after it has read.  Each row of a block has a barrier of its own.
 template <class S, bool BOTH>
 __device__ __forceinline__ float2 ln_row_sum(float a, float b, float2 (*slots)[16], int turn) {
 #pragma unroll
@@ -159,14 +171,15 @@ __device__ __forceinline__ float2 ln_row_sum(float a, float b, float2 (*slots)[1
         if (BOTH) b += __shfl_xor_sync(0xffffffffu, b, m);
     }
     if constexpr (S::WARPS > 1) {
+        const int warp = threadIdx.x >> 5, first = warp / S::WARPS * S::WARPS;
         float2* s = slots[turn & 1];
-        if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = make_float2(a, b);
-        __syncthreads();
+        if ((threadIdx.x & 31) == 0) s[warp] = make_float2(a, b);
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / S::WARPS), "n"(S::TPR) : "memory");
         a = b = 0.f;
 #pragma unroll
         for (int w = 0; w < S::WARPS; ++w) {
-            a += s[w].x;
-            if (BOTH) b += s[w].y;
+            a += s[first + w].x;
+            if (BOTH) b += s[first + w].y;
         }
     }
     return make_float2(a, b);
@@ -181,77 +194,78 @@ __device__ __forceinline__ void ln_copy_async(uint4* dst, const void* src, bool 
 __device__ __forceinline__ void ln_copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int PENDING>
 __device__ __forceinline__ void ln_copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
-template <class S>
+template <class S, int THREADS>
 __device__ __forceinline__ void ln_request(uint4* slots, const typename S::T* row, int t, int C) {
 #pragma unroll
     for (int v = 0; v < S::NV; ++v) {
         const int c = ln_col<S>(v, 0, t);
-        ln_copy_async(slots + v * S::THREADS + threadIdx.x, row + (c < C ? c : 0), c < C);
+        ln_copy_async(slots + v * THREADS + threadIdx.x, row + (c < C ? c : 0), c < C);
     }
 }
 
 template <class S>
-__global__ void __launch_bounds__(S::THREADS, S::FWD_BLOCKS) ln_fwd_kernel(const LnRows p) {
+__global__ void __launch_bounds__(S::FWD_THREADS, S::FWD_BLOCKS) ln_fwd_kernel(const LnRows p) {
     using T = typename S::T;
-    constexpr int ST = S::FWD_STAGES;
     extern __shared__ uint4 ring[];
     __shared__ float2 slots[2][16];
     pdl_wait();
     pdl_trigger();
     const int t = threadIdx.x % S::TPR;
-    const long first = static_cast<long>(blockIdx.x) * S::ROWS + threadIdx.x / S::TPR, step = static_cast<long>(gridDim.x) * S::ROWS;
+    const long first = static_cast<long>(blockIdx.x) * S::FWD_ROWS + threadIdx.x / S::TPR, step = static_cast<long>(gridDim.x) * S::FWD_ROWS;
     const T* x0 = static_cast<const T*>(p.x);
     if constexpr (S::ALIGNED) {
-#pragma unroll
-        for (int s = 0; s < ST - 1; ++s) {
-            const long r = first + s * step;
-            if (r < p.M) ln_request<S>(ring + s * S::NV * S::THREADS, x0 + r * p.x_pitch, t, p.C);
-            ln_copy_commit();
-        }
+        if (first < p.M) ln_request<S, S::FWD_THREADS>(ring, x0 + first * p.x_pitch, t, p.C);
+        ln_copy_commit();
     }
     const float inv = 1.f / static_cast<float>(p.C);
     int stage = 0;
     for (long r = first; r < p.M; r += step) {
-        LnChunk<S> x[S::NV];
         if constexpr (S::ALIGNED) {
-            const long ra = r + (ST - 1) * step;
-            const int sa = stage == 0 ? ST - 1 : stage - 1;          // the slot that was read last
-            if (ra < p.M) ln_request<S>(ring + sa * S::NV * S::THREADS, x0 + ra * p.x_pitch, t, p.C);
+            if (r + step < p.M) ln_request<S, S::FWD_THREADS>(ring + (stage ^ 1) * S::NV * S::FWD_THREADS, x0 + (r + step) * p.x_pitch, t, p.C);
             ln_copy_commit();
-            ln_copy_wait<ST - 1>();
-#pragma unroll
-            for (int v = 0; v < S::NV; ++v) ln_unpack(ring[(stage * S::NV + v) * S::THREADS + threadIdx.x], x[v].f);
-            if (++stage == ST) stage = 0;
-        } else {
-#pragma unroll
-            for (int v = 0; v < S::NV; ++v) ln_gather<S>(x0 + r * p.x_pitch, 0.f, v, t, p.C, x[v]);
+            ln_copy_wait<1>();
         }
+        // A chunk of the row, less `minus`; zeros past the row's end.  Read again in each of the three passes rather than held in fp32: with 32 registers
+        // less there are twice as many rows at work on an SM.
+        auto chunk = [&](int v, uint64_t minus, bool centred, LnChunk<S>& x) {
+            if constexpr (S::ALIGNED) {
+                ln_unpack(ring[(stage * S::NV + v) * S::FWD_THREADS + threadIdx.x], x.f);
+            } else {
+                ln_gather<S>(x0 + r * p.x_pitch, 0.f, v, t, p.C, x);
+            }
+            if (!centred) return;
+#pragma unroll
+            for (int i = 0; i < S::VEC / 2; ++i) x.f[i] = fadd2(x.f[i], minus);
+        };
         uint64_t s = 0;
 #pragma unroll
-        for (int v = 0; v < S::NV; ++v)
+        for (int v = 0; v < S::NV; ++v) {
+            LnChunk<S> x;
+            chunk(v, 0, false, x);
 #pragma unroll
-            for (int i = 0; i < S::VEC / 2; ++i) s = fadd2(s, x[v].f[i]);
+            for (int i = 0; i < S::VEC / 2; ++i) s = fadd2(s, x.f[i]);
+        }
         const float mean = ln_row_sum<S, false>(ln_pair_sum(s), 0.f, slots, 0).x * inv;
         const uint64_t minus = pack_f32x2(-mean, -mean);
         uint64_t q = 0, left = 0;
 #pragma unroll
         for (int v = 0; v < S::NV; ++v) {
-#pragma unroll
-            for (int i = 0; i < S::VEC / 2; ++i) x[v].f[i] = fadd2(x[v].f[i], minus);
+            LnChunk<S> x;
+            chunk(v, minus, true, x);
             if constexpr (S::ALIGNED) {
                 if (ln_col<S>(v, 0, t) >= p.C) continue;
             } else {
 #pragma unroll
                 for (int e = 0; e < S::VEC; e += 2) {
                     float a, b;
-                    unpack_f32x2(x[v].f[e / 2], a, b);
-                    x[v].f[e / 2] = pack_f32x2(ln_col<S>(v, e, t) < p.C ? a : 0.f, ln_col<S>(v, e + 1, t) < p.C ? b : 0.f);
+                    unpack_f32x2(x.f[e / 2], a, b);
+                    x.f[e / 2] = pack_f32x2(ln_col<S>(v, e, t) < p.C ? a : 0.f, ln_col<S>(v, e + 1, t) < p.C ? b : 0.f);
                 }
             }
 #pragma unroll
             for (int i = 0; i < S::VEC / 2; ++i) {
-                q = ffma2(x[v].f[i], x[v].f[i], q);
-                left = fadd2(left, x[v].f[i]);
+                q = ffma2(x.f[i], x.f[i], q);
+                left = fadd2(left, x.f[i]);
             }
         }
         // what rounding has left of the mean: it counts where a row's mean is much larger than its spread
@@ -266,43 +280,51 @@ __global__ void __launch_bounds__(S::THREADS, S::FWD_BLOCKS) ln_fwd_kernel(const
         T* out = static_cast<T*>(p.out) + r * p.C;
 #pragma unroll
         for (int v = 0; v < S::NV; ++v) {
-            LnChunk<S> w, b;
+            LnChunk<S> x, w, b;
             ln_load_param<S>(p.w, p.param_bf16, 1.f, v, t, p.C, w);
             ln_load_param<S>(p.b, p.param_bf16, 0.f, v, t, p.C, b);
+            chunk(v, minus, true, x);
 #pragma unroll
-            for (int i = 0; i < S::VEC / 2; ++i) x[v].f[i] = ffma2(ffma2(x[v].f[i], scale, shift), w.f[i], b.f[i]);
-            ln_store<S>(out, v, t, p.C, x[v]);
+            for (int i = 0; i < S::VEC / 2; ++i) x.f[i] = ffma2(ffma2(x.f[i], scale, shift), w.f[i], b.f[i]);
+            ln_store<S>(out, v, t, p.C, x);
         }
+        stage ^= 1;
     }
 }
 
 template <class S>
-__global__ void __launch_bounds__(S::THREADS, S::BWD_BLOCKS) ln_bwd_kernel(const LnRows p) {
+__global__ void __launch_bounds__(kLnBwdThreads, 1) ln_bwd_kernel(const LnRows p) {
     using T = typename S::T;
-    constexpr int ST = S::BWD_STAGES, ROW = 2 * S::NV * S::THREADS;
+    constexpr int ROW = 2 * S::NV * kLnBwdThreads;
     extern __shared__ uint4 ring[];
     __shared__ float2 slots[2][16];
     pdl_wait();
     pdl_trigger();
     const int t = threadIdx.x % S::TPR;
-    const long first = static_cast<long>(blockIdx.x) * S::ROWS + threadIdx.x / S::TPR, step = static_cast<long>(gridDim.x) * S::ROWS;
+    const long first = static_cast<long>(blockIdx.x) * S::BWD_ROWS + threadIdx.x / S::TPR, step = static_cast<long>(gridDim.x) * S::BWD_ROWS;
     const T *x0 = static_cast<const T*>(p.x), *g0 = static_cast<const T*>(p.dy);
     auto request = [&](int s, long r) {
-        ln_request<S>(ring + s * ROW, x0 + r * p.x_pitch, t, p.C);
-        ln_request<S>(ring + s * ROW + S::NV * S::THREADS, g0 + r * p.dy_pitch, t, p.C);
+        ln_request<S, kLnBwdThreads>(ring + s * ROW, x0 + r * p.x_pitch, t, p.C);
+        ln_request<S, kLnBwdThreads>(ring + s * ROW + S::NV * kLnBwdThreads, g0 + r * p.dy_pitch, t, p.C);
     };
+    uint4* wsave = ring + S::STAGES * ROW;      // the thread's weights
     float mean = 0.f, rstd = 0.f;
     if (first < p.M) {
         mean = p.mean[first];
         rstd = p.rstd[first];
     }
     if constexpr (S::ALIGNED) {
+        if (p.w) {
 #pragma unroll
-        for (int s = 0; s < ST - 1; ++s) {
-            const long r = first + s * step;
-            if (r < p.M) request(s, r);
-            ln_copy_commit();
+            for (int v = 0; v < S::NV; ++v) {
+                const int c = ln_col<S>(v, 0, t);
+                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const typename S::PT*>(p.w) + (c < p.C ? c : 0));
+#pragma unroll
+                for (int q = 0; q < S::PARAM_UNITS; ++q) ln_copy_async(wsave + (v * S::PARAM_UNITS + q) * kLnBwdThreads + threadIdx.x, src + q, c < p.C);
+            }
         }
+        if (first < p.M) request(0, first);
+        ln_copy_commit();
     }
     const float inv = 1.f / static_cast<float>(p.C);
     LnChunk<S> dw2[S::NV], db2[S::NV];
@@ -318,17 +340,31 @@ __global__ void __launch_bounds__(S::THREADS, S::BWD_BLOCKS) ln_bwd_kernel(const
             next_rstd = p.rstd[r + step];
         }
         if constexpr (S::ALIGNED) {
-            const long ra = r + (ST - 1) * step;
-            if (ra < p.M) request(stage == 0 ? ST - 1 : stage - 1, ra);          // the slot that was read last
+            if (r + step < p.M) request(stage ^ 1, r + step);
             ln_copy_commit();
-            ln_copy_wait<ST - 1>();
+            ln_copy_wait<1>();
         }
+        auto weight = [&](int v, LnChunk<S>& w) {
+            if constexpr (S::ALIGNED) {
+                if (p.w) {
+                    uint4 u[S::PARAM_UNITS];
+#pragma unroll
+                    for (int q = 0; q < S::PARAM_UNITS; ++q) u[q] = wsave[(v * S::PARAM_UNITS + q) * kLnBwdThreads + threadIdx.x];
+                    ln_unpack_param<S>(u, w);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < S::VEC / 2; ++i) w.f[i] = pack_f32x2(1.f, 1.f);
+                }
+            } else {
+                ln_load_param<S>(p.w, p.param_bf16, 1.f, v, t, p.C, w);
+            }
+        };
         // One chunk of both rows, xh and g: read again for the second pass rather than held, which would cost the registers that the sums are in.
         const uint64_t scale = pack_f32x2(rstd, rstd), minus = pack_f32x2(-mean, -mean);
         auto chunk = [&](int v, LnChunk<S>& x, LnChunk<S>& g) {
             if constexpr (S::ALIGNED) {
-                ln_unpack(ring[stage * ROW + v * S::THREADS + threadIdx.x], x.f);
-                ln_unpack(ring[stage * ROW + (S::NV + v) * S::THREADS + threadIdx.x], g.f);
+                ln_unpack(ring[stage * ROW + v * kLnBwdThreads + threadIdx.x], x.f);
+                ln_unpack(ring[stage * ROW + (S::NV + v) * kLnBwdThreads + threadIdx.x], g.f);
             } else {
                 ln_gather<S>(x0 + r * p.x_pitch, 0.f, v, t, p.C, x);
                 ln_gather<S>(g0 + r * p.dy_pitch, 0.f, v, t, p.C, g);
@@ -341,7 +377,7 @@ __global__ void __launch_bounds__(S::THREADS, S::BWD_BLOCKS) ln_bwd_kernel(const
         for (int v = 0; v < S::NV; ++v) {
             LnChunk<S> x, g, w;
             chunk(v, x, g);
-            ln_load_param<S>(p.w, p.param_bf16, 1.f, v, t, p.C, w);
+            weight(v, w);
 #pragma unroll
             for (int i = 0; i < S::VEC / 2; ++i) {
                 dw2[v].f[i] = ffma2(g.f[i], x.f[i], dw2[v].f[i]);
@@ -361,7 +397,7 @@ __global__ void __launch_bounds__(S::THREADS, S::BWD_BLOCKS) ln_bwd_kernel(const
             for (int v = 0; v < S::NV; ++v) {
                 LnChunk<S> x, g, w;
                 chunk(v, x, g);
-                ln_load_param<S>(p.w, p.param_bf16, 1.f, v, t, p.C, w);
+                weight(v, w);
 #pragma unroll
                 for (int i = 0; i < S::VEC / 2; ++i) g.f[i] = ffma2(fmul2(g.f[i], w.f[i]), scale, ffma2(x.f[i], slope, add));
                 ln_store<S>(out, v, t, p.C, g);
@@ -369,69 +405,54 @@ __global__ void __launch_bounds__(S::THREADS, S::BWD_BLOCKS) ln_bwd_kernel(const
         }
         mean = next_mean;
         rstd = next_rstd;
-        if (++stage == ST) stage = 0;
+        stage ^= 1;
     }
     if (!p.part) return;
-    float dw[S::NV][S::VEC], db[S::NV][S::VEC];
+    // The rows at work have the same columns: a chunk of each is laid out in the ring's place and added up, dw first, then db.
+    float* part = p.part + static_cast<long>(blockIdx.x) * 2 * p.C;
+    float* sums = reinterpret_cast<float*>(ring) + threadIdx.x / S::TPR * S::CHUNK_COLS;
+    ln_copy_wait<0>();
 #pragma unroll
     for (int v = 0; v < S::NV; ++v)
 #pragma unroll
-        for (int i = 0; i < S::VEC / 2; ++i) {
-            unpack_f32x2(dw2[v].f[i], dw[v][2 * i], dw[v][2 * i + 1]);
-            unpack_f32x2(db2[v].f[i], db[v][2 * i], db[v][2 * i + 1]);
+        for (int which = 0; which < 2; ++which) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < S::VEC / 2; ++i) {
+                float lo, hi;
+                unpack_f32x2(which ? db2[v].f[i] : dw2[v].f[i], lo, hi);
+                sums[ln_col<S>(0, 2 * i, t)] = lo;
+                sums[ln_col<S>(0, 2 * i + 1, t)] = hi;
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < S::CHUNK_COLS; i += kLnBwdThreads) {
+                const int c = v * S::CHUNK_COLS + i;
+                float a = 0.f;
+#pragma unroll
+                for (int w = 0; w < S::BWD_ROWS; ++w) a += reinterpret_cast<const float*>(ring)[w * S::CHUNK_COLS + i];
+                if (c < p.C) part[which * p.C + c] = a;
+            }
         }
-    float* part = p.part + static_cast<long>(blockIdx.x) * 2 * p.C;
-    if constexpr (S::ROWS == 1) {
-#pragma unroll
-        for (int v = 0; v < S::NV; ++v)
-#pragma unroll
-            for (int e = 0; e < S::VEC; ++e) {
-                const int c = ln_col<S>(v, e, t);
-                if (c < p.C) {
-                    part[c] = dw[v][e];
-                    part[p.C + c] = db[v][e];
-                }
-            }
-    } else {
-        // the block's warps have the same columns: add them up a chunk at a time
-        __shared__ float sums[S::ROWS][S::CHUNK_COLS + 4];
-#pragma unroll
-        for (int v = 0; v < S::NV; ++v)
-#pragma unroll
-            for (int which = 0; which < 2; ++which) {
-                __syncthreads();
-#pragma unroll
-                for (int e = 0; e < S::VEC; ++e) sums[threadIdx.x >> 5][ln_col<S>(0, e, t)] = which ? db[v][e] : dw[v][e];
-                __syncthreads();
-                for (int i = threadIdx.x; i < S::CHUNK_COLS; i += S::THREADS) {
-                    const int c = v * S::CHUNK_COLS + i;
-                    float a = 0.f;
-#pragma unroll
-                    for (int w = 0; w < S::ROWS; ++w) a += sums[w][i];
-                    if (c < p.C) part[which * p.C + c] = a;
-                }
-            }
-    }
 }
 
-// dw and db from the blocks' sums, in the order of the blocks: 32 columns a block, eight threads a column; grid y 0: dw, 1: db.
+// dw and db from the blocks' sums, in the order of the blocks: 32 columns a block, sixteen threads a column; grid y 0: dw, 1: db.
 constexpr int kLnFinishCols = 32;
-__global__ void __launch_bounds__(256) ln_finish_kernel(const float* __restrict__ part, int blocks, int C, void* __restrict__ dw, void* __restrict__ db, int bf16) {
+__global__ void __launch_bounds__(512) ln_finish_kernel(const float* __restrict__ part, int blocks, int C, void* __restrict__ dw, void* __restrict__ db, int bf16) {
     pdl_wait();
     pdl_trigger();
-    __shared__ float sums[8][kLnFinishCols];
+    __shared__ float sums[16][kLnFinishCols];
     void* out = blockIdx.y ? db : dw;
     if (!out) return;
     const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5, c = blockIdx.x * kLnFinishCols + lane;
     float s = 0.f;
     if (c < C)
-#pragma unroll 8
-        for (int j = grp; j < blocks; j += 8) s += part[(static_cast<long>(j) * 2 + blockIdx.y) * C + c];
+#pragma unroll 10
+        for (int j = grp; j < blocks; j += 16) s += part[(static_cast<long>(j) * 2 + blockIdx.y) * C + c];
     sums[grp][lane] = s;
     __syncthreads();
     if (grp == 0 && c < C) {
 #pragma unroll
-        for (int g = 1; g < 8; ++g) s += sums[g][lane];
+        for (int g = 1; g < 16; ++g) s += sums[g][lane];
         if (bf16) static_cast<__nv_bfloat16*>(out)[c] = __float2bfloat16(s);
         else static_cast<float*>(out)[c] = s;
     }

@@ -27,10 +27,13 @@
 //   (a weight gradient: K = tokens), into contiguous runs of k-slices, one per CTA pair, sized so that every pair ends up
 //   with the same number of k-slices over both tasks.  The partial tiles meet by TMA reduction: in an fp32 workspace, zeroed
 //   before and rounded once to bf16 afterwards by linear_finish_kernel, or, for callers without a workspace, in the zeroed
-//   bf16 output itself (one rounding per partial, at most eight).
+//   bf16 output itself (one rounding per partial, at most eight).  A forward with a fused epilogue is cut into equal parts, each with an fp32
+//   matrix of its own, which linear_fused_finish_kernel adds up in order: nothing to zero, and the result repeats.
 #pragma once
 
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "sm100_ptx.cuh"
 
@@ -41,8 +44,8 @@ namespace ib200 {
 enum : int {
     kEpiBias = 0,          // c = acc + bias
     kEpiResidual = 1,      // c = acc + bias + aux
-    kEpiGelu = 2,          // z = acc + bias;  c = gelu(z) (+ aux);  z kept as fp16 if it is wanted
-    kEpiSlope = 3,         // c = acc gelu'(z) with z = aux, and the column sums of c
+    kEpiGelu = 2,          // z = acc + bias;  c = gelu(z) (+ aux);  gelu'(z) kept as fp16 if it is wanted
+    kEpiSlope = 3,         // c = acc aux with aux = gelu'(z), and the column sums of c
 };
 
 struct GemmTraits {
@@ -75,20 +78,23 @@ struct GemmTask {
     int tiles_m, tiles;    // tiles = 0: no such task
     int k_slices;          // of 64
     int a_mn, b_mn;
+    int band_tiles;        // tiles of a band of eight tile rows, and its reciprocal
+    float band_inv;
 };
 
-enum : int { kPartWhole = 0, kPartReduceBf16 = 1, kPartReduceF32 = 2 };
+enum : int { kPartWhole = 0, kPartReduceBf16 = 1, kPartReduceF32 = 2, kPartSlab = 3 };
 
 struct GemmParams {
     GemmTask t[2];
     int split;             // task 1: kPartWhole, or how partial tiles are added up
     // split runs: pair c starts at k-slice total1 * (min(c, heavy) * w_heavy + max(0, c - heavy) * w_light) / w_total of task 1
+    int slabs;             // kPartSlab: parts of a tile
     int heavy;
     long long w_heavy, w_light, w_total;
     const void* bias;      // [N] of task 0 (task 1 when it is the only one), or null
     int bias_bf16;
     int has_aux;           // kEpiGelu: a residual is added
-    int write_pre;         // kEpiGelu: z is kept
+    int keep_slope;        // kEpiGelu: gelu'(z) is kept
     float* colsum;         // kEpiSlope: column sums of each 32 rows, [ceil(M / 32)][N], or null
     int* status;
 };
@@ -138,22 +144,27 @@ struct GemmWalk {
         }
         // tiles are numbered in bands of eight tile rows, so that the pairs at work share few rows of A and few columns of B in L2
         // (16384 x 768 x 2304 and 8192^3: 3 % and 5 % over one column of tiles after the other)
-        const int tm = p.t[q.task].tiles_m, tn = p.t[q.task].tiles / tm;
-        const int band = t / (kBandRows * tn), r = t - band * (kBandRows * tn), rows = min(kBandRows, tm - band * kBandRows);
-        q.m0 = (band * kBandRows + r % rows) * GemmTraits::BM;
-        q.n0 = (r / rows) * GemmTraits::BN;
+        // (the quotient by its reciprocal, put right by one where that was off: integer divisions cost an epilogue warp 500 cycles a tile)
+        const GemmTask& k = p.t[q.task];
+        int band = static_cast<int>(static_cast<float>(t) * k.band_inv), r = t - band * k.band_tiles;
+        if (r < 0) { --band; r += k.band_tiles; }
+        if (r >= k.band_tiles) { ++band; r -= k.band_tiles; }
+        const int rows = min(kBandRows, k.tiles_m - band * kBandRows);
+        const int down = rows == kBandRows ? r / kBandRows : r / rows;
+        q.m0 = (band * kBandRows + r - down * rows) * GemmTraits::BM;
+        q.n0 = down * GemmTraits::BN;
         return true;
     }
 };
 
 // The tensor maps of a launch: operands and outputs of the two tasks, and what a split task 1 is added into (its bf16 output,
-// or the fp32 accumulation workspace).
-// aux: what a fused epilogue reads beside its tile; pre: where it keeps z.
+// the fp32 accumulation workspace) or, slab by slab, stored to.
+// aux: what a fused epilogue reads beside its tile; keep: where it leaves gelu'(z).
 struct GemmMaps {
-    CUtensorMap a[2], b[2], c[2], sum, aux, pre;
+    CUtensorMap a[2], b[2], c[2], sum, aux, keep;
 };
 
-// Two columns of bias (col is even) as they are stored, converted where they are used: the load then waits for nobody.
+// Two columns of bias (col is even) as they are stored: converted where they are used, the load waits for nobody.
 __device__ __forceinline__ uint2 load_bias2(const GemmParams& p, int col) {
     if (!p.bias_bf16) return *reinterpret_cast<const uint2*>(static_cast<const float*>(p.bias) + col);
     return make_uint2(*reinterpret_cast<const uint32_t*>(static_cast<const __nv_bfloat16*>(p.bias) + col), 0u);
@@ -176,19 +187,21 @@ __device__ __forceinline__ uint64_t gelu_gate2(uint64_t z, uint64_t zz) {       
     return pack_f32x2(fast_rcp(a), fast_rcp(b));
 }
 __device__ __forceinline__ uint64_t gelu2(uint64_t z) { return fmul2(z, gelu_gate2(z, fmul2(z, z))); }
-__device__ __forceinline__ uint64_t gelu_slope2(uint64_t z) {                        // |z| <= kPreactLimit
-    const uint64_t zz = fmul2(z, z), s = gelu_gate2(z, zz);
-    return ffma2(fmul2(z, ffma2(splat2(kGeluDu3), zz, splat2(kGeluDu1))), fmul2(s, ffma2(s, splat2(-1.f), splat2(1.f))), s);
-}
-// z is kept for the backward in fp16: beyond 16 the slope is 0 or 1 to the last bit of an fp32, so it is kept as +-16 (NaN stays NaN), and within that
-// fp16 has three bits more than bf16.  With z in bf16 the gradients would be half as far off again as their own rounding leaves them.
-constexpr float kPreactLimit = 16.f;
-__device__ __forceinline__ uint32_t pack_preact2(uint64_t z) {
+// The backward needs gelu'(z) = s + z (2u)' s (1 - s) and nothing else of z, and all of it is at hand here, so the slope is what is kept, as
+// fp16: 2^-11 of itself, an eighth of what the gradient loses when it is rounded to bf16.  (With z kept as bf16 the gradients are half as far off
+// again as their rounding leaves them, and with z kept in any type their kernels pay for the exponentials once more: 8192 x 4096, dy -> dz
+// 62 us, 127 us for the product that does it in its epilogue.)  Beyond 16 the slope is 0 or 1 to the last bit, so z is limited
+// there, where the formula would meet infinity times zero; a NaN is kept by s.
+constexpr float kGeluFlat = 16.f;
+__device__ __forceinline__ uint64_t gelu_with_slope2(uint64_t z, uint32_t& slope) {
     float a, b;
     unpack_f32x2(z, a, b);
-    const __half2 lim = __float2half2_rn(kPreactLimit);
-    const __half2 h = __hmax2_nan(__hmin2_nan(__floats2half2_rn(a, b), lim), __hneg2(lim));
-    return *reinterpret_cast<const uint32_t*>(&h);
+    const uint64_t zc = pack_f32x2(clamp_abs(a, kGeluFlat), clamp_abs(b, kGeluFlat)), zz = fmul2(zc, zc);
+    const uint64_t s = gelu_gate2(z, zz);
+    unpack_f32x2(ffma2(fmul2(zc, ffma2(splat2(kGeluDu3), zz, splat2(kGeluDu1))), fmul2(s, ffma2(s, splat2(-1.f), splat2(1.f))), s), a, b);
+    const __half2 h = __floats2half2_rn(a, b);
+    slope = *reinterpret_cast<const uint32_t*>(&h);
+    return fmul2(z, s);
 }
 __device__ __forceinline__ uint64_t unpack_half2(uint32_t w) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
@@ -340,13 +353,10 @@ gemm_bf16_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ 
                 tma_load_3d(second, &maps.aux, &aux_full[warp], col, row, 0);
             }
         };
-        uint2 bias[8];
+        uint2 bias = make_uint2(0u, 0u);                         // of columns 2 lane, 2 lane + 1 of a step, handed round by shuffles
         auto request_bias = [&](const GemmPart& p, int c0) {
-            if (!prm.bias) return;
-            const int col = p.n0 + c0, N = prm.t[p.task].N;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (col + 8 * j < N) bias[j] = load_bias2(prm, col + 8 * j + pair_col);
+            const int col = p.n0 + c0 + 2 * lane;
+            if (EPI != kEpiSlope && prm.bias && col < prm.t[p.task].N) bias = load_bias2(prm, col);
         };
         auto tile_free = [&] {                                   // the last copies have read the staging tiles
             if (lane == 0) tma_store_wait_read_all();
@@ -363,7 +373,7 @@ gemm_bf16_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ 
             const bool fused = EPI != kEpiBias && q.task == 0;
             const uint32_t buf = n & 1;
             const int row = q.m0 + static_cast<int>(rank) * TR::CM + row0;
-            const bool with_bias = prm.bias && q.ks0 == 0;       // the part that starts the tile's K range brings the bias in
+            const bool with_bias = EPI != kEpiSlope && prm.bias && q.ks0 == 0;      // the part that starts the tile's K range brings the bias in
             mbar_wait(&acc_full[buf], (n >> 1) & 1, ab, 30);
             tc_fence_after_sync();
             GemmPart ahead;
@@ -372,17 +382,16 @@ gemm_bf16_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ 
             for (int c0 = colf; c0 < colf + BN / 2; c0 += 64) {
                 const int col = q.n0 + c0;
                 const bool inside = row < k.M && col < k.N, last = c0 != colf;
-                uint32_t a[8][4];
-                if (EPI != kEpiBias && has_aux && fused && inside) {
-                    mbar_wait(&aux_full[warp], aux_n & 1, ab, 31);
-                    ++aux_n;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) ld_matrix_sw128(second, lane, j, a[j]);
-                }
                 uint32_t r[2][32];
                 tmem_ld_16x256b_x8(tmem + buf * BN + c0 + lane_base, r[0]);
                 tmem_ld_16x256b_x8(tmem + buf * BN + c0 + lane_base + (16u << 16), r[1]);
                 tmem_wait_ld();
+                if (last) {
+                    // every column of the accumulator is in registers: hand it back to the MMA warp
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster_relaxed(free_bar[buf]);
+                }
                 // rows 8i + lane / 4, columns 8j + pair_col
                 uint64_t v[4][8];
 #pragma unroll
@@ -395,31 +404,28 @@ gemm_bf16_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ 
                 if (with_bias) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const uint64_t b = bias_pair(prm, bias[j]);
+                        const uint32_t lo = __shfl_sync(0xffffffffu, bias.x, 4 * j + (lane & 3));
+                        const uint64_t b = bias_pair(prm, make_uint2(lo, prm.bias_bf16 ? 0u : __shfl_sync(0xffffffffu, bias.y, 4 * j + (lane & 3))));
 #pragma unroll
                         for (int i = 0; i < 4; ++i) v[i][j] = fadd2(v[i][j], b);
                     }
                 }
                 if (last) {
-                    // every column of the accumulator is in registers: hand it back to the MMA warp
-                    tc_fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster_relaxed(free_bar[buf]);
                     more_ahead = walk.next(ahead);
-                    if (more_ahead) {
-                        request_aux(ahead, colf);
-                        request_bias(ahead, colf);
-                    }
+                    if (more_ahead) request_bias(ahead, colf);
                 } else {
-                    __syncwarp();                                // every lane has read the aux tile
-                    request_aux(q, c0 + 64);
                     request_bias(q, c0 + 64);
                 }
+                auto request_next_aux = [&] {                    // once every lane has read the tile that is there
+                    if (!last) request_aux(q, c0 + 64);
+                    else if (more_ahead) request_aux(ahead, colf);
+                };
+                if (!inside || !fused) request_next_aux();
                 if (!inside) continue;
                 tile_free();
                 if (!fused) {
                     const CUtensorMap* mc = q.partial ? &maps.sum : &maps.c[q.task];
-                    if (q.partial && prm.split == kPartReduceF32) {
+                    if (q.partial && prm.split >= kPartReduceF32) {
 #pragma unroll
                         for (int half = 0; half < 2; ++half) {
                             if (half) tile_free();
@@ -431,7 +437,9 @@ gemm_bf16_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ 
                             fence_proxy_async_smem();
                             __syncwarp();
                             if (lane == 0 && col + 32 * half < k.N) {
-                                tma_reduce_add_3d(mc, stage, col + 32 * half, row, 0);       // rows / columns past M / N are clipped by the copy
+                                // rows / columns past M / N are clipped by the copy
+                                if (prm.split == kPartSlab) tma_store_3d(mc, stage, col + 32 * half, row, pair % prm.slabs);
+                                else tma_reduce_add_3d(mc, stage, col + 32 * half, row, 0);
                                 tma_store_commit();
                             }
                         }
@@ -452,43 +460,56 @@ gemm_bf16_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ 
                     continue;
                 }
                 if constexpr (EPI != kEpiBias) {
-                    uint8_t* out = stage;
-                    if (EPI == kEpiGelu && prm.write_pre) {
+                    uint64_t sum[8];
+                    // One body for each combination: with the choice made element by element no two exponentials overlap (8192 x 1024 x 4096 with GELU
+                    // 53.7 -> 56.2 us, 16384 x 768 x 2304 54 -> 60).
+                    auto form = [&](auto keep_, auto aux_) {
+                        constexpr bool KEEP = decltype(keep_)::value, AUX = decltype(aux_)::value;
+                        uint32_t w[8][4];
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
-                            const uint32_t w[4] = {pack_preact2(v[0][j]), pack_preact2(v[1][j]), pack_preact2(v[2][j]), pack_preact2(v[3][j])};
-                            st_matrix_sw128(stage, lane, j, w);
+                            uint32_t slope[4], a[4];
+                            if (AUX) ld_matrix_sw128(second, lane, j, a);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                if (EPI == kEpiGelu) v[i][j] = KEEP ? gelu_with_slope2(v[i][j], slope[i]) : gelu2(v[i][j]);
+                                if (EPI == kEpiSlope) v[i][j] = fmul2(v[i][j], unpack_half2(a[i]));
+                                else if (AUX) v[i][j] = fadd2(v[i][j], unpack_bf16x2(a[i]));
+                                w[j][i] = pack_bf16_pair(v[i][j]);
+                            }
+                            if (EPI == kEpiSlope) sum[j] = fadd2(fadd2(v[0][j], v[1][j]), fadd2(v[2][j], v[3][j]));
+                            if (KEEP) st_matrix_sw128(stage, lane, j, slope);
+                            if (!KEEP || !AUX) st_matrix_sw128(KEEP ? second : stage, lane, j, w[j]);
                         }
                         fence_proxy_async_smem();
                         __syncwarp();
                         if (lane == 0) {
-                            tma_store_3d(&maps.pre, stage, col, row, 0);
+                            if (KEEP) tma_store_3d(&maps.keep, stage, col, row, 0);
+                            if (!KEEP || !AUX) tma_store_3d(&maps.c[0], KEEP ? second : stage, col, row, 0);
                             tma_store_commit();
                         }
-                        // gelu(z) goes out of the second tile, or, where that one is the residual's, out of the first again
-                        if (has_aux) tile_free();
-                        else out = second;
-                    }
-                    uint64_t sum[8];
+                        if (AUX) request_next_aux();
+                        if (KEEP && AUX) {               // the second tile is the residual's: c goes out of the first one, behind the slope
+                            tile_free();
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            if (EPI == kEpiGelu) v[i][j] = gelu2(v[i][j]);
-                            if (EPI == kEpiSlope) v[i][j] = fmul2(v[i][j], gelu_slope2(unpack_half2(a[j][i])));
-                            else if (has_aux) v[i][j] = fadd2(v[i][j], unpack_bf16x2(a[j][i]));
-                            w[i] = pack_bf16_pair(v[i][j]);
+                            for (int j = 0; j < 8; ++j) st_matrix_sw128(stage, lane, j, w[j]);
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                            if (lane == 0) {
+                                tma_store_3d(&maps.c[0], stage, col, row, 0);
+                                tma_store_commit();
+                            }
                         }
-                        if (EPI == kEpiSlope) sum[j] = fadd2(fadd2(v[0][j], v[1][j]), fadd2(v[2][j], v[3][j]));
-                        st_matrix_sw128(out, lane, j, w);
+                    };
+                    if (has_aux) {
+                        mbar_wait(&aux_full[warp], aux_n & 1, ab, 31);
+                        ++aux_n;
                     }
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        tma_store_3d(&maps.c[0], out, col, row, 0);
-                        tma_store_commit();
-                    }
+                    constexpr std::true_type yes{};
+                    constexpr std::false_type no{};
+                    if constexpr (EPI != kEpiGelu) form(no, yes);
+                    else if (prm.keep_slope) has_aux ? form(yes, yes) : form(yes, no);
+                    else has_aux ? form(no, yes) : form(no, no);
                     if (EPI == kEpiSlope && prm.colsum) {
                         // the eight lanes that share columns add up their rows' sums, each ending with one of the eight pairs (rows past M are zeros)
 #pragma unroll
@@ -524,18 +545,18 @@ gemm_bf16_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ 
 // the broadcast add, src/inferno/core/broadcastops.cpp) as one row of partial sums per row slab, and the zeroing of the
 // fp32 accumulation workspace.  Block (x, y): 256 columns, rows y * rows_per_block ...; a warp reads 512 contiguous bytes
 // of a row (16 bytes a lane) and keeps four rows in flight.  HBM-bound: one read of dY.
-// GELU: x is dy, `pre` the kept z; dz = dy gelu'(z) is written for the two products that follow, and its columns, not dy's, are summed
+// SLOPE: x is dy, `slope` the kept gelu'(z); dz = dy slope is written for the two products that follow, and its columns, not dy's, are summed
 // (before they are rounded): two reads and a write.
 constexpr int kColsumCols = 256, kMaxColsumSlabs = 128;
-template <bool GELU>
-__global__ void __launch_bounds__(256) linear_prep_kernel(const __nv_bfloat16* __restrict__ x, const __half* __restrict__ pre, __nv_bfloat16* __restrict__ dz,
+template <bool SLOPE>
+__global__ void __launch_bounds__(256) linear_prep_kernel(const __nv_bfloat16* __restrict__ x, const __half* __restrict__ slope, __nv_bfloat16* __restrict__ dz,
                                                           float* __restrict__ part, int M, int N, int rows_per_block, int atomic, float4* __restrict__ zero,
                                                           long zero4) {
     pdl_wait();
     pdl_trigger();
     const long zstep = static_cast<long>(gridDim.x) * gridDim.y * blockDim.x;
     for (long i = (static_cast<long>(blockIdx.y) * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x; i < zero4; i += zstep) zero[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (!GELU && !part) return;
+    if (!SLOPE && !part) return;
     __shared__ float sums[8][kColsumCols + 4];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int col = blockIdx.x * kColsumCols + lane * 8;
@@ -549,18 +570,18 @@ __global__ void __launch_bounds__(256) linear_prep_kernel(const __nv_bfloat16* _
             acc[2 * e + 1] += __uint_as_float(w[e] & 0xffff0000u);
         }
     };
-    if (GELU && col < N) {
+    if (SLOPE && col < N) {
         const uint4* src = reinterpret_cast<const uint4*>(x + col);
-        const uint4* zsrc = reinterpret_cast<const uint4*>(pre + col);
+        const uint4* ssrc = reinterpret_cast<const uint4*>(slope + col);
         uint4* dst = reinterpret_cast<uint4*>(dz + col);
         const long pitch = N / 8;
-        auto slopes = [&](long at, const uint4& g4, const uint4& z4) {
-            const uint32_t g[4] = {g4.x, g4.y, g4.z, g4.w}, z[4] = {z4.x, z4.y, z4.z, z4.w};
+        auto product = [&](long at, const uint4& g4, const uint4& s4) {
+            const uint32_t g[4] = {g4.x, g4.y, g4.z, g4.w}, f[4] = {s4.x, s4.y, s4.z, s4.w};
             uint32_t o[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 float a, b;
-                unpack_f32x2(fmul2(unpack_bf16x2(g[e]), gelu_slope2(unpack_half2(z[e]))), a, b);
+                unpack_f32x2(fmul2(unpack_bf16x2(g[e]), unpack_half2(f[e])), a, b);
                 acc[2 * e] += a;
                 acc[2 * e + 1] += b;
                 o[e] = pack_bf16x2(a, b);
@@ -568,16 +589,20 @@ __global__ void __launch_bounds__(256) linear_prep_kernel(const __nv_bfloat16* _
             dst[at] = make_uint4(o[0], o[1], o[2], o[3]);
         };
         int row = blockIdx.y * rows_per_block + warp;
-        for (; row + 8 < row1; row += 16) {
-            const long at = row * pitch, at1 = at + 8 * pitch;
-            const uint4 g0 = src[at], z0 = zsrc[at], g1 = src[at1], z1 = zsrc[at1];
-            slopes(at, g0, z0);
-            slopes(at1, g1, z1);
+        for (; row + 24 < row1; row += 32) {
+            uint4 g[4], f[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                g[u] = src[(row + 8 * u) * pitch];
+                f[u] = ssrc[(row + 8 * u) * pitch];
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) product((row + 8 * u) * pitch, g[u], f[u]);
         }
-        for (; row < row1; row += 8) slopes(row * pitch, src[row * pitch], zsrc[row * pitch]);
+        for (; row < row1; row += 8) product(row * pitch, src[row * pitch], ssrc[row * pitch]);
     }
     if (!part) return;
-    if (!GELU && col < N) {
+    if (!SLOPE && col < N) {
         const uint4* src = reinterpret_cast<const uint4*>(x + col);
         const long pitch = N / 8;
         int row = blockIdx.y * rows_per_block + warp;
@@ -654,13 +679,14 @@ __global__ void __launch_bounds__(256) linear_finish_kernel(const __grid_constan
     }
 }
 
-// Behind a forward product that was cut along K: the epilogue on its fp32 sums, 8 elements per thread.
+// Behind a forward product that was cut along K: its parts' sum, and the epilogue on it, 8 elements per thread.
 struct FusedFinish {
-    const float4* acc;
+    const float4* acc;          // [slabs][M][N]
+    int slabs;
     const void* bias;
     int bias_bf16, gelu;
     const uint4* residual;      // or null
-    uint4* pre;                 // fp16, or null
+    uint4* slope;               // gelu'(z), fp16, or null
     uint4* y;
     long n8;
     int N;
@@ -670,8 +696,15 @@ __global__ void __launch_bounds__(256) linear_fused_finish_kernel(const FusedFin
     pdl_trigger();
     const long step = static_cast<long>(gridDim.x) * blockDim.x;
     for (long i = static_cast<long>(blockIdx.x) * blockDim.x + threadIdx.x; i < p.n8; i += step) {
-        const float4 a = p.acc[2 * i], b = p.acc[2 * i + 1];
-        uint64_t v[4] = {pack_f32x2(a.x, a.y), pack_f32x2(a.z, a.w), pack_f32x2(b.x, b.y), pack_f32x2(b.z, b.w)};
+        uint64_t v[4] = {0, 0, 0, 0};
+#pragma unroll 4
+        for (int j = 0; j < p.slabs; ++j) {
+            const float4 a = p.acc[2 * (i + j * p.n8)], b = p.acc[2 * (i + j * p.n8) + 1];
+            v[0] = fadd2(v[0], pack_f32x2(a.x, a.y));
+            v[1] = fadd2(v[1], pack_f32x2(a.z, a.w));
+            v[2] = fadd2(v[2], pack_f32x2(b.x, b.y));
+            v[3] = fadd2(v[3], pack_f32x2(b.z, b.w));
+        }
         const int col = static_cast<int>(i * 8 % p.N);
         uint32_t o[4];
         const uint4 r4 = p.residual ? p.residual[i] : make_uint4(0, 0, 0, 0);
@@ -681,12 +714,11 @@ __global__ void __launch_bounds__(256) linear_fused_finish_kernel(const FusedFin
             if (p.bias)
                 v[e] = fadd2(v[e], p.bias_bf16 ? unpack_bf16x2(reinterpret_cast<const uint32_t*>(static_cast<const __nv_bfloat16*>(p.bias) + col)[e])
                                                : reinterpret_cast<const uint64_t*>(static_cast<const float*>(p.bias) + col)[e]);
-            o[e] = pack_preact2(v[e]);
+            if (p.gelu) v[e] = gelu_with_slope2(v[e], o[e]);
         }
-        if (p.pre) p.pre[i] = make_uint4(o[0], o[1], o[2], o[3]);
+        if (p.slope) p.slope[i] = make_uint4(o[0], o[1], o[2], o[3]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            if (p.gelu) v[e] = gelu2(v[e]);
             if (p.residual) v[e] = fadd2(v[e], unpack_bf16x2(r[e]));
             o[e] = pack_bf16_pair(v[e]);
         }

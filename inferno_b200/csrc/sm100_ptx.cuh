@@ -625,6 +625,12 @@ __device__ __forceinline__ float fast_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// x limited to [-limit, limit], in one instruction: the smaller magnitude, with the sign of x (limit > 0).  NaN becomes limit.
+__device__ __forceinline__ float clamp_abs(float x, float limit) {
+    float y;
+    asm("min.xorsign.abs.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(limit));
+    return y;
+}
 __device__ __forceinline__ float fast_rcp(float x) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

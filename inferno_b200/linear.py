@@ -37,19 +37,19 @@ class LinearFunction:
         return _capi.host().linear(x, w, bias)
 
 
-def fused_linear_forward(x, w, bias=None, activation: str | None = None, residual=None, keep_preact: bool = False):
-    """(y, preact) with y = act(x @ w + bias) + residual; activation is None or "gelu" (the tanh form), residual has y's shape.
+def fused_linear_forward(x, w, bias=None, activation: str | None = None, residual=None, keep_slope: bool = False):
+    """(y, slope) with y = act(x @ w + bias) + residual; activation is None or "gelu" (the tanh form), residual has y's shape.
 
-    preact is what the backward needs of the pre-activation: fp16, limited to +-16, beyond which the derivative is 0 or 1.
-    None without an activation, or when it is not kept."""
-    return _capi.host().fused_linear_forward(x, w, bias, activation, residual, keep_preact)
+    slope is what the backward needs: the activation's derivative at x @ w + bias, in fp16.  None without an activation, or
+    when it is not kept."""
+    return _capi.host().fused_linear_forward(x, w, bias, activation, residual, keep_slope)
 
 
-def fused_linear_backward(x, w, dy, preact=None, activation: str | None = None, need_dx=True, need_dw=True, need_db=True):
+def fused_linear_backward(x, w, dy, slope=None, activation: str | None = None, need_dx=True, need_dw=True, need_db=True):
     """(dx, dw, db) of ``fused_linear_forward``; db is fp32; what is not needed comes back as None.  The residual's gradient is dy.
 
     dw is added up as in ``linear_backward``; dx and db repeat bit for bit."""
-    return _capi.host().fused_linear_backward(x, w, dy, preact, activation, need_dx, need_dw, need_db)
+    return _capi.host().fused_linear_backward(x, w, dy, slope, activation, need_dx, need_dw, need_db)
 
 
 def fused_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,

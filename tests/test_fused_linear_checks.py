@@ -85,7 +85,7 @@ def test_c_abi_validation(built_lib):
     x, w, b, r, y, p, ws = (0x100000 * i for i in range(1, 8))
     fwd = lambda x=x, w=w, b=b, bd=B, r=r, act=1, y=y, p=p, M=16, K=32, N=64, ws=ws, n=1 << 20: C.ib200_fused_linear_fwd(x, w, b, bd, r, act, y, p, M, K, N, ws, n, None)
     assert fwd(x=None) == bad and fwd(w=None) == bad and fwd(y=None) == bad and fwd(bd=2) == bad and fwd(act=2) == bad and fwd(act=-1) == bad
-    assert fwd(act=0) == bad and fwd(M=0) == bad and fwd(K=-8) == bad and fwd(N=0) == bad            # a preact without an activation
+    assert fwd(act=0) == bad and fwd(M=0) == bad and fwd(K=-8) == bad and fwd(N=0) == bad            # a slope without an activation
     assert fwd(K=36) == _capi.ERR_UNSUPPORTED and fwd(N=60) == _capi.ERR_UNSUPPORTED
     for k in ("x", "w", "y", "r", "p", "b"):
         assert fwd(**{k: 0x900008}) == _capi.ERR_MISALIGNED
