@@ -617,9 +617,10 @@ int gemm_single(const GemmDesc& d, const void* bias, int bias_bf16, void* ws, si
 
 bool valid_dtype(int dtype) { return dtype == IB200_DTYPE_F32 || dtype == IB200_DTYPE_BF16; }
 
-// Up to 16 rows.  Blocks of a cluster split K until two blocks per SM are there, as long as every warp keeps two steps of 16 rows.
+// Up to 16 rows.  Blocks of a cluster split K until every SM has a block, as long as every warp keeps a box of 64 rows.
 template <int SPLIT>
-int launch_few(const FewRows& p, int strips, cudaStream_t stream) {
+int launch_few(const CUtensorMap& wmap, const FewRows& p, int strips, cudaStream_t stream) {
+    if (!allow_smem<linear_few_kernel<SPLIT>>(kFewSmem)) return IB200_ERR_CUDA;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -629,21 +630,27 @@ int launch_few(const FewRows& p, int strips, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(strips * SPLIT);
     cfg.blockDim = dim3(kFewWarps * 32);
+    cfg.dynamicSmemBytes = kFewSmem;
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = SPLIT > 1 ? 2 : 1;
-    return cuda_ok(cudaLaunchKernelEx(&cfg, linear_few_kernel<SPLIT>, p)) ? IB200_OK : IB200_ERR_CUDA;
+    return cuda_ok(cudaLaunchKernelEx(&cfg, linear_few_kernel<SPLIT>, wmap, p)) ? IB200_OK : IB200_ERR_CUDA;
 }
-int linear_few(FewRows p, int sms, cudaStream_t stream) {
-    const int strips = (p.N + kFewCols - 1) / kFewCols, steps = (p.K + 15) / 16;
+int linear_few(const void* w, FewRows p, int sms, cudaStream_t stream) {
+    CUtensorMap wmap;
+    if (!make_tmap_2d(&wmap, w, p.K, p.N, kFewStep)) return IB200_ERR_CUDA;
+    void* builtin = nullptr;
+    p.status = static_scratch(&builtin) == IB200_OK ? static_cast<int*>(builtin) : nullptr;
+    IB200_SET_BOUNDS(0, 0, 0, 0, 0, 1, 0, p.status, stream);
+    const int strips = (p.N + kFewCols - 1) / kFewCols, steps = (p.K + kFewStep - 1) / kFewStep;
     int split = 1;
-    while (split < 8 && strips * split * 2 <= 2 * sms && steps >= split * 2 * 2 * kFewWarps) split *= 2;
+    while (split < 8 && strips * split * 2 <= sms && steps >= split * 2 * kFewWarps) split *= 2;
     p.steps = (steps + split - 1) / split;
     switch (split) {
-        case 1: return launch_few<1>(p, strips, stream);
-        case 2: return launch_few<2>(p, strips, stream);
-        case 4: return launch_few<4>(p, strips, stream);
-        default: return launch_few<8>(p, strips, stream);
+        case 1: return launch_few<1>(wmap, p, strips, stream);
+        case 2: return launch_few<2>(wmap, p, strips, stream);
+        case 4: return launch_few<4>(wmap, p, strips, stream);
+        default: return launch_few<8>(wmap, p, strips, stream);
     }
 }
 
@@ -656,8 +663,8 @@ int fused_linear_fwd_core(const GemmDesc& d, const void* bias, int bias_bf16, co
     const DeviceInfo* dev = device_info();
     if (!dev) return IB200_ERR_CUDA;
     if (d.M <= kFewMaxRows)
-        return linear_few(FewRows{static_cast<const __nv_bfloat16*>(d.a), static_cast<const __nv_bfloat16*>(d.b), bias, bias_bf16, gelu,
-                                  static_cast<const __nv_bfloat16*>(residual), static_cast<__half*>(slope), static_cast<__nv_bfloat16*>(d.c), d.M, d.N, d.K, 0},
+        return linear_few(d.b, FewRows{static_cast<const __nv_bfloat16*>(d.a), bias, bias_bf16, gelu, static_cast<const __nv_bfloat16*>(residual),
+                                       static_cast<__half*>(slope), static_cast<__nv_bfloat16*>(d.c), d.M, d.N, d.K, 0, nullptr},
                           dev->sms, stream);
     const size_t n = static_cast<size_t>(d.M) * d.N;
     const int slabs = gemm_slabs(d, dev->sms / 2);
@@ -684,15 +691,17 @@ size_t linear_bwd_ws_bytes(int K, int N) { return round_up(static_cast<size_t>(K
 
 // The helper ahead of a backward's products: column sums of dy (`part`), zeroing of the accumulators, and with `slope` dz = dy slope.
 int launch_linear_prep(const void* dy, const void* slope, void* dz, float* part, int M, int N, bool atomic, float* zero, size_t zero_floats, cudaStream_t stream) {
-    const int slabs = colsum_slabs(M, N), rows = (M + slabs - 1) / slabs;
-    const dim3 grid((N + kColsumCols - 1) / kColsumCols, part || slope ? slabs : 64);
-    float4* z4 = reinterpret_cast<float4*>(zero);
+    const int slabs = part || slope ? colsum_slabs(M, N) : 0, rows = slabs ? (M + slabs - 1) / slabs : 0, gx = (N + kColsumCols - 1) / kColsumCols;
     const long n4 = static_cast<long>(zero_floats / 4);
+    const int zero_blocks = static_cast<int>(std::min<long>((n4 + 2047) / 2048, 4 * 148));
+    const dim3 grid(gx, slabs + (zero_blocks + gx - 1) / gx);
+    if (grid.y == 0) return IB200_OK;
+    float4* z4 = reinterpret_cast<float4*>(zero);
     const auto* g = static_cast<const __nv_bfloat16*>(dy);
     return slope ? launch_pdl<linear_prep_kernel<true>>(grid, 256, 0, stream, g, static_cast<const __half*>(slope), static_cast<__nv_bfloat16*>(dz), part, M, N, rows,
-                                                      static_cast<int>(atomic), z4, n4)
-               : launch_pdl<linear_prep_kernel<false>>(grid, 256, 0, stream, g, static_cast<const __half*>(nullptr), static_cast<__nv_bfloat16*>(nullptr), part, M, N,
-                                                       rows, static_cast<int>(atomic), z4, n4);
+                                                        slabs, static_cast<int>(atomic), z4, n4)
+                 : launch_pdl<linear_prep_kernel<false>>(grid, 256, 0, stream, g, static_cast<const __half*>(nullptr), static_cast<__nv_bfloat16*>(nullptr), part, M, N,
+                                                         rows, slabs, static_cast<int>(atomic), z4, n4);
 }
 
 // With `slope` (and a workspace) dy is first multiplied by it, into `dz`.

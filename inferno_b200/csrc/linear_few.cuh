@@ -1,14 +1,17 @@
 // y = act(x w + bias) + residual for up to 16 rows of x: one token, or a few that are decoded together.
 //
-// Nothing but the bytes of w counts here (2048 x 8192: 34 MB, 5.1 us at the measured copy rate), so the kernel is built to stream w [K, N] once, in the
-// order in which it lies, with many loads on their way, and without shared memory between a load and its product.  A warp takes 16 rows of
-// w by 64 columns at a time: lane t loads 16 bytes of rows 2q, 2q + 1, 2q + 8, 2q + 9 (q = t % 4) at columns 8 (t / 4), which are exactly the
-// (k, n) that it has to hold for eight m16n8k16 products, if product e is given the columns 8 n + e: the order of the columns among the
-// products is free, and two rows are woven into pairs by a byte permutation.  The rows of x, padded to 16, are the other operand; at this
-// size the warp-level MMA costs nothing and needs neither descriptors nor tensor memory.
-// The eight warps of a block share 64 columns and take the rows of w in turn; blocks of a cluster split the rows further, until the chip is full.
-// The sums meet in shared memory, of the cluster's blocks through distributed shared memory, in a fixed order, and whoever adds them up does
-// the epilogue.
+// Nothing but the bytes of w counts here (2048 x 8192: 34 MB, 5.1 us at the measured copy rate), so the kernel is built to stream w [K, N] once with as
+// many bytes on their way as an SM can hold.  (A plain loop of 16-byte loads reads that matrix in 14.4, 10.3 and 8.2 us with 64, 128 and
+// 256 KB on their way per SM, whatever the width of a block's strip.)  Each warp has a ring of three boxes of 64 rows by 64 columns, 8 KB each,
+// which one of its lanes has the TMA unit fill: 192 KB per SM, and no register, barrier or other thread stands between a box and its use.
+// (Sixteen loads a thread in registers, 128 KB per SM: 10.9 us; the same by 16-byte asynchronous copies into slots per thread: 14.)
+// A lane (q = t % 4, g = t / 4) reads 16 bytes of rows 2q, 2q + 1, 2q + 8, 2q + 9 at columns 8g, no bank twice, and these are exactly the (k, n) that it
+// has to hold for eight m16n8k16 products, if product e is given the columns 8 n + e: the order of the columns among the products is free,
+// and two rows are woven into pairs by a byte permutation.  The rows of x, padded to 16, are the other operand; at this size the
+// warp-level MMA costs nothing and needs neither descriptors nor tensor memory.
+// The eight warps of a block share 64 columns and take the boxes in turn; blocks of a cluster split the rows further, until every SM has
+// a block.  The sums meet in shared memory, of the cluster's blocks through distributed shared memory, in a fixed order, and whoever adds
+// them up does the epilogue.
 #pragma once
 
 #include "linear_gemm.cuh"
@@ -17,22 +20,19 @@ namespace ib200 {
 
 struct FewRows {
     const __nv_bfloat16* x;        // [M, K], M <= 16
-    const __nv_bfloat16* w;        // [K, N]
     const void* bias;              // [N], or null
     int bias_bf16, gelu;
     const __nv_bfloat16* residual; // [M, N], or null
     __half* slope;                 // gelu', or null
     __nv_bfloat16* y;
     int M, N, K;
-    int steps;                     // of 16 rows of w, per block
+    int steps;                     // of 64 rows of w, per block
+    int* status;
 };
-constexpr int kFewMaxRows = 16, kFewCols = 64, kFewWarps = 8, kFewBatch = 4;
+constexpr int kFewMaxRows = 16, kFewCols = 64, kFewStep = 64, kFewWarps = 8, kFewDepth = 3, kFewBox = kFewStep * kFewCols * 2;
+constexpr int kFewSmem = kFewWarps * kFewDepth * kFewBox + 1024;
+static_assert(kFewWarps * kFewMaxRows * (kFewCols + 4) * 4 <= kFewWarps * kFewDepth * kFewBox, "the warps' sums take the ring's place");
 
-__device__ __forceinline__ uint4 ld_stream(const void* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
 __device__ __forceinline__ void mma_16x8x16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -46,51 +46,51 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t cluster_addr) {
 
 // Grid: strips of 64 columns times the cluster's blocks (SPLIT, along K).
 template <int SPLIT>
-__global__ void __launch_bounds__(kFewWarps * 32, 2) linear_few_kernel(const FewRows p) {
-    __shared__ float part[kFewWarps][kFewMaxRows][kFewCols + 4];
+__global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __grid_constant__ CUtensorMap wmap, const FewRows p) {
+    extern __shared__ uint8_t few_smem[];
     __shared__ float total[kFewMaxRows][kFewCols];
+    __shared__ uint64_t bars[kFewWarps][kFewDepth];
+    __shared__ int abort_flag;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, q = lane & 3, g = lane >> 2;
+    const int strip = blockIdx.x / SPLIT, rank = blockIdx.x % SPLIT;
+    const int first = rank * p.steps + warp, last = min((p.K + kFewStep - 1) / kFewStep, (rank + 1) * p.steps);
+    uint8_t* boxes = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(few_smem) + 1023) & ~static_cast<uintptr_t>(1023));
+    uint8_t* mybox = boxes + warp * kFewDepth * kFewBox;
+    const ResidentAbortCtx ab{&abort_flag, p.status};
+    if (tid == 0) abort_flag = 0;
+    if (lane == 0) {
+        for (int u = 0; u < kFewDepth; ++u) mbar_init(&bars[warp][u], 1);
+        fence_mbar_init();
+        tma_prefetch_desc(&wmap);
+    }
+    __syncthreads();
     pdl_wait();
     pdl_trigger();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = lane & 3, g = lane >> 2;
-    const int strip = blockIdx.x / SPLIT, rank = blockIdx.x % SPLIT;
-    const int col = strip * kFewCols + 8 * g;
-    const int last = min((p.K + 15) / 16, (rank + 1) * p.steps);
-    float acc[8][4];
+
+    auto request = [&](int slot, int s) {          // lane 0
+        mbar_arrive_expect_tx(&bars[warp][slot], kFewBox);
+        tma_load_3d(mybox + slot * kFewBox, &wmap, &bars[warp][slot], strip * kFewCols, s * kFewStep, 0);
+    };
+    if (lane == 0) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[e][i] = 0.f;
-    for (int s0 = rank * p.steps + warp; s0 < last; s0 += kFewBatch * kFewWarps) {
-        uint4 w[kFewBatch][4];
-        uint32_t a[kFewBatch][4];
-#pragma unroll
-        for (int u = 0; u < kFewBatch; ++u) {
-            const int s = s0 + u * kFewWarps;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int k = 16 * s + 2 * q + (i & 1) + 8 * (i >> 1);
-                w[u][i] = s < last && k < p.K && col < p.N ? ld_stream(p.w + static_cast<long>(k) * p.N + col) : make_uint4(0, 0, 0, 0);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int xr = g + 8 * (i & 1), k = 16 * s + 2 * q + 8 * (i >> 1);
-                a[u][i] = s < last && k < p.K && xr < p.M ? *reinterpret_cast<const uint32_t*>(p.x + static_cast<long>(xr) * p.K + k) : 0u;
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < kFewBatch; ++u) {
-            const uint32_t lo[4] = {w[u][0].x, w[u][0].y, w[u][0].z, w[u][0].w}, lo1[4] = {w[u][1].x, w[u][1].y, w[u][1].z, w[u][1].w};
-            const uint32_t hi[4] = {w[u][2].x, w[u][2].y, w[u][2].z, w[u][2].w}, hi1[4] = {w[u][3].x, w[u][3].y, w[u][3].z, w[u][3].w};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t pick = e & 1 ? 0x7632u : 0x5410u;      // the odd or the even column of a pair, of two rows
-                mma_16x8x16(acc[e], a[u], __byte_perm(lo[e / 2], lo1[e / 2], pick), __byte_perm(hi[e / 2], hi1[e / 2], pick));
-            }
-        }
+        for (int u = 0; u < kFewDepth; ++u)
+            if (first + u * kFewWarps < last) request(u, first + u * kFewWarps);
     }
-    // what the epilogue will need, asked for ahead of the barriers
-    const int row = threadIdx.x / (kFewCols / 4), c4 = threadIdx.x % (kFewCols / 4) * 4, c = strip * kFewCols + c4;
-    const bool mine = row < p.M && c < p.N && static_cast<int>(threadIdx.x % SPLIT) == rank;      // the blocks share the adding up
+    // x of a step: of each 16 of its rows, columns 2q, 2q + 1 and 2q + 8, 2q + 9 of rows g and g + 8
+    auto load_x = [&](int s, uint32_t (&a)[4][4]) {
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = g + 8 * (i & 1), k = kFewStep * s + 16 * kk + 2 * q + 8 * (i >> 1);
+                a[kk][i] = s < last && k < p.K && row < p.M ? *reinterpret_cast<const uint32_t*>(p.x + static_cast<long>(row) * p.K + k) : 0u;
+            }
+    };
+    uint32_t a[4][4];
+    load_x(first, a);
+    // what the epilogue will need
+    const int row = tid / (kFewCols / 4), c4 = tid % (kFewCols / 4) * 4, c = strip * kFewCols + c4;
+    const bool mine = row < p.M && c < p.N && tid % SPLIT == rank;      // the blocks share the adding up
     const long at = static_cast<long>(row) * p.N + c;
     uint4 bias = make_uint4(0, 0, 0, 0);
     uint2 res = make_uint2(0, 0);
@@ -104,6 +104,44 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) linear_few_kernel(const Few
         }
         if (p.residual) res = *reinterpret_cast<const uint2*>(p.residual + at);
     }
+    float acc[8][4];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[e][i] = 0.f;
+    uint32_t slot = 0, phase = 0;
+    for (int s = first; s < last; s += kFewWarps) {
+        uint32_t next[4][4];
+        load_x(s + kFewWarps, next);
+        mbar_wait(&bars[warp][slot], phase, ab, 40);
+        const uint8_t* box = mybox + slot * kFewBox;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+            uint32_t w[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint4 v = *reinterpret_cast<const uint4*>(box + sw128_offset(16 * kk + 2 * q + (i & 1) + 8 * (i >> 1), g));
+                w[i][0] = v.x; w[i][1] = v.y; w[i][2] = v.z; w[i][3] = v.w;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t pick = e & 1 ? 0x7632u : 0x5410u;      // the odd or the even column of a pair, of two rows
+                mma_16x8x16(acc[e], a[kk], __byte_perm(w[0][e / 2], w[1][e / 2], pick), __byte_perm(w[2][e / 2], w[3][e / 2], pick));
+            }
+        }
+        __syncwarp();                              // every lane has read the box
+        if (lane == 0 && s + kFewDepth * kFewWarps < last) request(slot, s + kFewDepth * kFewWarps);
+        if (++slot == kFewDepth) { slot = 0; phase ^= 1; }
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[kk][i] = next[kk][i];
+    }
+    __syncthreads();                               // the ring's place is free for the warps' sums
+    if (*static_cast<volatile int*>(&abort_flag) != 0) {
+        for (int i = 0; i < 64; ++i) __nanosleep(1000);      // copies that are still on their way land before the block's memory is given back
+    }
+    float(*part)[kFewMaxRows][kFewCols + 4] = reinterpret_cast<float(*)[kFewMaxRows][kFewCols + 4]>(boxes);
     // product e of column index n is column 8 n + e: a thread has columns 16 q .. 16 q + 15 of rows g and g + 8
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

@@ -550,13 +550,15 @@ gemm_bf16_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ 
 constexpr int kColsumCols = 256, kMaxColsumSlabs = 128;
 template <bool SLOPE>
 __global__ void __launch_bounds__(256) linear_prep_kernel(const __nv_bfloat16* __restrict__ x, const __half* __restrict__ slope, __nv_bfloat16* __restrict__ dz,
-                                                          float* __restrict__ part, int M, int N, int rows_per_block, int atomic, float4* __restrict__ zero,
-                                                          long zero4) {
+                                                          float* __restrict__ part, int M, int N, int rows_per_block, int slabs, int atomic,
+                                                          float4* __restrict__ zero, long zero4) {
     pdl_wait();
     pdl_trigger();
-    const long zstep = static_cast<long>(gridDim.x) * gridDim.y * blockDim.x;
-    for (long i = (static_cast<long>(blockIdx.y) * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x; i < zero4; i += zstep) zero[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (!SLOPE && !part) return;
+    if (static_cast<int>(blockIdx.y) >= slabs) {      // blocks past the row slabs zero: a block that did both read nothing until its stores had drained
+        const long step = static_cast<long>(gridDim.x) * (gridDim.y - slabs) * blockDim.x;
+        for (long i = (static_cast<long>(blockIdx.y - slabs) * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x; i < zero4; i += step) zero[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        return;
+    }
     __shared__ float sums[8][kColsumCols + 4];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int col = blockIdx.x * kColsumCols + lane * 8;
