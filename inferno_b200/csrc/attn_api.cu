@@ -617,10 +617,13 @@ int gemm_single(const GemmDesc& d, const void* bias, int bias_bf16, void* ws, si
 
 bool valid_dtype(int dtype) { return dtype == IB200_DTYPE_F32 || dtype == IB200_DTYPE_BF16; }
 
-// Up to 16 rows.  Blocks of a cluster split K until every SM has a block, as long as every warp keeps a box of 64 rows.
-template <int SPLIT>
+// Up to 32 rows.  Up to four blocks of a cluster split K until every SM has a block, as long as every warp keeps two boxes of 64 rows.  us for split 1,
+// 2, 4, 8 where it has the choice: 1 x 8192 x 2048 14.1, 10.7, 9.9, 9.9; 1 x 4096 x 1024 8.2, 6.6, 5.4, 7.5 (one box a warp); 32 x 4096 x 1024
+// 15.1, 11.3, 8.9, 13.6; 1 x 1024 x 4096 4.2, 4.6 (one box).  More rows are the GEMM's: 32 and 33 of them, 2048 x 8192 13.2 and 15.7, 1024 x 4096
+// 7.0 and 12.3, 4096 x 4096 14.4 and 15.6.
+template <int SPLIT, int ROWS>
 int launch_few(const CUtensorMap& wmap, const FewRows& p, int strips, cudaStream_t stream) {
-    if (!allow_smem<linear_few_kernel<SPLIT>>(kFewSmem)) return IB200_ERR_CUDA;
+    if (!allow_smem<linear_few_kernel<SPLIT, ROWS>>(kFewSmem)) return IB200_ERR_CUDA;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -634,7 +637,7 @@ int launch_few(const CUtensorMap& wmap, const FewRows& p, int strips, cudaStream
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = SPLIT > 1 ? 2 : 1;
-    return cuda_ok(cudaLaunchKernelEx(&cfg, linear_few_kernel<SPLIT>, wmap, p)) ? IB200_OK : IB200_ERR_CUDA;
+    return cuda_ok(cudaLaunchKernelEx(&cfg, linear_few_kernel<SPLIT, ROWS>, wmap, p)) ? IB200_OK : IB200_ERR_CUDA;
 }
 int linear_few(const void* w, FewRows p, int sms, cudaStream_t stream) {
     CUtensorMap wmap;
@@ -644,13 +647,19 @@ int linear_few(const void* w, FewRows p, int sms, cudaStream_t stream) {
     IB200_SET_BOUNDS(0, 0, 0, 0, 0, 1, 0, p.status, stream);
     const int strips = (p.N + kFewCols - 1) / kFewCols, steps = (p.K + kFewStep - 1) / kFewStep;
     int split = 1;
-    while (split < 8 && strips * split * 2 <= sms && steps >= split * 2 * kFewWarps) split *= 2;
+    while (split < 4 && strips * split * 2 <= sms && steps >= split * 2 * 2 * kFewWarps) split *= 2;
     p.steps = (steps + split - 1) / split;
+    if (p.M <= 16) {
+        switch (split) {
+            case 1: return launch_few<1, 16>(wmap, p, strips, stream);
+            case 2: return launch_few<2, 16>(wmap, p, strips, stream);
+            default: return launch_few<4, 16>(wmap, p, strips, stream);
+        }
+    }
     switch (split) {
-        case 1: return launch_few<1>(wmap, p, strips, stream);
-        case 2: return launch_few<2>(wmap, p, strips, stream);
-        case 4: return launch_few<4>(wmap, p, strips, stream);
-        default: return launch_few<8>(wmap, p, strips, stream);
+        case 1: return launch_few<1, 32>(wmap, p, strips, stream);
+        case 2: return launch_few<2, 32>(wmap, p, strips, stream);
+        default: return launch_few<4, 32>(wmap, p, strips, stream);
     }
 }
 

@@ -1,4 +1,4 @@
-// y = act(x w + bias) + residual for up to 16 rows of x: one token, or a few that are decoded together.
+// y = act(x w + bias) + residual for up to 32 rows of x: one token, or a few that are decoded together.
 //
 // Nothing but the bytes of w counts here (2048 x 8192: 34 MB, 5.1 us at the measured copy rate), so the kernel is built to stream w [K, N] once with as
 // many bytes on their way as an SM can hold.  (A plain loop of 16-byte loads reads that matrix in 14.4, 10.3 and 8.2 us with 64, 128 and
@@ -7,7 +7,7 @@
 // (Sixteen loads a thread in registers, 128 KB per SM: 10.9 us; the same by 16-byte asynchronous copies into slots per thread: 14.)
 // A lane (q = t % 4, g = t / 4) reads 16 bytes of rows 2q, 2q + 1, 2q + 8, 2q + 9 at columns 8g, no bank twice, and these are exactly the (k, n) that it
 // has to hold for eight m16n8k16 products, if product e is given the columns 8 n + e: the order of the columns among the products is free,
-// and two rows are woven into pairs by a byte permutation.  The rows of x, padded to 16, are the other operand; at this size the
+// and two rows are woven into pairs by a byte permutation.  The rows of x, padded to 16 or 32, are the other operand; at this size the
 // warp-level MMA costs nothing and needs neither descriptors nor tensor memory.
 // The eight warps of a block share 64 columns and take the boxes in turn; blocks of a cluster split the rows further, until every SM has
 // a block.  The sums meet in shared memory, of the cluster's blocks through distributed shared memory, in a fixed order, and whoever adds
@@ -19,7 +19,7 @@
 namespace ib200 {
 
 struct FewRows {
-    const __nv_bfloat16* x;        // [M, K], M <= 16
+    const __nv_bfloat16* x;        // [M, K], M <= 32
     const void* bias;              // [N], or null
     int bias_bf16, gelu;
     const __nv_bfloat16* residual; // [M, N], or null
@@ -29,11 +29,11 @@ struct FewRows {
     int steps;                     // of 64 rows of w, per block
     int* status;
 };
-constexpr int kFewMaxRows = 16, kFewCols = 64, kFewStep = 64, kFewWarps = 8, kFewDepth = 3, kFewBox = kFewStep * kFewCols * 2;
+constexpr int kFewMaxRows = 32, kFewCols = 64, kFewStep = 64, kFewWarps = 8, kFewDepth = 3, kFewBox = kFewStep * kFewCols * 2;
 constexpr int kFewSmem = kFewWarps * kFewDepth * kFewBox + 1024;
 static_assert(kFewWarps * kFewMaxRows * (kFewCols + 4) * 4 <= kFewWarps * kFewDepth * kFewBox, "the warps' sums take the ring's place");
 
-__device__ __forceinline__ void mma_16x8x16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_16x8x16(float (&c)[4], const uint32_t* a, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -44,11 +44,12 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t cluster_addr) {
     return v;
 }
 
-// Grid: strips of 64 columns times the cluster's blocks (SPLIT, along K).
-template <int SPLIT>
+// Grid: strips of 64 columns times the cluster's blocks (SPLIT, along K).  ROWS: 16 or 32.
+template <int SPLIT, int ROWS>
 __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __grid_constant__ CUtensorMap wmap, const FewRows p) {
     extern __shared__ uint8_t few_smem[];
-    __shared__ float total[kFewMaxRows][kFewCols];
+    constexpr int MT = ROWS / 16;
+    __shared__ float total[ROWS][kFewCols];
     __shared__ uint64_t bars[kFewWarps][kFewDepth];
     __shared__ int abort_flag;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, q = lane & 3, g = lane >> 2;
@@ -76,25 +77,24 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
         for (int u = 0; u < kFewDepth; ++u)
             if (first + u * kFewWarps < last) request(u, first + u * kFewWarps);
     }
-    // x of a step: of each 16 of its rows, columns 2q, 2q + 1 and 2q + 8, 2q + 9 of rows g and g + 8
-    auto load_x = [&](int s, uint32_t (&a)[4][4]) {
+    // x of a step: of each 16 of its columns, 2q, 2q + 1 and 2q + 8, 2q + 9 of rows g and g + 8 (and 16 more)
+    auto load_x = [&](int s, uint32_t (&a)[4][4 * MT]) {
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = g + 8 * (i & 1), k = kFewStep * s + 16 * kk + 2 * q + 8 * (i >> 1);
+            for (int i = 0; i < 4 * MT; ++i) {
+                const int row = g + 8 * (i & 1) + 16 * (i >> 2), k = kFewStep * s + 16 * kk + 2 * q + 8 * (i >> 1 & 1);
                 a[kk][i] = s < last && k < p.K && row < p.M ? *reinterpret_cast<const uint32_t*>(p.x + static_cast<long>(row) * p.K + k) : 0u;
             }
     };
-    uint32_t a[4][4];
+    uint32_t a[4][4 * MT];
     load_x(first, a);
-    // what the epilogue will need
-    const int row = tid / (kFewCols / 4), c4 = tid % (kFewCols / 4) * 4, c = strip * kFewCols + c4;
-    const bool mine = row < p.M && c < p.N && tid % SPLIT == rank;      // the blocks share the adding up
-    const long at = static_cast<long>(row) * p.N + c;
+    // what the epilogue will need: the thread adds up four columns of one row in each 16
+    const int c4 = tid % (kFewCols / 4) * 4, c = strip * kFewCols + c4;
+    const bool my_share = c < p.N && tid % SPLIT == rank;               // the blocks share the adding up
     uint4 bias = make_uint4(0, 0, 0, 0);
-    uint2 res = make_uint2(0, 0);
-    if (mine) {
+    uint2 res[MT];
+    if (my_share) {
         if (p.bias && p.bias_bf16) {
             const uint2 b = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p.bias) + c);
             bias.x = b.x;
@@ -102,16 +102,22 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
         } else if (p.bias) {
             bias = *reinterpret_cast<const uint4*>(static_cast<const float*>(p.bias) + c);
         }
-        if (p.residual) res = *reinterpret_cast<const uint2*>(p.residual + at);
     }
-    float acc[8][4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
+    for (int m = 0; m < MT; ++m) {
+        const int row = 16 * m + tid / (kFewCols / 4);
+        res[m] = my_share && p.residual && row < p.M ? *reinterpret_cast<const uint2*>(p.residual + static_cast<long>(row) * p.N + c) : make_uint2(0, 0);
+    }
+    float acc[MT][8][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[e][i] = 0.f;
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[m][e][i] = 0.f;
     uint32_t slot = 0, phase = 0;
     for (int s = first; s < last; s += kFewWarps) {
-        uint32_t next[4][4];
+        uint32_t next[4][4 * MT];
         load_x(s + kFewWarps, next);
         mbar_wait(&bars[warp][slot], phase, ab, 40);
         const uint8_t* box = mybox + slot * kFewBox;
@@ -126,7 +132,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const uint32_t pick = e & 1 ? 0x7632u : 0x5410u;      // the odd or the even column of a pair, of two rows
-                mma_16x8x16(acc[e], a[kk], __byte_perm(w[0][e / 2], w[1][e / 2], pick), __byte_perm(w[2][e / 2], w[3][e / 2], pick));
+                const uint32_t b0 = __byte_perm(w[0][e / 2], w[1][e / 2], pick), b1 = __byte_perm(w[2][e / 2], w[3][e / 2], pick);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) mma_16x8x16(acc[m][e], &a[kk][4 * m], b0, b1);
             }
         }
         __syncwarp();                              // every lane has read the box
@@ -135,51 +143,60 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) linear_few_kernel(const __g
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) a[kk][i] = next[kk][i];
+            for (int i = 0; i < 4 * MT; ++i) a[kk][i] = next[kk][i];
     }
     __syncthreads();                               // the ring's place is free for the warps' sums
     if (*static_cast<volatile int*>(&abort_flag) != 0) {
         for (int i = 0; i < 64; ++i) __nanosleep(1000);      // copies that are still on their way land before the block's memory is given back
     }
-    float(*part)[kFewMaxRows][kFewCols + 4] = reinterpret_cast<float(*)[kFewMaxRows][kFewCols + 4]>(boxes);
+    float(*part)[ROWS][kFewCols + 4] = reinterpret_cast<float(*)[ROWS][kFewCols + 4]>(boxes);
     // product e of column index n is column 8 n + e: a thread has columns 16 q .. 16 q + 15 of rows g and g + 8
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float* dst = &part[warp][g + 8 * (i >> 1)][16 * q + 8 * (i & 1)];
-        *reinterpret_cast<float4*>(dst) = make_float4(acc[0][i], acc[1][i], acc[2][i], acc[3][i]);
-        *reinterpret_cast<float4*>(dst + 4) = make_float4(acc[4][i], acc[5][i], acc[6][i], acc[7][i]);
-    }
-    __syncthreads();
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](const float4& v) { sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w; };
-    if (row < p.M) {
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int w = 0; w < kFewWarps; ++w) add(*reinterpret_cast<const float4*>(&part[w][row][c4]));
+        for (int i = 0; i < 4; ++i) {
+            float* dst = &part[warp][16 * m + g + 8 * (i >> 1)][16 * q + 8 * (i & 1)];
+            *reinterpret_cast<float4*>(dst) = make_float4(acc[m][0][i], acc[m][1][i], acc[m][2][i], acc[m][3][i]);
+            *reinterpret_cast<float4*>(dst + 4) = make_float4(acc[m][4][i], acc[m][5][i], acc[m][6][i], acc[m][7][i]);
+        }
+    __syncthreads();
+    float4 sum[MT];
+    auto add = [](float4& s, const float4& v) { s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w; };
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int row = 16 * m + tid / (kFewCols / 4);
+        sum[m] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (row < p.M) {
+#pragma unroll
+            for (int w = 0; w < kFewWarps; ++w) add(sum[m], *reinterpret_cast<const float4*>(&part[w][row][c4]));
+        }
+        if (SPLIT > 1) *reinterpret_cast<float4*>(&total[row][c4]) = sum[m];
     }
-    if constexpr (SPLIT > 1) {
-        *reinterpret_cast<float4*>(&total[row][c4]) = sum;
-        cluster_sync_all();
-        if (mine) {
+    if constexpr (SPLIT > 1) cluster_sync_all();
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int row = 16 * m + tid / (kFewCols / 4);
+        if (!my_share || row >= p.M) continue;
+        if constexpr (SPLIT > 1) {
             const uint32_t src = smem_u32(&total[row][c4]);
             float4 v[SPLIT];
 #pragma unroll
             for (int r = 0; r < SPLIT; ++r) v[r] = ld_cluster_f4(mapa_u32(src, r));
-            sum = v[0];
+            sum[m] = v[0];
 #pragma unroll
-            for (int r = 1; r < SPLIT; ++r) add(v[r]);
+            for (int r = 1; r < SPLIT; ++r) add(sum[m], v[r]);
         }
-    }
-    if (mine) {
-        uint64_t v[2] = {pack_f32x2(sum.x, sum.y), pack_f32x2(sum.z, sum.w)};
+        uint64_t v[2] = {pack_f32x2(sum[m].x, sum[m].y), pack_f32x2(sum[m].z, sum[m].w)};
         if (p.bias) {
             v[0] = fadd2(v[0], p.bias_bf16 ? unpack_bf16x2(bias.x) : pack_f32x2(__uint_as_float(bias.x), __uint_as_float(bias.y)));
             v[1] = fadd2(v[1], p.bias_bf16 ? unpack_bf16x2(bias.y) : pack_f32x2(__uint_as_float(bias.z), __uint_as_float(bias.w)));
         }
+        const long at = static_cast<long>(row) * p.N + c;
         uint32_t slope[2], out[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             if (p.gelu) v[e] = gelu_with_slope2(v[e], slope[e]);
-            if (p.residual) v[e] = fadd2(v[e], unpack_bf16x2(e ? res.y : res.x));
+            if (p.residual) v[e] = fadd2(v[e], unpack_bf16x2(e ? res[m].y : res[m].x));
             out[e] = pack_bf16_pair(v[e]);
         }
         *reinterpret_cast<uint2*>(p.y + at) = make_uint2(out[0], out[1]);

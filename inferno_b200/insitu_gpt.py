@@ -5,7 +5,8 @@ embedding + sinusoidal positional encoding, pre-LayerNorm transformer blocks (ln
 ln2 -> Linear 4x -> tanh-GELU -> Linear -> +x), final LayerNorm, untied output head, cross-entropy loss,
 AdamW (lr 3e-4, betas (0.9, 0.95), weight decay 0.1: include/inferno/optim/adamw.h:15-22).  Everything
 around attention is PyTorch library code and is only the harness; the attention sub-path -- the part this
-repository replaces -- is `inferno_b200.attention.causal_attention`.  Attention is timed with CUDA events
+repository replaces -- is `inferno_b200.attention.causal_attention`.  With `--attn ib200_block` the rest of each block runs on
+this library as well: layer norms, the output projection with its residual, the feed-forward block with GELU and residual.  Attention is timed with CUDA events
 placed by the library's timing hook right around its main kernels, while the whole step runs.
 
     python -m inferno_b200.insitu_gpt [--layers 12 --d-model 768 --heads 12 --vocab 8192 --T 1024 --B 16 --steps 5]
@@ -22,6 +23,7 @@ import torch.nn.functional as F
 
 from . import attention as A
 from . import linear as L
+from . import norm as N
 
 
 def sinusoidal_pe(T: int, C: int, device) -> torch.Tensor:
@@ -37,6 +39,10 @@ class Block(nn.Module):
     def __init__(self, C: int, H: int, attn_impl: str):
         super().__init__()
         self.H, self.attn_impl = H, attn_impl
+        if attn_impl == "ib200_block":     # the whole block on this library
+            self.ln1, self.ln2 = N.LayerNorm(C), N.LayerNorm(C)
+            self.wqkv, self.wout, self.ff = L.Linear(C, 3 * C), L.Linear(C, C), L.FeedForward(C, 4 * C)
+            return
         self.ln1, self.ln2 = nn.LayerNorm(C), nn.LayerNorm(C)
         if attn_impl == "ib200_full":      # projections on this library's tcgen05 GEMM too (weights stored [in, out] like the reference)
             self.wqkv, self.wout = L.Linear(C, 3 * C), L.Linear(C, C)
@@ -60,6 +66,9 @@ class Block(nn.Module):
         return self.wout(y.transpose(1, 2).reshape(B, T, C))
 
     def forward(self, x):
+        if self.attn_impl == "ib200_block":
+            x = self.wout(A.causal_attention_packed(self.wqkv(self.ln1(x)), self.H), residual=x)
+            return self.ff(self.ln2(x), residual=x)
         x = x + self.attention(self.ln1(x))
         return x + self.ff2(F.gelu(self.ff1(self.ln2(x)), approximate="tanh"))
 
@@ -69,7 +78,7 @@ class GPT(nn.Module):
         super().__init__()
         self.emb = nn.Embedding(vocab, C)
         self.blocks = nn.ModuleList(Block(C, H, attn_impl) for _ in range(layers))
-        self.ln_f, self.head = nn.LayerNorm(C), nn.Linear(C, vocab)
+        self.ln_f, self.head = (N.LayerNorm if attn_impl == "ib200_block" else nn.LayerNorm)(C), nn.Linear(C, vocab)
         self.T = T
         for p in self.parameters():            # random-init weights N(0, 0.02)
             if p.dim() >= 2:
@@ -138,7 +147,7 @@ if __name__ == "__main__":
     ap.add_argument("--heads", type=int, default=12); ap.add_argument("--vocab", type=int, default=8192)
     ap.add_argument("--T", type=int, default=1024); ap.add_argument("--B", type=int, default=16)
     ap.add_argument("--steps", type=int, default=5)
-    ap.add_argument("--attn", default="ib200", choices=["ib200", "ib200_packed", "ib200_full"],
-                    help="ib200: dense [B,H,T,D] operands (the reference's layout copies stay); ib200_packed: operands read in place; ib200_full: packed attention plus this library's GEMM for Wqkv / W_out")
+    ap.add_argument("--attn", default="ib200", choices=["ib200", "ib200_packed", "ib200_full", "ib200_block"],
+                    help="ib200: dense [B,H,T,D] operands (the reference's layout copies stay); ib200_packed: operands read in place; ib200_full: packed attention plus this library's GEMM for Wqkv / W_out; ib200_block: layer norms and feed-forward too")
     a = ap.parse_args()
     print(json.dumps(run(a.layers, a.d_model, a.heads, a.vocab, a.T, a.B, a.steps, attn_impl=a.attn)))
