@@ -825,27 +825,27 @@ int launch_ln(bool backward, const LnRows& p, int blocks, cudaStream_t stream) {
     return backward ? launch_pdl<ln_bwd_kernel<S>>(blocks, kLnBwdThreads, S::BWD_SMEM, stream, p)
                     : launch_pdl<ln_fwd_kernel<S>>(std::min((p.M - 1) / S::FWD_ROWS + 1, S::FWD_BLOCKS * device_info()->sms), S::FWD_THREADS, S::FWD_SMEM, stream, p);
 }
-template <class T, class PT, int TPR, bool ALIGNED>
+template <class T, class PT, int TPR, int AU>
 int launch_ln_row(bool backward, const LnRows& p, int blocks, cudaStream_t stream) {
-    const int nv = (p.C - 1) / LnShape<T, PT, TPR, 1, true>::CHUNK_COLS + 1;
+    const int nv = (p.C - 1) / LnShape<T, PT, TPR, 1, AU>::CHUNK_COLS + 1;
     if constexpr (TPR == 32) {
-        if (nv == 1) return launch_ln<LnShape<T, PT, TPR, 1, ALIGNED>>(backward, p, blocks, stream);
+        if (nv == 1) return launch_ln<LnShape<T, PT, TPR, 1, AU>>(backward, p, blocks, stream);
     }
     if constexpr (TPR <= 64) {
-        if (nv == 2) return launch_ln<LnShape<T, PT, TPR, 2, ALIGNED>>(backward, p, blocks, stream);
+        if (nv == 2) return launch_ln<LnShape<T, PT, TPR, 2, AU>>(backward, p, blocks, stream);
     }
-    if (TPR == 32 || nv == 3) return launch_ln<LnShape<T, PT, TPR, 3, ALIGNED>>(backward, p, blocks, stream);
-    if constexpr (TPR > 32) return launch_ln<LnShape<T, PT, TPR, 4, ALIGNED>>(backward, p, blocks, stream);
+    if (TPR == 32 || nv == 3) return launch_ln<LnShape<T, PT, TPR, 3, AU>>(backward, p, blocks, stream);
+    if constexpr (TPR > 32) return launch_ln<LnShape<T, PT, TPR, 4, AU>>(backward, p, blocks, stream);
     return IB200_ERR_UNSUPPORTED;
 }
-template <class T, class PT, bool ALIGNED>
+template <class T, class PT, int AU>
 int launch_ln_shape(int dtype, bool backward, const LnRows& p, int blocks, cudaStream_t stream) {
     switch (ln_threads_per_row(p.C, dtype)) {
-        case 32: return launch_ln_row<T, PT, 32, ALIGNED>(backward, p, blocks, stream);
-        case 64: return launch_ln_row<T, PT, 64, ALIGNED>(backward, p, blocks, stream);
-        case 128: return launch_ln_row<T, PT, 128, ALIGNED>(backward, p, blocks, stream);
-        case 256: return launch_ln_row<T, PT, 256, ALIGNED>(backward, p, blocks, stream);
-        default: return launch_ln_row<T, PT, 512, ALIGNED>(backward, p, blocks, stream);
+        case 32: return launch_ln_row<T, PT, 32, AU>(backward, p, blocks, stream);
+        case 64: return launch_ln_row<T, PT, 64, AU>(backward, p, blocks, stream);
+        case 128: return launch_ln_row<T, PT, 128, AU>(backward, p, blocks, stream);
+        case 256: return launch_ln_row<T, PT, 256, AU>(backward, p, blocks, stream);
+        default: return launch_ln_row<T, PT, 512, AU>(backward, p, blocks, stream);
     }
 }
 // PT: type of weight and bias in the kernels for aligned rows.
@@ -853,9 +853,16 @@ template <class T, class PT>
 int launch_ln_type(int dtype, bool backward, const LnRows& p, int blocks, cudaStream_t stream) {
     constexpr int kVec = 16 / sizeof(T);
     const bool typed = (!p.w && !p.b) || p.param_bf16 == (sizeof(PT) == 2);
-    const bool aligned = typed && p.C % kVec == 0 && p.x_pitch % kVec == 0 && p.dy_pitch % kVec == 0 && aligned16(p.x) && aligned16(p.dy) && aligned16(p.w) &&
-                         aligned16(p.b) && aligned16(p.out);
-    return aligned ? launch_ln_shape<T, PT, true>(dtype, backward, p, blocks, stream) : launch_ln_shape<T, float, false>(dtype, backward, p, blocks, stream);
+    auto whole = [&](int elements) {       // rows begin on, and consist of, so many elements
+        auto on = [&](const void* t) { return reinterpret_cast<uintptr_t>(t) % (elements * sizeof(T)) == 0; };
+        return p.C % elements == 0 && p.x_pitch % elements == 0 && p.dy_pitch % elements == 0 && on(p.x) && on(p.dy) && on(p.out);
+    };
+    if (typed && whole(kVec) && aligned16(p.w) && aligned16(p.b)) return launch_ln_shape<T, PT, kVec>(dtype, backward, p, blocks, stream);
+    if constexpr (sizeof(T) == 2) {
+        const uintptr_t pair = p.param_bf16 ? 4 : 8;
+        if (whole(2) && reinterpret_cast<uintptr_t>(p.w) % pair == 0 && reinterpret_cast<uintptr_t>(p.b) % pair == 0) return launch_ln_shape<T, float, 2>(dtype, backward, p, blocks, stream);
+    }
+    return launch_ln_shape<T, float, 1>(dtype, backward, p, blocks, stream);
 }
 // fp32 rows with bf16 weights, which nobody keeps, share the kernels for rows that do not begin on 16 bytes.
 int launch_ln_any(int dtype, bool backward, const LnRows& p, int blocks, cudaStream_t stream) {

@@ -40,23 +40,24 @@ struct LnRows {
     float eps;
 };
 
-// TPR threads per row, chunks of 16 bytes, NV of them per thread.  PT: type of weight and bias.  ALIGNED: rows begin on 16 bytes and hold whole
-// chunks, and so do weight and bias; a thread's chunk is then 16 contiguous bytes.  Otherwise the same columns are dealt out element by
-// element, so that a warp's loads still run together, and the type of weight and bias is looked up.
+// TPR threads per row, chunks of 16 bytes, NV of them per thread.  AU: elements per access.  Where rows, weight and bias begin on 16 bytes and hold
+// whole chunks it is a chunk (ALIGNED), PT being the type of weight and bias; otherwise 4 bytes or a single bf16, dealt out to the threads in
+// turn, so that a warp's accesses still run together, and the type of weight and bias is looked up.
 constexpr int kLnBwdThreads = 512;      // a block of the backward, one per SM: as few blocks' sums as there can be
-template <class T_, class PT_, int TPR_, int NV_, bool ALIGNED_>
+template <class T_, class PT_, int TPR_, int NV_, int AU_>
 struct LnShape {
     using T = T_;
     using PT = PT_;
     static constexpr int TPR = TPR_, NV = NV_, VEC = 16 / sizeof(T_), WARPS = TPR_ / 32;
-    static constexpr bool ALIGNED = ALIGNED_;
+    static constexpr int AU = AU_;
+    static constexpr bool ALIGNED = AU_ * sizeof(T_) == 16, RING = AU_ * sizeof(T_) >= 4;      // (asynchronous copies are of 4 bytes at least)
     static constexpr int FWD_THREADS = TPR_ < 256 ? 256 : TPR_, FWD_ROWS = FWD_THREADS / TPR_, FWD_BLOCKS = 1024 / FWD_THREADS;      // blocks resident per SM
     static constexpr int BWD_ROWS = kLnBwdThreads / TPR_;
     static constexpr int CHUNK_COLS = TPR_ * VEC;                                       // columns of one chunk of all threads
     static constexpr int STAGES = 2;                                                    // rows of a thread's ring: this one and the next
     static constexpr int PARAM_UNITS = sizeof(PT_) * VEC / 16 ? sizeof(PT_) * VEC / 16 : 1;      // 16-byte units of a chunk's weights
-    static constexpr int FWD_SMEM = ALIGNED_ ? STAGES * NV_ * FWD_THREADS * 16 : 0;
-    static constexpr int BWD_RING = ALIGNED_ ? (STAGES * 2 + PARAM_UNITS) * NV_ * kLnBwdThreads * 16 : 0;
+    static constexpr int FWD_SMEM = RING ? STAGES * NV_ * FWD_THREADS * 16 : 0;
+    static constexpr int BWD_RING = RING ? (STAGES * 2 + PARAM_UNITS) * NV_ * kLnBwdThreads * 16 : 0;
     static constexpr int BWD_SUMS = kLnBwdThreads * VEC * 4;                            // one chunk's columns of every row at work, in the ring's place
     static constexpr int BWD_SMEM = BWD_RING > BWD_SUMS ? BWD_RING : BWD_SUMS;
 };
@@ -69,7 +70,7 @@ __device__ __forceinline__ void ln_from_float(float v, __nv_bfloat16& o) { o = _
 // Column of element e of chunk v of thread t; past the row's end: C and more.
 template <class S>
 __device__ __forceinline__ int ln_col(int v, int e, int t) {
-    return S::ALIGNED ? (v * S::TPR + t) * S::VEC + e : v * S::CHUNK_COLS + e * S::TPR + t;
+    return v * S::CHUNK_COLS + (e / S::AU * S::TPR + t) * S::AU + e % S::AU;
 }
 // A chunk in registers: pairs of fp32, for the packed arithmetic (two lanes an instruction: with single ones the issue slots, not the memory, bound
 // the forward).
@@ -129,6 +130,14 @@ __device__ __forceinline__ void ln_load_param(const void* p, int bf16, float non
     } else if (!p) {
 #pragma unroll
         for (int i = 0; i < S::VEC / 2; ++i) k.f[i] = pack_f32x2(none, none);
+    } else if constexpr (S::AU == 2) {               // pairs, which begin on their own size
+#pragma unroll
+        for (int i = 0; i < S::VEC / 2; ++i) {
+            const int c = ln_col<S>(v, 2 * i, t);
+            if (c >= C) k.f[i] = pack_f32x2(none, none);
+            else if (bf16) k.f[i] = ln_pair_bf16(*reinterpret_cast<const uint32_t*>(static_cast<const __nv_bfloat16*>(p) + c));
+            else k.f[i] = *reinterpret_cast<const uint64_t*>(static_cast<const float*>(p) + c);
+        }
     } else if (bf16) {
         ln_gather<S>(static_cast<const __nv_bfloat16*>(p), none, v, t, C, k);
     } else {
@@ -147,6 +156,12 @@ __device__ __forceinline__ void ln_store(typename S::T* row, int v, int t, int C
         if constexpr (S::VEC == 8) u = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
         else u = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
         *reinterpret_cast<uint4*>(row + c) = u;
+    } else if constexpr (S::AU == 2) {
+#pragma unroll
+        for (int e = 0; e < S::VEC; e += 2) {
+            const int c = ln_col<S>(v, e, t);
+            if (c < C) *reinterpret_cast<uint32_t*>(row + c) = pack_bf16x2(f[e], f[e + 1]);
+        }
     } else {
 #pragma unroll
         for (int e = 0; e < S::VEC; ++e) {
@@ -191,6 +206,9 @@ __device__ __forceinline__ float2 ln_row_sum(float a, float b, float2 (*slots)[1
 __device__ __forceinline__ void ln_copy_async(uint4* dst, const void* src, bool inside) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(inside ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void ln_copy_async4(void* dst, const void* src, bool inside) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(inside ? 4 : 0) : "memory");
+}
 __device__ __forceinline__ void ln_copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int PENDING>
 __device__ __forceinline__ void ln_copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
@@ -198,8 +216,17 @@ template <class S, int THREADS>
 __device__ __forceinline__ void ln_request(uint4* slots, const typename S::T* row, int t, int C) {
 #pragma unroll
     for (int v = 0; v < S::NV; ++v) {
-        const int c = ln_col<S>(v, 0, t);
-        ln_copy_async(slots + v * THREADS + threadIdx.x, row + (c < C ? c : 0), c < C);
+        uint4* slot = slots + v * THREADS + threadIdx.x;
+        if constexpr (S::ALIGNED) {
+            const int c = ln_col<S>(v, 0, t);
+            ln_copy_async(slot, row + (c < C ? c : 0), c < C);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = ln_col<S>(v, i * S::AU, t);
+                ln_copy_async4(reinterpret_cast<uint32_t*>(slot) + i, row + (c < C ? c : 0), c < C);
+            }
+        }
     }
 }
 
@@ -213,14 +240,14 @@ __global__ void __launch_bounds__(S::FWD_THREADS, S::FWD_BLOCKS) ln_fwd_kernel(c
     const int t = threadIdx.x % S::TPR;
     const long first = static_cast<long>(blockIdx.x) * S::FWD_ROWS + threadIdx.x / S::TPR, step = static_cast<long>(gridDim.x) * S::FWD_ROWS;
     const T* x0 = static_cast<const T*>(p.x);
-    if constexpr (S::ALIGNED) {
+    if constexpr (S::RING) {
         if (first < p.M) ln_request<S, S::FWD_THREADS>(ring, x0 + first * p.x_pitch, t, p.C);
         ln_copy_commit();
     }
     const float inv = 1.f / static_cast<float>(p.C);
     int stage = 0;
     for (long r = first; r < p.M; r += step) {
-        if constexpr (S::ALIGNED) {
+        if constexpr (S::RING) {
             if (r + step < p.M) ln_request<S, S::FWD_THREADS>(ring + (stage ^ 1) * S::NV * S::FWD_THREADS, x0 + (r + step) * p.x_pitch, t, p.C);
             ln_copy_commit();
             ln_copy_wait<1>();
@@ -228,7 +255,7 @@ __global__ void __launch_bounds__(S::FWD_THREADS, S::FWD_BLOCKS) ln_fwd_kernel(c
         // A chunk of the row, less `minus`; zeros past the row's end.  Read again in each of the three passes rather than held in fp32: with 32 registers
         // less there are twice as many rows at work on an SM.
         auto chunk = [&](int v, uint64_t minus, bool centred, LnChunk<S>& x) {
-            if constexpr (S::ALIGNED) {
+            if constexpr (S::RING) {
                 ln_unpack(ring[(stage * S::NV + v) * S::FWD_THREADS + threadIdx.x], x.f);
             } else {
                 ln_gather<S>(x0 + r * p.x_pitch, 0.f, v, t, p.C, x);
@@ -313,14 +340,24 @@ __global__ void __launch_bounds__(kLnBwdThreads, 1) ln_bwd_kernel(const LnRows p
         mean = p.mean[first];
         rstd = p.rstd[first];
     }
-    if constexpr (S::ALIGNED) {
+    if constexpr (S::RING) {
         if (p.w) {
 #pragma unroll
             for (int v = 0; v < S::NV; ++v) {
-                const int c = ln_col<S>(v, 0, t);
-                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const typename S::PT*>(p.w) + (c < p.C ? c : 0));
+                uint4* save = wsave + v * S::PARAM_UNITS * kLnBwdThreads + threadIdx.x;
+                if constexpr (S::ALIGNED) {
+                    const int c = ln_col<S>(v, 0, t);
+                    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const typename S::PT*>(p.w) + (c < p.C ? c : 0));
 #pragma unroll
-                for (int q = 0; q < S::PARAM_UNITS; ++q) ln_copy_async(wsave + (v * S::PARAM_UNITS + q) * kLnBwdThreads + threadIdx.x, src + q, c < p.C);
+                    for (int q = 0; q < S::PARAM_UNITS; ++q) ln_copy_async(save + q * kLnBwdThreads, src + q, c < p.C);
+                } else {                           // as fp32, whatever they are
+                    LnChunk<S> w;
+                    ln_load_param<S>(p.w, p.param_bf16, 1.f, v, t, p.C, w);
+#pragma unroll
+                    for (int q = 0; q < S::PARAM_UNITS; ++q)
+                        save[q * kLnBwdThreads] = make_uint4(static_cast<uint32_t>(w.f[2 * q]), static_cast<uint32_t>(w.f[2 * q] >> 32),
+                                                             static_cast<uint32_t>(w.f[2 * q + 1]), static_cast<uint32_t>(w.f[2 * q + 1] >> 32));
+                }
             }
         }
         if (first < p.M) request(0, first);
@@ -339,13 +376,13 @@ __global__ void __launch_bounds__(kLnBwdThreads, 1) ln_bwd_kernel(const LnRows p
             next_mean = p.mean[r + step];
             next_rstd = p.rstd[r + step];
         }
-        if constexpr (S::ALIGNED) {
+        if constexpr (S::RING) {
             if (r + step < p.M) request(stage ^ 1, r + step);
             ln_copy_commit();
             ln_copy_wait<1>();
         }
         auto weight = [&](int v, LnChunk<S>& w) {
-            if constexpr (S::ALIGNED) {
+            if constexpr (S::RING) {
                 if (p.w) {
                     uint4 u[S::PARAM_UNITS];
 #pragma unroll
@@ -362,7 +399,7 @@ __global__ void __launch_bounds__(kLnBwdThreads, 1) ln_bwd_kernel(const LnRows p
         // One chunk of both rows, xh and g: read again for the second pass rather than held, which would cost the registers that the sums are in.
         const uint64_t scale = pack_f32x2(rstd, rstd), minus = pack_f32x2(-mean, -mean);
         auto chunk = [&](int v, LnChunk<S>& x, LnChunk<S>& g) {
-            if constexpr (S::ALIGNED) {
+            if constexpr (S::RING) {
                 ln_unpack(ring[stage * ROW + v * kLnBwdThreads + threadIdx.x], x.f);
                 ln_unpack(ring[stage * ROW + (S::NV + v) * kLnBwdThreads + threadIdx.x], g.f);
             } else {
