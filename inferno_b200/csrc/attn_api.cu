@@ -700,17 +700,15 @@ size_t linear_bwd_ws_bytes(int K, int N) { return round_up(static_cast<size_t>(K
 
 // The helper ahead of a backward's products: column sums of dy (`part`), zeroing of the accumulators, and with `slope` dz = dy slope.
 int launch_linear_prep(const void* dy, const void* slope, void* dz, float* part, int M, int N, bool atomic, float* zero, size_t zero_floats, cudaStream_t stream) {
-    const int slabs = part || slope ? colsum_slabs(M, N) : 0, rows = slabs ? (M + slabs - 1) / slabs : 0, gx = (N + kColsumCols - 1) / kColsumCols;
-    const long n4 = static_cast<long>(zero_floats / 4);
-    const int zero_blocks = static_cast<int>(std::min<long>((n4 + 2047) / 2048, 4 * 148));
-    const dim3 grid(gx, slabs + (zero_blocks + gx - 1) / gx);
-    if (grid.y == 0) return IB200_OK;
+    const int slabs = colsum_slabs(M, N), rows = (M + slabs - 1) / slabs;
+    const dim3 grid((N + kColsumCols - 1) / kColsumCols, part || slope ? slabs : 64);
     float4* z4 = reinterpret_cast<float4*>(zero);
+    const long n4 = static_cast<long>(zero_floats / 4);
     const auto* g = static_cast<const __nv_bfloat16*>(dy);
     return slope ? launch_pdl<linear_prep_kernel<true>>(grid, 256, 0, stream, g, static_cast<const __half*>(slope), static_cast<__nv_bfloat16*>(dz), part, M, N, rows,
-                                                        slabs, static_cast<int>(atomic), z4, n4)
+                                                        static_cast<int>(atomic), z4, n4)
                  : launch_pdl<linear_prep_kernel<false>>(grid, 256, 0, stream, g, static_cast<const __half*>(nullptr), static_cast<__nv_bfloat16*>(nullptr), part, M, N,
-                                                         rows, slabs, static_cast<int>(atomic), z4, n4);
+                                                         rows, static_cast<int>(atomic), z4, n4);
 }
 
 // With `slope` (and a workspace) dy is first multiplied by it, into `dz`.

@@ -550,15 +550,18 @@ gemm_bf16_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ 
 constexpr int kColsumCols = 256, kMaxColsumSlabs = 128;
 template <bool SLOPE>
 __global__ void __launch_bounds__(256) linear_prep_kernel(const __nv_bfloat16* __restrict__ x, const __half* __restrict__ slope, __nv_bfloat16* __restrict__ dz,
-                                                          float* __restrict__ part, int M, int N, int rows_per_block, int slabs, int atomic,
-                                                          float4* __restrict__ zero, long zero4) {
+                                                          float* __restrict__ part, int M, int N, int rows_per_block, int atomic, float4* __restrict__ zero,
+                                                          long zero4) {
     pdl_wait();
     pdl_trigger();
-    if (static_cast<int>(blockIdx.y) >= slabs) {      // blocks past the row slabs zero: a block that did both read nothing until its stores had drained
-        const long step = static_cast<long>(gridDim.x) * (gridDim.y - slabs) * blockDim.x;
-        for (long i = (static_cast<long>(blockIdx.y - slabs) * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x; i < zero4; i += step) zero[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        return;
-    }
+    // The accumulators are zeroed behind the reads where there are only reads, and ahead of them where dz is written as well: backward of
+    // 8192 x 1024 x 4096 117.4 us (ahead: 120.2), with GELU 138.7 (behind: 141.2); 16384 x 768 x 768 with GELU 51.9 (54.1).
+    auto clear = [&] {
+        const long step = static_cast<long>(gridDim.x) * gridDim.y * blockDim.x;
+        for (long i = (static_cast<long>(blockIdx.y) * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x; i < zero4; i += step) zero[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    };
+    if (SLOPE || !part) clear();
+    if (!SLOPE && !part) return;
     __shared__ float sums[8][kColsumCols + 4];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int col = blockIdx.x * kColsumCols + lane * 8;
@@ -603,7 +606,6 @@ __global__ void __launch_bounds__(256) linear_prep_kernel(const __nv_bfloat16* _
         }
         for (; row < row1; row += 8) product(row * pitch, src[row * pitch], ssrc[row * pitch]);
     }
-    if (!part) return;
     if (!SLOPE && col < N) {
         const uint4* src = reinterpret_cast<const uint4*>(x + col);
         const long pitch = N / 8;
@@ -617,6 +619,8 @@ __global__ void __launch_bounds__(256) linear_prep_kernel(const __nv_bfloat16* _
         }
         for (; row < row1; row += 8) add(src[row * pitch]);
     }
+    if (!part) return;
+    if (!SLOPE) clear();
 #pragma unroll
     for (int e = 0; e < 8; ++e) sums[warp][lane * 8 + e] = acc[e];
     __syncthreads();
