@@ -14,6 +14,8 @@
 // which has up to four 16-byte chunks of it: a row of one warp needs no barrier.  The backward's threads keep their columns from row to row
 // and sum dw and db in registers; a block's sums meet in the workspace, which ln_finish_kernel adds up in a fixed order.  All sums are
 // fp32; the only rounding to fewer bits is that of the results.
+// Measured (us; floor at the measured copy rate): bf16 16384 x 8192 forward 101 (82), backward 126 (123); 16384 x 4096 55 (41), 68 (61); 16384 x 768 10.8 (7.7),
+// 19.8 (11.5); fp32 16384 x 1024 27 (20), 37 (31).  The forward is bound by issue slots (0.75 a cycle), the backward by memory.
 #pragma once
 
 #include <cuda_bf16.h>

@@ -21,6 +21,9 @@
 // MMAs into one of two 256-column TMEM accumulators, and eight warps drain the other accumulator (TMEM -> registers -> +bias ->
 // TMA store), so the epilogue of a tile overlaps the main loop of the next.
 //
+// Measured, us: 8192 x 1024 x 4096 47 (1470 TFLOP/s), with a residual 54, GELU 50, GELU with its slope kept 62; 16384 x 768 x 2304 43, 49, 50, 63.  The operands of a
+// pair at the tensor pipe's full rate are 64 bytes per clock and SM, all that an SM takes from L2: what an epilogue reads or writes more is added.
+//
 // One launch runs up to two products ("tasks"), so that dX and dW of a projection share a grid:
 //   task 0 is cut into whole tiles, dealt out round-robin;
 //   task 1 is either cut the same way (its tiles follow task 0's), or, when it has too few tiles for the chip and a long K

@@ -396,3 +396,14 @@ def test_a_transformer_block_of_these_operators():
     assert rel(y.detach(), yd.detach()) <= 2e-2
     for (name, g), wg in zip([("x", grads[0])] + list(zip(p, grads[1:])), want):
         assert rel(g, wg) <= 2e-2, (name, rel(g, wg))
+
+
+@pytest.mark.parametrize("M", [1, 3, 33, 1001])
+def test_plain_projection_takes_any_number_of_rows(M):
+    x, w, b, _, dy = problem(M, 136, 264, seed=M)
+    for t in (x, w, b):
+        t.requires_grad_()
+    y = L.LinearFunction.apply(x, w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    _, wy, wdx, wdw, wdb, _ = reference(x.detach(), w.detach(), b.detach(), None, dy, False)
+    assert rel(y.detach(), wy) <= ONE and rel(dx, wdx) <= ONE and rel(dw, wdw) <= ONE and rel(db, wdb) <= ONE
