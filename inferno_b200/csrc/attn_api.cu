@@ -503,9 +503,9 @@ int launch_gemm_form(int pairs, const GemmMaps& maps, const GemmParams& p, cudaS
 // together, and saves the slices that other pairs take over, 0.3 us each.  Whole against cut, us: 777 x 1000 x 2008 (saves 8 slices) 15.1 and 16.3,
 // 17 x 1024 x 4096 (8) 12.2 and 10.9, 512 x 2048 x 512 (24) 17.0 and 13.0, 1023 x 4096 x 1024 (48) 27.0 and 19.1, 64 x 4096 x 1024 (56) 25.7 and 12.2.
 constexpr int kMinSavedSlices = 12;
-int gemm_slabs(const GemmDesc& d, int pairs) {
+int gemm_slabs(const GemmDesc& d, int pairs, int least = kMinSavedSlices) {
     const int parts = std::min(std::min(8, pairs / d.tiles()), d.k_slices() / kMinPartSlices);
-    return parts > 1 && d.k_slices() - (d.k_slices() + parts - 1) / parts > kMinSavedSlices ? parts : 1;
+    return parts > 1 && d.k_slices() - (d.k_slices() + parts - 1) / parts > least ? parts : 1;
 }
 
 // One launch: `whole` cut into whole tiles (may be null), `other` cut into whole tiles or, with split != kPartWhole, along K.
@@ -663,6 +663,16 @@ int linear_few(const void* w, FewRows p, int sms, cudaStream_t stream) {
     }
 }
 
+// Adds up the slabs of a product that was cut along K; `p`: its epilogue.
+int launch_fused_finish(FusedFinish p, const void* slabs_at, int slabs, int M, int N, void* y, cudaStream_t stream) {
+    p.acc = static_cast<const float4*>(slabs_at);
+    p.slabs = slabs;
+    p.y = static_cast<uint4*>(y);
+    p.n8 = static_cast<long>(M) * N / 8;
+    p.N = N;
+    return launch_pdl<linear_fused_finish_kernel>(static_cast<int>(std::min<long>((p.n8 + 255) / 256, 148 * 8)), 256, 0, stream, p);
+}
+
 // y = act(x w + bias) + residual.
 int fused_linear_fwd_core(const GemmDesc& d, const void* bias, int bias_bf16, const void* residual, void* slope, bool gelu, void* ws, size_t ws_bytes,
                           cudaStream_t stream) {
@@ -679,9 +689,13 @@ int fused_linear_fwd_core(const GemmDesc& d, const void* bias, int bias_bf16, co
     const int slabs = gemm_slabs(d, dev->sms / 2);
     if (slabs > 1 && ws && ws_bytes >= slabs * n * 4) {
         if ((rc = launch_gemms(nullptr, &d, kPartSlab, static_cast<float*>(ws), nullptr, 0, stream))) return rc;
-        const FusedFinish p{static_cast<const float4*>(ws), slabs, bias, bias_bf16, gelu, static_cast<const uint4*>(residual), static_cast<uint4*>(slope), static_cast<uint4*>(d.c),
-                            static_cast<long>(n / 8), d.N};
-        return launch_pdl<linear_fused_finish_kernel>(static_cast<int>(std::min<long>((p.n8 + 255) / 256, 148 * 8)), 256, 0, stream, p);
+        FusedFinish p{};
+        p.bias = bias;
+        p.bias_bf16 = bias_bf16;
+        p.gelu = gelu;
+        p.residual = static_cast<const uint4*>(residual);
+        p.slope = static_cast<uint4*>(slope);
+        return launch_fused_finish(p, ws, slabs, d.M, d.N, d.c, stream);
     }
     GemmEpi epi;
     epi.mode = gelu ? kEpiGelu : residual ? kEpiResidual : kEpiBias;
@@ -711,9 +725,20 @@ int launch_linear_prep(const void* dy, const void* slope, void* dz, float* part,
                                                          rows, static_cast<int>(atomic), z4, n4);
 }
 
-// With `slope` (and a workspace) dy is first multiplied by it, into `dz`.
+// dX (and dW) of a projection whose dX has few tiles and a long contraction: dX in slabs, dW in whole tiles beside them, and the slabs' sum.
+int launch_dx_slabs(const GemmDesc& gx, const GemmDesc* gw, int parts, void* slabs, cudaStream_t stream) {
+    const int rc = launch_gemms(gw, &gx, kPartSlab, static_cast<float*>(slabs), nullptr, 0, stream);
+    return rc ? rc : launch_fused_finish(FusedFinish{}, slabs, parts, gx.M, gx.N, gx.c, stream);
+}
+// Parts of dX.  It has a launch more to pay for than a forward, and dW beside it must not want to be cut (along the tokens) itself.  Uncut and cut, us:
+// backward of 777 x 1000 x 2008 (saves 24 slices) 22.9 and 26.1, 5 x 1024 x 4096 (56) 25.8 and 16.8; feed-forward of 1023 x 1024 x 4096 (48) 73 and 62, of
+// 1 x 2048 x 8192 (112) 79 and 55, of 4096 x 512 x 2048 (16) 51 and 68.
+int dx_parts(int M, int K, int N, int pairs) { return M > 1024 ? 1 : gemm_slabs(GemmDesc{nullptr, nullptr, nullptr, M, K, N, 0, 0}, pairs, 32); }
+
+// With `slope` (and a workspace) dy is first multiplied by it, into `dz`.  `slabs`: room for dx_parts fp32 matrices like dX, or null: then a dX alone
+// that is cut along N is added up in bf16.
 int linear_bwd_core(const void* x, const void* w, const void* dy, void* dx, void* dw, void* db, int db_bf16, int M, int K, int N, void* ws, size_t ws_bytes,
-                    cudaStream_t stream, const void* slope = nullptr, void* dz = nullptr) {
+                    cudaStream_t stream, const void* slope = nullptr, void* dz = nullptr, void* slabs = nullptr) {
     if (!x || !w || !dy) return IB200_ERR_INVALID_ARGUMENT;
     const void* g = slope ? dz : dy;
     // dx[M,K] = g[M,N] w^T: w is stored [K, N], i.e. the "B" of this product stored [N_out = K rows, contraction N contiguous]
@@ -731,7 +756,8 @@ int linear_bwd_core(const void* x, const void* w, const void* dy, void* dx, void
     const DeviceInfo* dev = device_info();
     if (!dev) return IB200_ERR_CUDA;
     const int pairs = dev->sms / 2;
-    const bool split = dw && have_ws && (dx ? gemm_wants_split_beside(gw, pairs) : gemm_wants_split(gw, pairs));
+    const int parts = dx && slabs ? dx_parts(M, K, N, pairs) : 1;
+    const bool split = dw && have_ws && parts == 1 && (dx ? gemm_wants_split_beside(gw, pairs) : gemm_wants_split(gw, pairs));
     float* acc = split ? static_cast<float*>(ws) : nullptr;
     float* part = nullptr;
     if (db) {
@@ -741,8 +767,12 @@ int linear_bwd_core(const void* x, const void* w, const void* dy, void* dx, void
     if (db || split || slope) {
         if ((rc = launch_linear_prep(dy, slope, dz, part, M, N, !have_ws, acc, split ? static_cast<size_t>(K) * N : 0, stream))) return rc;
     }
-    if (have_ws && dx && dw) {
+    if (parts > 1) {
+        if ((rc = launch_dx_slabs(gx, dw ? &gw : nullptr, parts, slabs, stream))) return rc;
+    } else if (have_ws && dx && dw) {
         if ((rc = launch_gemms(&gx, &gw, split ? kPartReduceF32 : kPartWhole, acc, nullptr, 0, stream))) return rc;
+    } else if (slabs && dx) {
+        if ((rc = launch_gemms(&gx, nullptr, kPartWhole, nullptr, nullptr, 0, stream))) return rc;
     } else {
         if (dx && (rc = gemm_single(gx, nullptr, 0, nullptr, 0, stream))) return rc;
         if (dw && split && (rc = launch_gemms(nullptr, &gw, kPartReduceF32, acc, nullptr, 0, stream))) return rc;
@@ -751,34 +781,47 @@ int linear_bwd_core(const void* x, const void* w, const void* dy, void* dx, void
     return launch_linear_finish(finish_job(acc, dw, static_cast<long>(K) * N, part, colsum_slabs(M, N), N, have_ws ? db : nullptr, db_bf16), stream);
 }
 
+// Workspace of a fused projection's backward: [what a projection's takes | dz | dx's slabs].
+struct FusedBwdWorkspace {
+    size_t dz, slabs, bytes;
+    FusedBwdWorkspace(int M, int K, int N, int activation) {
+        const DeviceInfo* dev = device_info();
+        const int parts = dx_parts(M, K, N, (dev ? dev->sms : 148) / 2);
+        dz = round_up(linear_bwd_ws_bytes(K, N), 256);
+        slabs = dz + (activation == IB200_ACT_GELU ? round_up(static_cast<size_t>(M) * N * 2, 256) : 0);
+        bytes = slabs + (parts > 1 ? static_cast<size_t>(parts) * M * K * 4 : 0);
+    }
+};
+
 // The feed-forward block's backward: dz = (dy w2^T) slope with the columns' sums in the epilogue of that product, which shares its launch with
-// dw2 = h^T dy; then dx = dz w1^T and dw1 = x^T dz in another.  Workspace: [acc1 | acc2 | dy's column sums | dz's column sums | dz].
+// dw2 = h^T dy; then dx = dz w1^T and dw1 = x^T dz in another.  Workspace: [acc1 | acc2 | dy's column sums | dz's column sums | dz | dx's slabs].
 struct FfWorkspace {
-    size_t acc1, acc2, part2, part1, dz, bytes;
-    FfWorkspace(int M, int C, int H) {
+    size_t acc1, acc2, part2, part1, dz, slabs, bytes;
+    FfWorkspace(int M, int C, int H, int parts) {
         const size_t w = round_up(static_cast<size_t>(C) * H * 4, 256);
         acc1 = 0;
         acc2 = w;
         part2 = 2 * w;
         part1 = part2 + round_up(static_cast<size_t>(kMaxColsumSlabs) * C * 4, 256);
         dz = part1 + round_up((static_cast<size_t>(M) + 31) / 32 * H * 4, 256);
-        bytes = dz + round_up(static_cast<size_t>(M) * H * 2, 256);
+        slabs = dz + round_up(static_cast<size_t>(M) * H * 2, 256);
+        bytes = slabs + (parts > 1 ? static_cast<size_t>(parts) * M * C * 4 : 0);
     }
 };
 int ff_bwd_core(const void* x, const void* w1, const void* kept, const void* h, const void* w2, const void* dy, void* dx, void* dw1, void* db1, int db1_bf16,
                 void* dw2, void* db2, int db2_bf16, int M, int C, int H, uint8_t* ws, cudaStream_t stream) {
-    const FfWorkspace L(M, C, H);
+    const DeviceInfo* dev = device_info();
+    const int pairs = (dev ? dev->sms : 148) / 2, parts = dx ? dx_parts(M, C, H, pairs) : 1;
+    const FfWorkspace L(M, C, H, parts);
     const bool inner = dx || dw1 || db1;
     void* dz = ws + L.dz;
     const GemmDesc gz{dy, w2, dz, M, H, C, 0, 0}, gw2{h, dy, dw2, H, C, M, 1, 1}, gx{dz, w1, dx, M, C, H, 0, 0}, gw1{x, dz, dw1, C, H, M, 1, 1};
     int rc;
     if ((inner && (rc = gemm_check(gz))) || (dw2 && (rc = gemm_check(gw2))) || (dx && (rc = gemm_check(gx))) || (dw1 && (rc = gemm_check(gw1)))) return rc;
     if (!aligned16(dy) || !aligned16(kept)) return IB200_ERR_MISALIGNED;
-    const DeviceInfo* dev = device_info();
     if (!dev) return IB200_ERR_NO_DEVICE;
-    const int pairs = dev->sms / 2;
     const bool split2 = dw2 && (inner ? gemm_wants_split_beside(gw2, pairs) : gemm_wants_split(gw2, pairs));
-    const bool split1 = dw1 && (dx ? gemm_wants_split_beside(gw1, pairs) : gemm_wants_split(gw1, pairs));
+    const bool split1 = dw1 && parts == 1 && (dx ? gemm_wants_split_beside(gw1, pairs) : gemm_wants_split(gw1, pairs));
     float *acc1 = split1 ? reinterpret_cast<float*>(ws + L.acc1) : nullptr, *acc2 = split2 ? reinterpret_cast<float*>(ws + L.acc2) : nullptr;
     float *part1 = db1 ? reinterpret_cast<float*>(ws + L.part1) : nullptr, *part2 = db2 ? reinterpret_cast<float*>(ws + L.part2) : nullptr;
     if (db2 || split1 || split2) {
@@ -794,10 +837,12 @@ int ff_bwd_core(const void* x, const void* w1, const void* kept, const void* h, 
     } else if (dw2) {
         if ((rc = split2 ? launch_gemms(nullptr, &gw2, kPartReduceF32, acc2, nullptr, 0, stream) : gemm_single(gw2, nullptr, 0, nullptr, 0, stream))) return rc;
     }
-    if (dx && dw1) {
+    if (parts > 1) {
+        if ((rc = launch_dx_slabs(gx, dw1 ? &gw1 : nullptr, parts, ws + L.slabs, stream))) return rc;
+    } else if (dx && dw1) {
         if ((rc = launch_gemms(&gx, &gw1, split1 ? kPartReduceF32 : kPartWhole, acc1, nullptr, 0, stream))) return rc;
     } else {
-        if (dx && (rc = gemm_single(gx, nullptr, 0, nullptr, 0, stream))) return rc;
+        if (dx && (rc = launch_gemms(&gx, nullptr, kPartWhole, nullptr, nullptr, 0, stream))) return rc;
         if (dw1 && (rc = split1 ? launch_gemms(nullptr, &gw1, kPartReduceF32, acc1, nullptr, 0, stream) : gemm_single(gw1, nullptr, 0, nullptr, 0, stream))) return rc;
     }
     const long n = static_cast<long>(C) * H;
@@ -1156,8 +1201,7 @@ size_t ib200_fused_linear_workspace_bytes(int M, int K, int N, int activation, i
         const int slabs = gemm_slabs(GemmDesc{nullptr, nullptr, nullptr, M, N, K, 0, 1}, dev->sms / 2);
         return slabs > 1 ? static_cast<size_t>(slabs) * M * N * 4 : 0;
     }
-    const size_t base = linear_bwd_ws_bytes(K, N);
-    return activation == IB200_ACT_GELU ? round_up(base, 256) + static_cast<size_t>(M) * N * 2 : base;
+    return FusedBwdWorkspace(M, K, N, activation).bytes;
 }
 
 int ib200_fused_linear_fwd(const void* x, const void* w, const void* bias, int bias_dtype, const void* residual, int activation, void* y, void* slope, int M, int K,
@@ -1177,11 +1221,17 @@ int ib200_fused_linear_bwd(const void* x, const void* w, const void* dy, const v
     if (!workspace || !aligned16(workspace) || workspace_bytes < ib200_fused_linear_workspace_bytes(M, K, N, activation, IB200_PASS_BWD)) return IB200_ERR_WORKSPACE;
     if (!dx && !dw && !db) return IB200_OK;
     if (N % 8) return IB200_ERR_UNSUPPORTED;
-    void* dz = slope ? static_cast<uint8_t*>(workspace) + round_up(linear_bwd_ws_bytes(K, N), 256) : nullptr;
-    return linear_bwd_core(x, w, dy, dx, dw, db, db_dtype == IB200_DTYPE_BF16, M, K, N, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream), slope, dz);
+    const FusedBwdWorkspace L(M, K, N, activation);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    return linear_bwd_core(x, w, dy, dx, dw, db, db_dtype == IB200_DTYPE_BF16, M, K, N, ws, workspace_bytes, reinterpret_cast<cudaStream_t>(stream), slope, ws + L.dz,
+                           ws + L.slabs);
 }
 
-size_t ib200_feed_forward_workspace_bytes(int M, int C, int H) { return M <= 0 || C <= 0 || H <= 0 ? 0 : FfWorkspace(M, C, H).bytes; }
+size_t ib200_feed_forward_workspace_bytes(int M, int C, int H) {
+    if (M <= 0 || C <= 0 || H <= 0) return 0;
+    const DeviceInfo* dev = device_info();
+    return FfWorkspace(M, C, H, dx_parts(M, C, H, (dev ? dev->sms : 148) / 2)).bytes;
+}
 
 int ib200_feed_forward_bwd(const void* x, const void* w1, const void* slope, const void* h, const void* w2, const void* dy, void* dx, void* dw1, void* db1,
                            int db1_dtype, void* dw2, void* db2, int db2_dtype, int M, int C, int H, void* workspace, size_t workspace_bytes, ib200_stream_t stream) {

@@ -30,8 +30,9 @@
 //   (a weight gradient: K = tokens), into contiguous runs of k-slices, one per CTA pair, sized so that every pair ends up
 //   with the same number of k-slices over both tasks.  The partial tiles meet by TMA reduction: in an fp32 workspace, zeroed
 //   before and rounded once to bf16 afterwards by linear_finish_kernel, or, for callers without a workspace, in the zeroed
-//   bf16 output itself (one rounding per partial, at most eight).  A forward with a fused epilogue is cut into equal parts, each with an fp32
-//   matrix of its own, which linear_fused_finish_kernel adds up in order: nothing to zero, and the result repeats.
+//   bf16 output itself (one rounding per partial, at most eight).  A forward with a fused epilogue,
+//   and the dX of a few rows, are cut into equal parts, each with an fp32 matrix of its own, which linear_fused_finish_kernel adds up in
+//   order: nothing to zero, and the result repeats.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -90,8 +91,8 @@ enum : int { kPartWhole = 0, kPartReduceBf16 = 1, kPartReduceF32 = 2, kPartSlab 
 struct GemmParams {
     GemmTask t[2];
     int split;             // task 1: kPartWhole, or how partial tiles are added up
-    // split runs: pair c starts at k-slice total1 * (min(c, heavy) * w_heavy + max(0, c - heavy) * w_light) / w_total of task 1
     int slabs;             // kPartSlab: parts of a tile
+    // split runs: pair c starts at k-slice total1 * (min(c, heavy) * w_heavy + max(0, c - heavy) * w_light) / w_total of task 1
     int heavy;
     long long w_heavy, w_light, w_total;
     const void* bias;      // [N] of task 0 (task 1 when it is the only one), or null
@@ -181,7 +182,7 @@ __device__ __forceinline__ uint64_t bias_pair(const GemmParams& p, uint2 b) {
 // infinite).  Constants: -2 sqrt(2 / pi) log2 e, and that times 0.044715.
 constexpr float kGeluExp1 = -2.302208198f, kGeluExp3 = kGeluExp1 * 0.044715f;
 constexpr float kGeluDu1 = 1.595769122f, kGeluDu3 = kGeluDu1 * 3.f * 0.044715f;      // d(2u)/dz = kGeluDu1 + kGeluDu3 z^2
-// Two at a time: the polynomials in packed fp32, an exponential and a reciprocal each (gelu of 64 elements a thread: 290 issue slots, 510 one by one).
+// Two at a time: the polynomials in packed fp32, an exponential and a reciprocal each (gelu of 64 elements a thread: about 290 issue slots, 510 one by one).
 __device__ __forceinline__ uint64_t splat2(float a) { return pack_f32x2(a, a); }
 __device__ __forceinline__ uint64_t gelu_gate2(uint64_t z, uint64_t zz) {            // s(2u)
     float a, b;
@@ -338,7 +339,7 @@ gemm_bf16_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ 
         // of the tile), so no barrier ties the warps together.  Registers straight to global memory (a 32-byte sector per thread) took 6200
         // cycles a tile, at three cycles per sector, and 2800 more in the release of the accumulator, which had to wait for the stores; four
         // warps that shared staging panels under named barriers took 7300.
-        // A thread holds pairs of columns of four rows (tmem_ld_16x256b_x8), the same columns in each, so the bias is eight pairs in registers, and the
+        // A thread holds pairs of columns of four rows (tmem_ld_16x256b_x8), the same columns in each, so a step's bias is eight shuffles, and the
         // arithmetic is packed.  With a row per thread each element's bias came by a shuffle, and two warps a scheduler could not hide it
         // all: 15000 cycles a 256 x 256 tile with GELU and z, 10800 with a residual (8192 x 1024 x 4096: 69.7 and 56.8 us).
         const int h = warp >> 2, row0 = (warp & 3) * 32;
@@ -688,7 +689,7 @@ __global__ void __launch_bounds__(256) linear_finish_kernel(const __grid_constan
     }
 }
 
-// Behind a forward product that was cut along K: its parts' sum, and the epilogue on it, 8 elements per thread.
+// Behind a product that was cut along K into slabs: their sum, and the epilogue on it, 8 elements per thread.
 struct FusedFinish {
     const float4* acc;          // [slabs][M][N]
     int slabs;

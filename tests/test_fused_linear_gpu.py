@@ -407,3 +407,25 @@ def test_plain_projection_takes_any_number_of_rows(M):
     dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
     _, wy, wdx, wdw, wdb, _ = reference(x.detach(), w.detach(), b.detach(), None, dy, False)
     assert rel(y.detach(), wy) <= ONE and rel(dx, wdx) <= ONE and rel(dw, wdw) <= ONE and rel(db, wdb) <= ONE
+
+
+@pytest.mark.parametrize("M,K,N", [(1, 264, 4096), (5, 1024, 4096), (40, 2048, 8192), (300, 512, 4104), (600, 256, 2056)])
+def test_few_rows_backward(M, K, N):
+    """dX of few rows is cut along its long contraction and added up in fp32: rounded once, with weights that need gradients or not, and repeats."""
+    x, w, b, res, dy = problem(M, K, N, seed=M + N)
+    for act in (False, True):
+        slope = L.fused_linear_forward(x, w, b, "gelu", None, True)[1] if act else None
+        _, _, wdx, wdw, wdb, sdb = reference(x, w, b, None, dy, act)
+        name = "gelu" if act else None
+        full = L.fused_linear_backward(x, w, dy, slope, name)
+        alone = L.fused_linear_backward(x, w, dy, slope, name, True, False, False)[0]
+        assert rel(full[0], wdx) <= (TWO if act else ONE) and rel(full[1], wdw) <= (TWO if act else ONE)
+        assert float((full[2].double() - wdb).norm()) <= (2.0 ** -11 if act else 2.0 ** -18) * float(sdb.norm()) + 2.0 ** -18 * float(wdb.norm())
+        assert rel(alone, wdx) <= (TWO if act else ONE) and torch.equal(full[0], L.fused_linear_backward(x, w, dy, slope, name)[0])
+    C, H = K, N
+    x, w1, b1, w2, b2, res, dy = ff_problem(M, C, H, seed=M)
+    x.requires_grad_()
+    dx, = torch.autograd.grad(L.feed_forward(x, w1, b1, w2, b2, res), x, dy)
+    want = ff_reference(x.detach(), w1, b1, w2, b2, res, dy)
+    assert rel(dx, want[2]) <= TWO
+    check_ff(x.detach().clone(), w1, b1, w2, b2, res, dy)
