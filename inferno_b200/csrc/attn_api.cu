@@ -597,6 +597,16 @@ int launch_linear_finish(const FinishJob& one, const FinishJob& two, cudaStream_
 }
 int launch_linear_finish(const FinishJob& one, cudaStream_t stream) { return launch_linear_finish(one, FinishJob{}, stream); }
 
+// Adds up the slabs of a product that was cut along K; `p`: its epilogue.
+int launch_fused_finish(FusedFinish p, const void* slabs_at, int slabs, int M, int N, void* y, cudaStream_t stream) {
+    p.acc = static_cast<const float4*>(slabs_at);
+    p.slabs = slabs;
+    p.y = static_cast<uint4*>(y);
+    p.n8 = static_cast<long>(M) * N / 8;
+    p.N = N;
+    return launch_pdl<linear_fused_finish_kernel>(static_cast<int>(std::min<long>((p.n8 + 255) / 256, 148 * 8)), 256, 0, stream, p);
+}
+
 // One product.  With a workspace of at least M * N floats a split product is added up in fp32.
 int gemm_single(const GemmDesc& d, const void* bias, int bias_bf16, void* ws, size_t ws_bytes, cudaStream_t stream) {
     int rc = gemm_check(d);
@@ -611,8 +621,11 @@ int gemm_single(const GemmDesc& d, const void* bias, int bias_bf16, void* ws, si
         return launch_gemms(nullptr, &d, kPartReduceBf16, nullptr, bias, bias_bf16, stream);
     }
     if (!cuda_ok(cudaMemsetAsync(ws, 0, n * 4, stream))) return IB200_ERR_CUDA;
-    if ((rc = launch_gemms(nullptr, &d, kPartReduceF32, static_cast<float*>(ws), bias, bias_bf16, stream))) return rc;
-    return launch_linear_finish(finish_job(static_cast<const float*>(ws), d.c, static_cast<long>(n), nullptr, 0, 0, nullptr, 0), stream);
+    if ((rc = launch_gemms(nullptr, &d, kPartReduceF32, static_cast<float*>(ws), nullptr, 0, stream))) return rc;
+    FusedFinish f{};
+    f.bias = bias;
+    f.bias_bf16 = bias_bf16;
+    return launch_fused_finish(f, ws, 1, d.M, d.N, d.c, stream);
 }
 
 bool valid_dtype(int dtype) { return dtype == IB200_DTYPE_F32 || dtype == IB200_DTYPE_BF16; }
@@ -661,16 +674,6 @@ int linear_few(const void* w, FewRows p, int sms, cudaStream_t stream) {
         case 2: return launch_few<2, 32>(wmap, p, strips, stream);
         default: return launch_few<4, 32>(wmap, p, strips, stream);
     }
-}
-
-// Adds up the slabs of a product that was cut along K; `p`: its epilogue.
-int launch_fused_finish(FusedFinish p, const void* slabs_at, int slabs, int M, int N, void* y, cudaStream_t stream) {
-    p.acc = static_cast<const float4*>(slabs_at);
-    p.slabs = slabs;
-    p.y = static_cast<uint4*>(y);
-    p.n8 = static_cast<long>(M) * N / 8;
-    p.N = N;
-    return launch_pdl<linear_fused_finish_kernel>(static_cast<int>(std::min<long>((p.n8 + 255) / 256, 148 * 8)), 256, 0, stream, p);
 }
 
 // y = act(x w + bias) + residual.

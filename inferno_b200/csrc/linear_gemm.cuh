@@ -377,7 +377,8 @@ gemm_bf16_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ 
             const bool fused = EPI != kEpiBias && q.task == 0;
             const uint32_t buf = n & 1;
             const int row = q.m0 + static_cast<int>(rank) * TR::CM + row0;
-            const bool with_bias = EPI != kEpiSlope && prm.bias && q.ks0 == 0;      // the part that starts the tile's K range brings the bias in
+            const bool with_bias = EPI != kEpiSlope && prm.bias && q.ks0 == 0;      // (a part that is added in bf16: the one that starts the tile's K range)
+            const bool f32_part = q.partial && prm.split >= kPartReduceF32;
             mbar_wait(&acc_full[buf], (n >> 1) & 1, ab, 30);
             tc_fence_after_sync();
             GemmPart ahead;
@@ -387,14 +388,40 @@ gemm_bf16_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ 
                 const int col = q.n0 + c0;
                 const bool inside = row < k.M && col < k.N, last = c0 != colf;
                 uint32_t r[2][32];
-                tmem_ld_16x256b_x8(tmem + buf * BN + c0 + lane_base, r[0]);
-                tmem_ld_16x256b_x8(tmem + buf * BN + c0 + lane_base + (16u << 16), r[1]);
+                if (f32_part) {
+                    // A row per lane, for 16-byte stores of fp32.  Backward of 1000 x 768 x 768 and 16384 x 768 x 768, us: 15.0 and 41.0; pairs stored 8 bytes
+                    // at a time 15.5 and 40.9; added in memory straight from the registers 16.1 and 45.
+                    tmem_ld_x32(tmem + buf * BN + c0 + lane_base, r[0]);
+                    tmem_ld_x32(tmem + buf * BN + c0 + 32 + lane_base, r[1]);
+                } else {
+                    tmem_ld_16x256b_x8(tmem + buf * BN + c0 + lane_base, r[0]);
+                    tmem_ld_16x256b_x8(tmem + buf * BN + c0 + lane_base + (16u << 16), r[1]);
+                }
                 tmem_wait_ld();
                 if (last) {
                     // every column of the accumulator is in registers: hand it back to the MMA warp
                     tc_fence_before_sync();
                     __syncwarp();
                     if (lane == 0) mbar_arrive_cluster_relaxed(free_bar[buf]);
+                }
+                if (f32_part) {
+                    if (inside) {
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            if (col + 32 * half >= k.N) continue;
+                            tile_free();
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) st_shared_sw128(stage, lane, c, make_uint4(r[half][4 * c], r[half][4 * c + 1], r[half][4 * c + 2], r[half][4 * c + 3]));
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                            if (lane == 0) {
+                                // rows / columns past M / N are clipped by the copy
+                                if (prm.split == kPartSlab) tma_store_3d(&maps.sum, stage, col + 32 * half, row, pair % prm.slabs);
+                                else tma_reduce_add_3d(&maps.sum, stage, col + 32 * half, row, 0);
+                                tma_store_commit();
+                            }
+                        }
+                    }
                 }
                 // rows 8i + lane / 4, columns 8j + pair_col
                 uint64_t v[4][8];
@@ -425,41 +452,20 @@ gemm_bf16_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ 
                     else if (more_ahead) request_aux(ahead, colf);
                 };
                 if (!inside || !fused) request_next_aux();
-                if (!inside) continue;
+                if (!inside || f32_part) continue;
                 tile_free();
                 if (!fused) {
-                    const CUtensorMap* mc = q.partial ? &maps.sum : &maps.c[q.task];
-                    if (q.partial && prm.split >= kPartReduceF32) {
 #pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            if (half) tile_free();
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                                for (int i = 0; i < 4; ++i)      // 32 columns of fp32: a pair is half a 16-byte chunk
-                                    *reinterpret_cast<uint64_t*>(stage + sw128_offset(8 * i + (lane >> 2), 2 * j + ((lane & 3) >> 1)) + (lane & 1) * 8) = v[i][4 * half + j];
-                            fence_proxy_async_smem();
-                            __syncwarp();
-                            if (lane == 0 && col + 32 * half < k.N) {
-                                // rows / columns past M / N are clipped by the copy
-                                if (prm.split == kPartSlab) tma_store_3d(mc, stage, col + 32 * half, row, pair % prm.slabs);
-                                else tma_reduce_add_3d(mc, stage, col + 32 * half, row, 0);
-                                tma_store_commit();
-                            }
-                        }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const uint32_t w[4] = {pack_bf16_pair(v[0][j]), pack_bf16_pair(v[1][j]), pack_bf16_pair(v[2][j]), pack_bf16_pair(v[3][j])};
-                            st_matrix_sw128(stage, lane, j, w);
-                        }
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                        if (lane == 0) {
-                            if (q.partial) tma_reduce_add_3d(mc, stage, col, row, 0);
-                            else tma_store_3d(mc, stage, col, row, 0);
-                            tma_store_commit();
-                        }
+                    for (int j = 0; j < 8; ++j) {
+                        const uint32_t w[4] = {pack_bf16_pair(v[0][j]), pack_bf16_pair(v[1][j]), pack_bf16_pair(v[2][j]), pack_bf16_pair(v[3][j])};
+                        st_matrix_sw128(stage, lane, j, w);
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (q.partial) tma_reduce_add_3d(&maps.sum, stage, col, row, 0);
+                        else tma_store_3d(&maps.c[q.task], stage, col, row, 0);
+                        tma_store_commit();
                     }
                     continue;
                 }
