@@ -621,11 +621,8 @@ int gemm_single(const GemmDesc& d, const void* bias, int bias_bf16, void* ws, si
         return launch_gemms(nullptr, &d, kPartReduceBf16, nullptr, bias, bias_bf16, stream);
     }
     if (!cuda_ok(cudaMemsetAsync(ws, 0, n * 4, stream))) return IB200_ERR_CUDA;
-    if ((rc = launch_gemms(nullptr, &d, kPartReduceF32, static_cast<float*>(ws), nullptr, 0, stream))) return rc;
-    FusedFinish f{};
-    f.bias = bias;
-    f.bias_bf16 = bias_bf16;
-    return launch_fused_finish(f, ws, 1, d.M, d.N, d.c, stream);
+    if ((rc = launch_gemms(nullptr, &d, kPartReduceF32, static_cast<float*>(ws), bias, bias_bf16, stream))) return rc;
+    return launch_linear_finish(finish_job(static_cast<const float*>(ws), d.c, static_cast<long>(n), nullptr, 0, 0, nullptr, 0), stream);
 }
 
 bool valid_dtype(int dtype) { return dtype == IB200_DTYPE_F32 || dtype == IB200_DTYPE_BF16; }

@@ -377,8 +377,8 @@ gemm_bf16_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ 
             const bool fused = EPI != kEpiBias && q.task == 0;
             const uint32_t buf = n & 1;
             const int row = q.m0 + static_cast<int>(rank) * TR::CM + row0;
-            const bool with_bias = EPI != kEpiSlope && prm.bias && q.ks0 == 0;      // (a part that is added in bf16: the one that starts the tile's K range)
-            const bool f32_part = q.partial && prm.split >= kPartReduceF32;
+            const bool with_bias = EPI != kEpiSlope && prm.bias && q.ks0 == 0;      // the part that starts the tile's K range brings the bias in
+            const bool f32_part = (EPI == kEpiBias || EPI == kEpiSlope) && q.partial && prm.split >= kPartReduceF32;      // (the other forms are never cut)
             mbar_wait(&acc_full[buf], (n >> 1) & 1, ab, 30);
             tc_fence_after_sync();
             GemmPart ahead;
@@ -405,6 +405,15 @@ gemm_bf16_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ 
                     if (lane == 0) mbar_arrive_cluster_relaxed(free_bar[buf]);
                 }
                 if (f32_part) {
+                    if (with_bias) {                             // (converted ahead of the shuffles: a choice of type around each cost 2 us of 128 x 8192 x 256's 14.4)
+                        float b0, b1;
+                        unpack_f32x2(bias_pair(prm, bias), b0, b1);
+#pragma unroll
+                        for (int half = 0; half < 2; ++half)
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                r[half][j] = __float_as_uint(__uint_as_float(r[half][j]) + __shfl_sync(0xffffffffu, j & 1 ? b1 : b0, 16 * half + j / 2));
+                    }
                     if (inside) {
 #pragma unroll
                         for (int half = 0; half < 2; ++half) {
@@ -432,7 +441,7 @@ gemm_bf16_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ 
                         const uint32_t* x = &r[i >> 1][4 * j + 2 * (i & 1)];
                         v[i][j] = pack_f32x2(__uint_as_float(x[0]), __uint_as_float(x[1]));
                     }
-                if (with_bias) {
+                if (with_bias && !f32_part) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const uint32_t lo = __shfl_sync(0xffffffffu, bias.x, 4 * j + (lane & 3));
