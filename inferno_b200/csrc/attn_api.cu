@@ -4,6 +4,7 @@
 
 #include <cuda.h>
 #include <cuda_runtime.h>
+#include <limits.h>
 #include <math.h>
 
 #include <algorithm>
@@ -466,14 +467,17 @@ struct GemmDesc {
     const void *a, *b;
     void* c;
     int M, N, K, a_mn, b_mn;
-    int tiles() const { return ((M + GemmTraits::BM - 1) / GemmTraits::BM) * ((N + GemmTraits::BN - 1) / GemmTraits::BN); }
-    int k_slices() const { return (K + GemmTraits::BK - 1) / GemmTraits::BK; }
+    long tiles() const { return ((M + GemmTraits::BM - 1L) / GemmTraits::BM) * ((N + GemmTraits::BN - 1L) / GemmTraits::BN); }
+    int k_slices() const { return static_cast<int>((K + GemmTraits::BK - 1L) / GemmTraits::BK); }
 };
+// Sizes of which a tile's last row and column still have a number of their own.
+constexpr int kMaxGemmSize = INT_MAX - GemmTraits::BM;
+bool gemm_sizes_ok(int M, int K, int N) { return M <= kMaxGemmSize && K <= kMaxGemmSize && N <= kMaxGemmSize; }
 
 bool gemm_set_task(GemmParams& p, GemmMaps& m, int i, const GemmDesc& d) {
     using TR = GemmTraits;
     const int band = kBandRows * ((d.N + TR::BN - 1) / TR::BN);
-    p.t[i] = GemmTask{d.M, d.N, (d.M + TR::BM - 1) / TR::BM, d.tiles(), d.k_slices(), d.a_mn, d.b_mn, band, 1.f / static_cast<float>(band)};
+    p.t[i] = GemmTask{d.M, d.N, (d.M + TR::BM - 1) / TR::BM, static_cast<int>(d.tiles()), d.k_slices(), d.a_mn, d.b_mn, band, 1.f / static_cast<float>(band)};
     // A: [M, K] (box 128 rows) or stored [K, M] (box 64 k-rows); B: stored [K, N] (box 64 k-rows) or [N, K] (box 128 rows)
     return (d.a_mn ? make_tmap_2d(&m.a[i], d.a, d.K, d.M, TR::BK) : make_tmap_2d(&m.a[i], d.a, d.M, d.K, TR::CM)) &&
            (d.b_mn ? make_tmap_2d(&m.b[i], d.b, d.K, d.N, TR::BK) : make_tmap_2d(&m.b[i], d.b, d.N, d.K, TR::CN)) &&
@@ -504,7 +508,7 @@ int launch_gemm_form(int pairs, const GemmMaps& maps, const GemmParams& p, cudaS
 // 17 x 1024 x 4096 (8) 12.2 and 10.9, 512 x 2048 x 512 (24) 17.0 and 13.0, 1023 x 4096 x 1024 (48) 27.0 and 19.1, 64 x 4096 x 1024 (56) 25.7 and 12.2.
 constexpr int kMinSavedSlices = 12;
 int gemm_slabs(const GemmDesc& d, int pairs, int least = kMinSavedSlices) {
-    const int parts = std::min(std::min(8, pairs / d.tiles()), d.k_slices() / kMinPartSlices);
+    const int parts = std::min(static_cast<int>(std::min(8L, pairs / d.tiles())), d.k_slices() / kMinPartSlices);
     return parts > 1 && d.k_slices() - (d.k_slices() + parts - 1) / parts > least ? parts : 1;
 }
 
@@ -577,7 +581,8 @@ int launch_gemms(const GemmDesc* whole, const GemmDesc* other, int split, float*
 int gemm_check(const GemmDesc& d) {
     if (!d.a || !d.b || !d.c) return IB200_ERR_INVALID_ARGUMENT;
     if (d.M <= 0 || d.N <= 0 || d.K <= 0 || (d.a_mn != 0 && d.a_mn != 1) || (d.b_mn != 0 && d.b_mn != 1)) return IB200_ERR_INVALID_ARGUMENT;
-    // a row of each matrix, as it is stored, is a whole number of 16-byte units
+    // a row of each matrix, as it is stored, is a whole number of 16-byte units; (half of) an int counts the tiles
+    if (!gemm_sizes_ok(d.M, d.K, d.N) || d.tiles() > INT_MAX / 2) return IB200_ERR_UNSUPPORTED;
     if ((d.a_mn ? d.M : d.K) % 8 || (d.b_mn ? d.N : d.K) % 8 || d.N % 8) return IB200_ERR_UNSUPPORTED;
     if (!aligned16(d.a) || !aligned16(d.b) || !aligned16(d.c)) return IB200_ERR_MISALIGNED;
     return device_ok();
@@ -626,6 +631,7 @@ int gemm_single(const GemmDesc& d, const void* bias, int bias_bf16, void* ws, si
 }
 
 bool valid_dtype(int dtype) { return dtype == IB200_DTYPE_F32 || dtype == IB200_DTYPE_BF16; }
+bool whole_elements(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % (dtype == IB200_DTYPE_F32 ? 4 : 2) == 0; }
 
 // Up to 32 rows.  Up to four blocks of a cluster split K until every SM has a block, as long as every warp keeps two boxes of 64 rows.  us for split 1,
 // 2, 4, 8 where it has the choice: 1 x 8192 x 2048 14.1, 10.7, 9.9, 9.9; 1 x 4096 x 1024 8.2, 6.6, 5.4, 7.5 (one box a warp); 32 x 4096 x 1024
@@ -749,7 +755,7 @@ int linear_bwd_core(const void* x, const void* w, const void* dy, void* dx, void
     if (dx && (rc = gemm_check(gx))) return rc;
     if (dw && (rc = gemm_check(gw))) return rc;
     if (db && (M <= 0 || N <= 0)) return IB200_ERR_INVALID_ARGUMENT;
-    if (db && N % 8) return IB200_ERR_UNSUPPORTED;
+    if (db && (N % 8 || !gemm_sizes_ok(M, K, N))) return IB200_ERR_UNSUPPORTED;
     if (!aligned16(dy)) return IB200_ERR_MISALIGNED;
     const bool have_ws = ws && aligned16(ws) && ws_bytes >= linear_bwd_ws_bytes(K, N);
     if (db && db_bf16 && !have_ws) return IB200_ERR_WORKSPACE;
@@ -916,10 +922,9 @@ int launch_ln_any(int dtype, bool backward, const LnRows& p, int blocks, cudaStr
 
 int ln_check(const void* x, long x_pitch, int M, int C, int dtype, int param_dtype) {
     if (!x || M <= 0 || C <= 0 || x_pitch < 0) return IB200_ERR_INVALID_ARGUMENT;
-    if ((dtype != IB200_DTYPE_F32 && dtype != IB200_DTYPE_BF16) || (param_dtype != IB200_DTYPE_F32 && param_dtype != IB200_DTYPE_BF16)) return IB200_ERR_INVALID_ARGUMENT;
+    if (!valid_dtype(dtype) || !valid_dtype(param_dtype)) return IB200_ERR_INVALID_ARGUMENT;
     return ln_threads_per_row(C, dtype) ? IB200_OK : IB200_ERR_UNSUPPORTED;
 }
-bool ln_whole_elements(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % (dtype == IB200_DTYPE_F32 ? 4 : 2) == 0; }
 
 int fwd_core(const void* q, const void* k, const void* v, void* o, float* lse, const ib200_layout* lq_, const ib200_layout* lk_,
              const ib200_layout* lv_, const ib200_layout* lo_, int B, int H, int T, int D, float scale, int causal, int dtype,
@@ -1217,7 +1222,8 @@ int ib200_fused_linear_bwd(const void* x, const void* w, const void* dy, const v
                            int N, void* workspace, size_t workspace_bytes, ib200_stream_t stream) {
     if (!valid_dtype(db_dtype) || (activation != IB200_ACT_NONE && activation != IB200_ACT_GELU)) return IB200_ERR_INVALID_ARGUMENT;
     if ((activation == IB200_ACT_GELU) != (slope != nullptr) || M <= 0 || K <= 0 || N <= 0) return IB200_ERR_INVALID_ARGUMENT;
-    if (!aligned16(slope)) return IB200_ERR_MISALIGNED;
+    if (!gemm_sizes_ok(M, K, N)) return IB200_ERR_UNSUPPORTED;
+    if (!aligned16(slope) || !whole_elements(db, db_dtype)) return IB200_ERR_MISALIGNED;
     if (!workspace || !aligned16(workspace) || workspace_bytes < ib200_fused_linear_workspace_bytes(M, K, N, activation, IB200_PASS_BWD)) return IB200_ERR_WORKSPACE;
     if (!dx && !dw && !db) return IB200_OK;
     if (N % 8) return IB200_ERR_UNSUPPORTED;
@@ -1236,7 +1242,8 @@ size_t ib200_feed_forward_workspace_bytes(int M, int C, int H) {
 int ib200_feed_forward_bwd(const void* x, const void* w1, const void* slope, const void* h, const void* w2, const void* dy, void* dx, void* dw1, void* db1,
                            int db1_dtype, void* dw2, void* db2, int db2_dtype, int M, int C, int H, void* workspace, size_t workspace_bytes, ib200_stream_t stream) {
     if (!x || !w1 || !slope || !h || !w2 || !dy || M <= 0 || C <= 0 || H <= 0 || !valid_dtype(db1_dtype) || !valid_dtype(db2_dtype)) return IB200_ERR_INVALID_ARGUMENT;
-    if (C % 8 || H % 8) return IB200_ERR_UNSUPPORTED;
+    if (C % 8 || H % 8 || !gemm_sizes_ok(M, C, H)) return IB200_ERR_UNSUPPORTED;
+    if (!whole_elements(db1, db1_dtype) || !whole_elements(db2, db2_dtype)) return IB200_ERR_MISALIGNED;
     if (!workspace || !aligned16(workspace) || workspace_bytes < ib200_feed_forward_workspace_bytes(M, C, H)) return IB200_ERR_WORKSPACE;
     if (!dx && !dw1 && !db1 && !dw2 && !db2) return IB200_OK;
     return ff_bwd_core(x, w1, slope, h, w2, dy, dx, dw1, db1, db1_dtype == IB200_DTYPE_BF16, dw2, db2, db2_dtype == IB200_DTYPE_BF16, M, C, H,
@@ -1254,8 +1261,8 @@ int ib200_layer_norm_fwd(const void* x, int64_t x_pitch, const void* weight, con
     int rc = ln_check(x, x_pitch, M, C, dtype, param_dtype);
     if (rc != IB200_OK) return rc;
     if (!y || !mean != !rstd || !(eps >= 0.f) || !isfinite(eps)) return IB200_ERR_INVALID_ARGUMENT;
-    if (!ln_whole_elements(x, dtype) || !ln_whole_elements(y, dtype) || !ln_whole_elements(weight, param_dtype) || !ln_whole_elements(bias, param_dtype) ||
-        !ln_whole_elements(mean, IB200_DTYPE_F32) || !ln_whole_elements(rstd, IB200_DTYPE_F32))
+    if (!whole_elements(x, dtype) || !whole_elements(y, dtype) || !whole_elements(weight, param_dtype) || !whole_elements(bias, param_dtype) ||
+        !whole_elements(mean, IB200_DTYPE_F32) || !whole_elements(rstd, IB200_DTYPE_F32))
         return IB200_ERR_MISALIGNED;
     if ((rc = device_ok()) != IB200_OK) return rc;
     const LnRows p{x, static_cast<long>(x_pitch), nullptr, 0, weight, bias, param_dtype == IB200_DTYPE_BF16, y, mean, rstd, nullptr, M, C, eps};
@@ -1269,9 +1276,9 @@ int ib200_layer_norm_bwd(const void* x, int64_t x_pitch, const void* weight, con
     if (rc != IB200_OK) return rc;
     if (!dy || dy_pitch < 0 || !mean || !rstd) return IB200_ERR_INVALID_ARGUMENT;
     if (!dx && !dw && !db) return IB200_OK;
-    if (!ln_whole_elements(x, dtype) || !ln_whole_elements(dy, dtype) || !ln_whole_elements(dx, dtype) || !ln_whole_elements(weight, param_dtype) ||
-        !ln_whole_elements(dw, param_dtype) || !ln_whole_elements(db, param_dtype) || !ln_whole_elements(mean, IB200_DTYPE_F32) ||
-        !ln_whole_elements(rstd, IB200_DTYPE_F32))
+    if (!whole_elements(x, dtype) || !whole_elements(dy, dtype) || !whole_elements(dx, dtype) || !whole_elements(weight, param_dtype) ||
+        !whole_elements(dw, param_dtype) || !whole_elements(db, param_dtype) || !whole_elements(mean, IB200_DTYPE_F32) ||
+        !whole_elements(rstd, IB200_DTYPE_F32))
         return IB200_ERR_MISALIGNED;
     const bool params = dw || db;
     if (params && (!workspace || !aligned16(workspace) || workspace_bytes < ib200_layer_norm_workspace_bytes(M, C, dtype))) return IB200_ERR_WORKSPACE;

@@ -583,15 +583,16 @@ Tensor dense16(const Tensor& t) {
     const Tensor d = t.contiguous();
     return reinterpret_cast<uintptr_t>(d.data_ptr()) & 15u ? d.clone() : d;
 }
+// (the sizes that the kernels number, ib200_fused_linear_fwd)
 int rows_of(const Tensor& x, int64_t K) {
     const int64_t M = x.numel() / K;
-    TORCH_CHECK_VALUE(M <= 0x7fffffff, "linear: too many rows, x is ", x.sizes());
+    TORCH_CHECK_VALUE(M <= 0x7fffff00 - 1, "linear: too many rows, x is ", x.sizes());
     return static_cast<int>(M);
 }
 // A projection's weight and bias, the shapes ahead of devices and types; `like`: a tensor on the device they must be on.
 void check_weight_shapes(const Tensor& w, const Tensor& bias) {
     const int64_t K = w.size(0), N = w.size(1);
-    TORCH_CHECK_VALUE(K > 0 && N > 0 && K <= 0x7fffffff && N <= 0x7fffffff, "linear: w must have rows and columns, w is ", w.sizes());
+    TORCH_CHECK_VALUE(K > 0 && N > 0 && K <= 0x7fffff00 - 1 && N <= 0x7fffff00 - 1, "linear: w must have rows and columns, up to 2^31 - 257 of each, w is ", w.sizes());
     TORCH_CHECK_VALUE(!bias.defined() || (bias.dim() == 1 && bias.size(0) == N), "linear: the bias must be [", N, "]");
 }
 void check_weight_types(const Tensor& w, const Tensor& bias, const Tensor& like) {

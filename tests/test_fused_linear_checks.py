@@ -35,6 +35,11 @@ def test_shapes(built_lib, device):
             L.feed_forward(x, w, b, bad, None)
     with pytest.raises(ValueError, match="residual"):
         L.feed_forward(x, w, b, z(64, 32, device=device), None, z(16, 64, device=device))
+    for M in (2**31 - 256, 2**31, 2**33):                                      # one row, over and over: nothing is allocated for them
+        rows = z(1, 32, device=device).expand(M, 32)
+        for call in (lambda: L.fused_linear(rows, w, b, "gelu"), lambda: L.feed_forward(rows, w, b, z(64, 32, device=device), None)):
+            with pytest.raises(ValueError, match="too many rows"):
+                call()
     with pytest.raises(ValueError, match="rows and columns"):
         L.fused_linear(z(4, 0, device=device), z(0, 8, device=device))
     for name in ("relu", "GELU", "", 3, True):
@@ -105,3 +110,26 @@ def test_c_abi_validation(built_lib):
     assert ff(Cc=36, n=1 << 24) == _capi.ERR_UNSUPPORTED and ff(n=need - 1) == _capi.ERR_WORKSPACE and ff(ws=None) == _capi.ERR_WORKSPACE
     if not torch.cuda.is_available():
         assert fwd() in (_capi.ERR_NO_DEVICE, _capi.ERR_CUDA) and bwd() in (_capi.ERR_NO_DEVICE, _capi.ERR_CUDA) and ff() == _capi.ERR_NO_DEVICE
+
+
+def test_c_abi_sizes_at_the_end_of_an_int(built_lib):
+    """Fake addresses again: sizes whose tiles or rows an int cannot number are refused, and no size makes a workspace's formula divide by zero."""
+    C = _capi.lib()
+    big, un = 2**31 - 1, _capi.ERR_UNSUPPORTED
+    fwd = lambda M, K, N: C.ib200_fused_linear_fwd(0x100000, 0x200000, None, 0, None, 1, 0x300000, None, M, K, N, None, 0, None)
+    bwd = lambda M, K, N, db=0x700000: C.ib200_fused_linear_bwd(0x100000, 0x200000, 0x300000, 0x400000, 1, 0x500000, 0x600000, db, 0, M, K, N, 0x800000, 2**63, None)
+    ff = lambda M, Cc, H, d1=0xA00000: C.ib200_feed_forward_bwd(0x100000, 0x200000, 0x300000, 0x400000, 0x500000, 0x600000, 0x700000, 0x800000, d1, 0, 0x900000, 0xB00000, 0, M, Cc,
+                                                               H, 0xC00000, 2**63, None)
+    for M, K, N in ((big, 64, 64), (64, big - 7, 64), (64, 64, big - 7), (2**31 - 256, 64, 64), (2**30, 64, 2**30)):
+        assert fwd(M, K, N) == un, (M, K, N)
+    for M, K, N in ((big, 64, 64), (64, big - 7, 64), (64, 64, big - 7), (2**31 - 256, 64, 64)):
+        assert bwd(M, K, N) == un and ff(M, K, N) == un, (M, K, N)
+    assert fwd(33, 2**31 - 260, 64) == un                                         # not a multiple of 8
+    for M in (1, 33, 2**24, big):
+        for K in (8, 2**24, big):
+            for N in (8, 2**24, big):
+                for act in (0, 1):
+                    C.ib200_fused_linear_workspace_bytes(M, K, N, act, _capi.PASS_FWD)
+                    assert C.ib200_fused_linear_workspace_bytes(M, K, N, act, _capi.PASS_BWD) > 0
+                assert C.ib200_feed_forward_workspace_bytes(M, K, N) > 0
+    assert bwd(16, 32, 64, db=0x700002) == _capi.ERR_MISALIGNED and ff(16, 32, 64, d1=0xA00001) == _capi.ERR_MISALIGNED
