@@ -575,6 +575,24 @@ Tensor linear(const Tensor& x, const Tensor& w, const Tensor& bias) {
     return y;
 }
 
+// The gradients of the operators below are not differentiable themselves.  Made with create_graph they get this node, so that a second derivative
+// raises; without one it would come out short by their part of it.
+struct NoSecondDerivative : torch::autograd::Node {
+    const char* op;
+    explicit NoSecondDerivative(const char* op_) : op(op_) {}
+    variable_list apply(variable_list&&) override {
+        TORCH_CHECK_NOT_IMPLEMENTED(false, op, ": second derivatives are not implemented");
+    }
+    std::string name() const override { return "NoSecondDerivative"; }
+};
+void refuse_second_derivative(std::initializer_list<Tensor*> grads, const variable_list& from, const char* op) {
+    if (!at::GradMode::is_enabled() || !torch::autograd::compute_requires_grad(from)) return;
+    auto node = std::shared_ptr<NoSecondDerivative>(new NoSecondDerivative(op), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(from));
+    for (Tensor* g : grads)
+        if (g->defined()) torch::autograd::set_history(*g, node);
+}
+
 // ---- projections with an activation and a residual, and the feed-forward block of two of them ----------------------------
 void* ptr_or_null(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 // What the kernels address: dense, on 16 bytes.
@@ -702,8 +720,9 @@ struct FusedLinearBackward : torch::autograd::Node {
         if (!grads[0].defined()) return out;
         const Tensor tx = x.unpack(), tw = w.unpack(), tp = act != IB200_ACT_NONE ? slope.unpack() : Tensor();
         at::AutoDispatchBelowADInplaceOrView below;
-        const LinearGrads g = fused_linear_backward(tx, tw, grads[0], tp, act, task_should_compute_output(0), task_should_compute_output(1),
-                                                    task_should_compute_output(2), bias_type == at::kBFloat16);
+        LinearGrads g = fused_linear_backward(tx, tw, grads[0], tp, act, task_should_compute_output(0), task_should_compute_output(1),
+                                              task_should_compute_output(2), bias_type == at::kBFloat16);
+        refuse_second_derivative({&g.dx, &g.dw, &g.db}, {tx, tw, grads[0]}, "fused_linear");
         out = {g.dx, g.dw, g.db, task_should_compute_output(3) ? grads[0] : Tensor()};      // the residual's gradient is dy itself
         return out;
     }
@@ -792,7 +811,8 @@ struct FeedForwardBackward : torch::autograd::Node {
         at::AutoDispatchBelowADInplaceOrView below;
         bool need[5];
         for (int i = 0; i < 5; ++i) need[i] = task_should_compute_output(i);
-        const FeedForwardGrads g = feed_forward_backward(tx, t1, tp, th, t2, grads[0], need, b1_type, b2_type);
+        FeedForwardGrads g = feed_forward_backward(tx, t1, tp, th, t2, grads[0], need, b1_type, b2_type);
+        refuse_second_derivative({&g.dx, &g.dw1, &g.db1, &g.dw2, &g.db2}, {tx, t1, t2, grads[0]}, "feed_forward");
         return {g.dx, g.dw1, g.db1, g.dw2, g.db2, task_should_compute_output(5) ? grads[0] : Tensor()};
     }
     void release_variables() override {
@@ -943,8 +963,9 @@ struct LayerNormBackward : torch::autograd::Node {
         if (!grads[0].defined()) return variable_list(3);
         const Tensor tx = x.unpack(), tw = has_weight ? weight.unpack() : Tensor(), tm = mean.unpack(), tr = rstd.unpack();
         at::AutoDispatchBelowADInplaceOrView below;
-        const NormGrads g = layer_norm_backward(tx, grads[0], tm, tr, tw, task_should_compute_output(0), task_should_compute_output(1),
-                                                task_should_compute_output(2), param_type);
+        NormGrads g = layer_norm_backward(tx, grads[0], tm, tr, tw, task_should_compute_output(0), task_should_compute_output(1),
+                                          task_should_compute_output(2), param_type);
+        refuse_second_derivative({&g.dx, &g.dw, &g.db}, has_weight ? variable_list{tx, tw, grads[0]} : variable_list{tx, grads[0]}, "layer_norm");
         return {g.dx, g.dw, g.db};
     }
     void release_variables() override {

@@ -55,7 +55,7 @@ def fused_linear_backward(x, w, dy, slope=None, activation: str | None = None, n
 def fused_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
                  residual: torch.Tensor | None = None) -> torch.Tensor:
     """``act(x @ w + bias) + residual`` in one kernel; differentiable (backward node in csrc/host_ops.cpp).  bf16 tensors, a bias of
-    either type; in_features and out_features are multiples of 8, the number of rows is free."""
+    either type; in_features and out_features are multiples of 8, the number of rows is free.  Second derivatives are refused (NotImplementedError)."""
     return _capi.host().fused_linear(x, w, bias, activation, residual)
 
 
@@ -64,7 +64,8 @@ def feed_forward(x: torch.Tensor, w1: torch.Tensor, b1: torch.Tensor | None, w2:
     """``gelu(x @ w1 + b1) @ w2 + b2 + residual``; differentiable.  w1 [C, H], w2 [H, C]; biases and residual may be None.
 
     Two kernels forward; backward the gradient of the hidden layer is multiplied by gelu' in the epilogue of the product that
-    makes it.  The hidden layer is rounded to bf16 between the products, and so is its gradient."""
+    makes it.  The hidden layer is rounded to bf16 between the products, and so is its gradient.  Second derivatives are
+    refused (NotImplementedError)."""
     return _capi.host().feed_forward(x, w1, b1, w2, b2, residual)
 
 

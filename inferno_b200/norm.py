@@ -25,7 +25,8 @@ def layer_norm_backward(x, dy, mean, rstd, weight=None, need_dx=True, need_dw=Tr
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor:
-    """Layer norm over the last axis of x; differentiable (backward node in csrc/host_ops.cpp)."""
+    """Layer norm over the last axis of x; differentiable once (backward node in csrc/host_ops.cpp), a second derivative raises
+    NotImplementedError."""
     return _capi.host().layer_norm(x, weight, bias, eps)
 
 

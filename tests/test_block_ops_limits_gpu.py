@@ -210,3 +210,25 @@ def test_one_input_in_several_places():
     db = b.detach().double().requires_grad_()
     want, = torch.autograd.grad(torch.nn.functional.layer_norm(d.detach(), (128,), db, db, 1e-5), db, dy.double())
     assert rel(g, want) <= 3 * 2 ** -8
+
+
+def test_second_derivatives_are_refused():
+    """create_graph gives the same first gradients; going through them again raises, whichever tensor is asked for, also beside a residual's own path."""
+    x, w1, b1, w2 = bf16(40, 64, seed=1), bf16(64, 128, seed=2, std=0.1), bf16(128, seed=3), bf16(128, 64, seed=4, std=0.1)
+    res, lw, lb = bf16(40, 128, seed=5), bf16(64, seed=6), bf16(64, seed=7)
+    for call, leaves in ((lambda: L.fused_linear(x, w1, b1, "gelu", res), (x, w1, b1, res)), (lambda: L.fused_linear(x, w1, None, None, res), (x, w1)),
+                         (lambda: L.feed_forward(x, w1, b1, w2, None, x), (x, w1, b1, w2)), (lambda: N.layer_norm(x, lw, lb), (x, lw, lb)), (lambda: N.layer_norm(x), (x,))):
+        for t in leaves:
+            t.requires_grad_()
+        dy = torch.ones_like(call().detach()).requires_grad_()
+        want = torch.autograd.grad(call(), leaves, dy)
+        got = torch.autograd.grad(call(), leaves, dy, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))                 # (40 rows: no sum is cut, all of them repeat)
+        for of in leaves + (dy,):
+            if of is not b1 and of is not res and of is not lb:                  # (the first gradients do not depend on what is only added)
+                with pytest.raises(NotImplementedError, match="second derivatives"):
+                    torch.autograd.grad(sum((g.float() ** 2).sum() for g in got), of, retain_graph=True)
+        for t in leaves:
+            t.requires_grad_(False)
+    y = L.fused_linear(x, w1, b1, "gelu")                                        # without any leaf, and without create_graph, nothing is in the way
+    assert not y.requires_grad and all(not g.requires_grad for g in want)
