@@ -585,10 +585,15 @@ struct NoSecondDerivative : torch::autograd::Node {
     }
     std::string name() const override { return "NoSecondDerivative"; }
 };
-void refuse_second_derivative(std::initializer_list<Tensor*> grads, const variable_list& from, const char* op) {
-    if (!at::GradMode::is_enabled() || !torch::autograd::compute_requires_grad(from)) return;
+// `from`: which of the backward node's inputs the gradients depend on, saved there or not; all of them depend on dy.
+void refuse_second_derivative(std::initializer_list<Tensor*> grads, const torch::autograd::Node& backward, std::initializer_list<uint32_t> from, const Tensor& dy,
+                              const char* op) {
+    if (!at::GradMode::is_enabled()) return;
+    torch::autograd::edge_list edges = torch::autograd::collect_next_edges(dy);
+    for (uint32_t i : from) edges.push_back(backward.next_edge(i));
+    if (std::none_of(edges.begin(), edges.end(), [](const torch::autograd::Edge& e) { return e.is_valid(); })) return;
     auto node = std::shared_ptr<NoSecondDerivative>(new NoSecondDerivative(op), torch::autograd::deleteNode);
-    node->set_next_edges(torch::autograd::collect_next_edges(from));
+    node->set_next_edges(std::move(edges));
     for (Tensor* g : grads)
         if (g->defined()) torch::autograd::set_history(*g, node);
 }
@@ -722,7 +727,9 @@ struct FusedLinearBackward : torch::autograd::Node {
         at::AutoDispatchBelowADInplaceOrView below;
         LinearGrads g = fused_linear_backward(tx, tw, grads[0], tp, act, task_should_compute_output(0), task_should_compute_output(1),
                                               task_should_compute_output(2), bias_type == at::kBFloat16);
-        refuse_second_derivative({&g.dx, &g.dw, &g.db}, {tx, tw, grads[0]}, "fused_linear");
+        // the slope of an activation was taken at x w + bias
+        if (act != IB200_ACT_NONE) refuse_second_derivative({&g.dx, &g.dw, &g.db}, *this, {0, 1, 2}, grads[0], "fused_linear");
+        else refuse_second_derivative({&g.dx, &g.dw, &g.db}, *this, {0, 1}, grads[0], "fused_linear");
         out = {g.dx, g.dw, g.db, task_should_compute_output(3) ? grads[0] : Tensor()};      // the residual's gradient is dy itself
         return out;
     }
@@ -812,7 +819,7 @@ struct FeedForwardBackward : torch::autograd::Node {
         bool need[5];
         for (int i = 0; i < 5; ++i) need[i] = task_should_compute_output(i);
         FeedForwardGrads g = feed_forward_backward(tx, t1, tp, th, t2, grads[0], need, b1_type, b2_type);
-        refuse_second_derivative({&g.dx, &g.dw1, &g.db1, &g.dw2, &g.db2}, {tx, t1, t2, grads[0]}, "feed_forward");
+        refuse_second_derivative({&g.dx, &g.dw1, &g.db1, &g.dw2, &g.db2}, *this, {0, 1, 2, 3}, grads[0], "feed_forward");      // x, w1, b1, w2
         return {g.dx, g.dw1, g.db1, g.dw2, g.db2, task_should_compute_output(5) ? grads[0] : Tensor()};
     }
     void release_variables() override {
@@ -965,7 +972,7 @@ struct LayerNormBackward : torch::autograd::Node {
         at::AutoDispatchBelowADInplaceOrView below;
         NormGrads g = layer_norm_backward(tx, grads[0], tm, tr, tw, task_should_compute_output(0), task_should_compute_output(1),
                                           task_should_compute_output(2), param_type);
-        refuse_second_derivative({&g.dx, &g.dw, &g.db}, has_weight ? variable_list{tx, tw, grads[0]} : variable_list{tx, grads[0]}, "layer_norm");
+        refuse_second_derivative({&g.dx, &g.dw, &g.db}, *this, {0, 1}, grads[0], "layer_norm");      // x, weight
         return {g.dx, g.dw, g.db};
     }
     void release_variables() override {

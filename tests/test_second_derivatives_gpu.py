@@ -1,0 +1,69 @@
+"""Gradients made with create_graph are refused a second derivative by everything that they depend on.  The slope of a GELU is taken at x w + b, so
+behind one they depend on the bias as well, also where the bias is all that needs a gradient; without one they do not."""
+import pytest
+import torch
+
+from inferno_b200 import linear as L
+
+pytestmark = pytest.mark.gpu
+
+
+def bf16(*shape, seed, std=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, device="cuda", generator=g) * std).to(torch.bfloat16)
+
+
+def problem():
+    return bf16(40, 64, seed=1), bf16(64, 128, seed=2, std=0.1), bf16(128, seed=3), bf16(128, 64, seed=4, std=0.1), bf16(64, seed=5)
+
+
+def refused(grads, of):
+    """Through the gradients and through a path of its own: the gradients' part must not be left out."""
+    with pytest.raises(NotImplementedError, match="second derivatives"):
+        torch.autograd.grad(sum((g.float() ** 2).sum() for g in grads) + (of.float() ** 2).sum(), of, retain_graph=True)
+
+
+@pytest.mark.parametrize("bias_type", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("leaves", ["b", "xb", "wb", "xwb"])
+def test_bias_ahead_of_gelu(leaves, bias_type):
+    x, w, b, _, _ = problem()
+    t = dict(x=x, w=w, b=b.to(bias_type))
+    for n in leaves:
+        t[n].requires_grad_()
+    call = lambda: L.fused_linear(t["x"], t["w"], t["b"], "gelu")
+    dy = bf16(40, 128, seed=6)
+    want = torch.autograd.grad(call(), [t[n] for n in leaves], dy)
+    got = torch.autograd.grad(call(), [t[n] for n in leaves], dy, create_graph=True)
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+    for g in got:
+        assert g.requires_grad
+        refused([g], t["b"])
+    with pytest.raises(NotImplementedError, match="second derivatives"):
+        (sum((g.float() ** 2).sum() for g in got) + (t["b"].float() ** 2).sum()).backward()
+
+
+@pytest.mark.parametrize("leaves", [("b1",), ("x", "b1"), ("w1", "b1"), ("b1", "w2"), ("b1", "b2"), ("x", "w1", "b1", "w2", "b2")])
+def test_first_bias_of_the_feed_forward_block(leaves):
+    t = dict(zip(("x", "w1", "b1", "w2", "b2"), problem()))
+    for n in leaves:
+        t[n].requires_grad_()
+    call = lambda: L.feed_forward(t["x"], t["w1"], t["b1"], t["w2"], t["b2"], t["x"])
+    dy = bf16(40, 64, seed=7)
+    want = torch.autograd.grad(call(), [t[n] for n in leaves], dy)
+    got = torch.autograd.grad(call(), [t[n] for n in leaves], dy, create_graph=True)
+    for n, g, c in zip(leaves, got, want):
+        assert torch.equal(g, c)
+        if n != "b2":                              # (db2 is the sum of dy)
+            refused([g], t["b1"])
+
+
+def test_a_bias_that_is_only_added_is_free():
+    """Nothing depends on it, and a second path through it gives what it should."""
+    x, w, b, _, _ = problem()
+    for t in (x, w, b):
+        t.requires_grad_()
+    gx, gw = torch.autograd.grad(L.fused_linear(x, w, b, None, x.new_zeros(40, 128)), (x, w), bf16(40, 128, seed=6), create_graph=True)
+    g, = torch.autograd.grad((gx.float() ** 2).sum() + (gw.float() ** 2).sum() + (b.float() ** 2).sum(), b, retain_graph=True)
+    assert torch.equal(g, 2 * b.detach())
+    refused([gx], w)
+    refused([gw], x)
