@@ -531,6 +531,29 @@ LinearGrads linear_backward(const Tensor& x, const Tensor& w, const Tensor& dy, 
     return g;
 }
 
+// The gradients of the operators below are not differentiable themselves.  Made with create_graph they get this node, so that a second derivative
+// raises; without one it would come out short by their part of it.
+struct NoSecondDerivative : torch::autograd::Node {
+    const char* op;
+    explicit NoSecondDerivative(const char* op_) : op(op_) {}
+    variable_list apply(variable_list&&) override {
+        TORCH_CHECK_NOT_IMPLEMENTED(false, op, ": second derivatives are not implemented");
+    }
+    std::string name() const override { return "NoSecondDerivative"; }
+};
+// `from`: which of the backward node's inputs the gradients depend on, saved there or not; all of them depend on dy.
+void refuse_second_derivative(std::initializer_list<Tensor*> grads, const torch::autograd::Node& backward, std::initializer_list<uint32_t> from, const Tensor& dy,
+                              const char* op) {
+    if (!at::GradMode::is_enabled()) return;
+    torch::autograd::edge_list edges = torch::autograd::collect_next_edges(dy);
+    for (uint32_t i : from) edges.push_back(backward.next_edge(i));
+    if (std::none_of(edges.begin(), edges.end(), [](const torch::autograd::Edge& e) { return e.is_valid(); })) return;
+    auto node = std::shared_ptr<NoSecondDerivative>(new NoSecondDerivative(op), torch::autograd::deleteNode);
+    node->set_next_edges(std::move(edges));
+    for (Tensor* g : grads)
+        if (g->defined()) torch::autograd::set_history(*g, node);
+}
+
 struct LinearBackward : torch::autograd::Node {
     SavedVariable x, w;
     bool has_bias = false;
@@ -546,9 +569,9 @@ struct LinearBackward : torch::autograd::Node {
         at::AutoDispatchBelowADInplaceOrView below;
         LinearGrads g = linear_backward(tx, tw, grads[0], task_should_compute_output(0), task_should_compute_output(1),
                                         has_bias && task_should_compute_output(2), bias_type == at::kBFloat16);
-        out[0] = g.dx;
-        out[1] = g.dw;
-        if (g.db.defined()) out[2] = g.db.to(bias_type);      // fp32 and bf16 come in the right type
+        if (g.db.defined()) g.db = g.db.to(bias_type);      // fp32 and bf16 come in the right type
+        refuse_second_derivative({&g.dx, &g.dw, &g.db}, *this, {0, 1}, grads[0], "linear");
+        out = {g.dx, g.dw, g.db};
         return out;
     }
     void release_variables() override { x.reset_data(); w.reset_data(); }
@@ -573,29 +596,6 @@ Tensor linear(const Tensor& x, const Tensor& w, const Tensor& bias) {
         torch::autograd::set_history(y, node);
     }
     return y;
-}
-
-// The gradients of the operators below are not differentiable themselves.  Made with create_graph they get this node, so that a second derivative
-// raises; without one it would come out short by their part of it.
-struct NoSecondDerivative : torch::autograd::Node {
-    const char* op;
-    explicit NoSecondDerivative(const char* op_) : op(op_) {}
-    variable_list apply(variable_list&&) override {
-        TORCH_CHECK_NOT_IMPLEMENTED(false, op, ": second derivatives are not implemented");
-    }
-    std::string name() const override { return "NoSecondDerivative"; }
-};
-// `from`: which of the backward node's inputs the gradients depend on, saved there or not; all of them depend on dy.
-void refuse_second_derivative(std::initializer_list<Tensor*> grads, const torch::autograd::Node& backward, std::initializer_list<uint32_t> from, const Tensor& dy,
-                              const char* op) {
-    if (!at::GradMode::is_enabled()) return;
-    torch::autograd::edge_list edges = torch::autograd::collect_next_edges(dy);
-    for (uint32_t i : from) edges.push_back(backward.next_edge(i));
-    if (std::none_of(edges.begin(), edges.end(), [](const torch::autograd::Edge& e) { return e.is_valid(); })) return;
-    auto node = std::shared_ptr<NoSecondDerivative>(new NoSecondDerivative(op), torch::autograd::deleteNode);
-    node->set_next_edges(std::move(edges));
-    for (Tensor* g : grads)
-        if (g->defined()) torch::autograd::set_history(*g, node);
 }
 
 // ---- projections with an activation and a residual, and the feed-forward block of two of them ----------------------------

@@ -30,7 +30,8 @@ def linear_backward(x, w, dy, need_dx=True, need_dw=True, need_db=True):
 
 
 class LinearFunction:
-    """The differentiable projection (backward node in csrc/host_ops.cpp), under the name it had as an autograd function."""
+    """The differentiable projection (backward node in csrc/host_ops.cpp), under the name it had as an autograd function.  Second
+    derivatives are refused (NotImplementedError)."""
 
     @staticmethod
     def apply(x, w, bias):

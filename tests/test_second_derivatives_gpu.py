@@ -67,3 +67,32 @@ def test_a_bias_that_is_only_added_is_free():
     assert torch.equal(g, 2 * b.detach())
     refused([gx], w)
     refused([gw], x)
+
+
+@pytest.mark.parametrize("form", ["function", "module"])
+def test_plain_projection(form):
+    """A projection without activation and residual refuses what one with them refuses."""
+    x, w, b, _, _ = problem()
+    if form == "module":
+        lin = L.Linear(64, 128).cuda().to(torch.bfloat16)
+        w, b, call = lin.weight, lin.bias, lambda: lin(x)
+    else:
+        call = lambda: L.LinearFunction.apply(x, w, b)
+    leaves = (x, w, b)
+    for t in leaves:
+        t.requires_grad_()
+    dy = bf16(40, 128, seed=6).requires_grad_()
+    want = torch.autograd.grad(call(), leaves, dy)
+    assert all(not g.requires_grad for g in want)
+    got = torch.autograd.grad(call(), leaves, dy, create_graph=True)
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+    refused([got[0]], w)
+    refused([got[1]], x)
+    for g in got:
+        refused([g], dy)
+    g, = torch.autograd.grad(sum((t.float() ** 2).sum() for t in got[:2]) + (b.float() ** 2).sum(), b, retain_graph=True)      # only added: nothing depends on it
+    assert torch.equal(g, 2 * b.detach())
+    y = call()                                     # a gradient penalty beside the loss itself
+    gx, = torch.autograd.grad(y, x, dy, create_graph=True)
+    with pytest.raises(NotImplementedError, match="second derivatives"):
+        (y.float().sum() + (gx.float() ** 2).sum()).backward()
