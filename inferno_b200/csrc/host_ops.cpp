@@ -463,9 +463,23 @@ void check_bf16_cuda(const Tensor& t, const char* name) {
     TORCH_CHECK_TYPE(t.scalar_type() == at::kBFloat16, "linear: ", name, " must be bfloat16");
 }
 
+// The sizes that the kernels number (ib200_fused_linear_fwd).
+constexpr int64_t kMaxLinearSize = 0x7fffff00 - 1;
+int rows_of(const Tensor& x, int64_t K) {
+    const int64_t M = x.numel() / K;
+    TORCH_CHECK_VALUE(M <= kMaxLinearSize, "linear: too many rows, x is ", x.sizes());
+    return static_cast<int>(M);
+}
+void check_weight_size(const Tensor& w) {
+    const int64_t K = w.size(0), N = w.size(1);
+    TORCH_CHECK_VALUE(K > 0 && N > 0 && K <= kMaxLinearSize && N <= kMaxLinearSize, "linear: w must have rows and columns, up to 2^31 - 257 of each, w is ", w.sizes());
+}
+
 Tensor linear_forward(const Tensor& x, const Tensor& w, const Tensor& bias) {
     check_linear_shapes(x, w);
+    check_weight_size(w);
     const int64_t K = w.size(0), N = w.size(1);
+    const int M = rows_of(x, K);
     TORCH_CHECK_VALUE(!bias.defined() || bias.numel() == N, "linear: the bias must have ", N, " elements");
     check_bf16_cuda(x, "x");
     check_bf16_cuda(w, "w");
@@ -481,7 +495,6 @@ Tensor linear_forward(const Tensor& x, const Tensor& w, const Tensor& bias) {
     auto shape = x.sizes().vec();
     shape.back() = N;
     Tensor y = at::empty(shape, x.options());
-    const int M = static_cast<int>(x2.size(0));
     const size_t bytes = g_abi.linear_workspace_bytes(M, static_cast<int>(K), static_cast<int>(N), IB200_PASS_FWD);
     cudaStream_t stream = c10::cuda::getCurrentCUDAStream(x.device().index()).stream();
     std::unique_lock<std::mutex> lock;
@@ -503,8 +516,10 @@ struct LinearGrads {
 };
 LinearGrads linear_backward(const Tensor& x, const Tensor& w, const Tensor& dy, bool need_dx, bool need_dw, bool need_db, bool db_bf16) {
     check_linear_shapes(x, w);
+    check_weight_size(w);
     const int64_t K = w.size(0), N = w.size(1);
-    TORCH_CHECK_VALUE(dy.dim() >= 1 && dy.size(-1) == N && dy.numel() / std::max<int64_t>(N, 1) == x.numel() / std::max<int64_t>(K, 1),
+    const int M = rows_of(x, K);
+    TORCH_CHECK_VALUE(dy.dim() >= 1 && dy.size(-1) == N && dy.numel() / N == M,
                       "linear: dy must have the rows of x and ", N, " columns, dy is ", dy.sizes(), ", x is ", x.sizes());
     check_bf16_cuda(x, "x");
     check_bf16_cuda(w, "w");
@@ -513,7 +528,6 @@ LinearGrads linear_backward(const Tensor& x, const Tensor& w, const Tensor& dy, 
     check_same_device(dy, x, "dy");
     const c10::cuda::CUDAGuard guard(x.device());
     const Tensor x2 = x.reshape({-1, K}).contiguous(), dy2 = dy.reshape({-1, N}).contiguous(), wc = w.contiguous();
-    const int M = static_cast<int>(x2.size(0));
     LinearGrads g;
     if (need_dx) g.dx = at::empty(x.sizes(), x.options());
     if (need_dw) g.dw = at::empty({K, N}, x.options());
@@ -606,16 +620,10 @@ Tensor dense16(const Tensor& t) {
     const Tensor d = t.contiguous();
     return reinterpret_cast<uintptr_t>(d.data_ptr()) & 15u ? d.clone() : d;
 }
-// (the sizes that the kernels number, ib200_fused_linear_fwd)
-int rows_of(const Tensor& x, int64_t K) {
-    const int64_t M = x.numel() / K;
-    TORCH_CHECK_VALUE(M <= 0x7fffff00 - 1, "linear: too many rows, x is ", x.sizes());
-    return static_cast<int>(M);
-}
 // A projection's weight and bias, the shapes ahead of devices and types; `like`: a tensor on the device they must be on.
 void check_weight_shapes(const Tensor& w, const Tensor& bias) {
-    const int64_t K = w.size(0), N = w.size(1);
-    TORCH_CHECK_VALUE(K > 0 && N > 0 && K <= 0x7fffff00 - 1 && N <= 0x7fffff00 - 1, "linear: w must have rows and columns, up to 2^31 - 257 of each, w is ", w.sizes());
+    check_weight_size(w);
+    const int64_t N = w.size(1);
     TORCH_CHECK_VALUE(!bias.defined() || (bias.dim() == 1 && bias.size(0) == N), "linear: the bias must be [", N, "]");
 }
 void check_weight_types(const Tensor& w, const Tensor& bias, const Tensor& like) {
