@@ -495,6 +495,7 @@ Tensor linear_forward(const Tensor& x, const Tensor& w, const Tensor& bias) {
     auto shape = x.sizes().vec();
     shape.back() = N;
     Tensor y = at::empty(shape, x.options());
+    if (M == 0) return y;
     const size_t bytes = g_abi.linear_workspace_bytes(M, static_cast<int>(K), static_cast<int>(N), IB200_PASS_FWD);
     cudaStream_t stream = c10::cuda::getCurrentCUDAStream(x.device().index()).stream();
     std::unique_lock<std::mutex> lock;
@@ -529,9 +530,11 @@ LinearGrads linear_backward(const Tensor& x, const Tensor& w, const Tensor& dy, 
     const c10::cuda::CUDAGuard guard(x.device());
     const Tensor x2 = x.reshape({-1, K}).contiguous(), dy2 = dy.reshape({-1, N}).contiguous(), wc = w.contiguous();
     LinearGrads g;
+    const auto db_type = x.options().dtype(db_bf16 ? at::kBFloat16 : at::kFloat);
     if (need_dx) g.dx = at::empty(x.sizes(), x.options());
-    if (need_dw) g.dw = at::empty({K, N}, x.options());
-    if (need_db) g.db = at::empty({N}, x.options().dtype(db_bf16 ? at::kBFloat16 : at::kFloat));
+    if (need_dw) g.dw = M ? at::empty({K, N}, x.options()) : at::zeros({K, N}, x.options());
+    if (need_db) g.db = M ? at::empty({N}, db_type) : at::zeros({N}, db_type);
+    if (M == 0) return g;
     const size_t bytes = g_abi.linear_workspace_bytes(M, static_cast<int>(K), static_cast<int>(N), IB200_PASS_BWD);
     cudaStream_t stream = c10::cuda::getCurrentCUDAStream(x.device().index()).stream();
     Workspace& ws = workspace_of(x.device().index(), stream);

@@ -29,3 +29,34 @@ def test_weights_that_are_empty_or_too_wide(built_lib, device):
         for call in (lambda: L.linear_forward(x, w), lambda: L.LinearFunction.apply(x, w, None), lambda: L.linear_backward(x, w, dy)):
             with pytest.raises(ValueError, match="rows and columns"):
                 call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(0, 64), (3, 0, 64), (0, 5, 64)])
+@pytest.mark.parametrize("bias_type", [torch.bfloat16, torch.float32, None])
+def test_no_rows(shape, bias_type):
+    """An empty output, an empty dx, and gradients of zero, as with an activation or a residual."""
+    x, w = z(*shape, device="cuda").requires_grad_(), torch.ones(64, 128, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    b = None if bias_type is None else torch.ones(128, device="cuda", dtype=bias_type, requires_grad=True)
+    y = L.LinearFunction.apply(x, w, b)
+    assert y.shape == shape[:-1] + (128,) and L.linear_forward(x.detach(), w.detach(), b).shape == y.shape
+    leaves = [t for t in (x, w, b) if t is not None]
+    grads = torch.autograd.grad(y, leaves, torch.empty_like(y))
+    for t, g in zip(leaves, grads):
+        assert g.shape == t.shape and g.dtype == t.dtype and not g.any()
+    dx, dw, db = L.linear_backward(x.detach(), w.detach(), torch.empty_like(y))
+    assert dx.shape == x.shape and not dw.any() and not db.any() and db.dtype == torch.float32
+    for g, have in zip(L.linear_backward(x.detach(), w.detach(), torch.empty_like(y), False, True, False), (False, True, False)):
+        assert (g is not None) == have
+
+
+@pytest.mark.gpu
+def test_module_without_rows_in_every_form():
+    x = torch.empty(0, 64, device="cuda", dtype=torch.bfloat16)
+    for lin in (L.Linear(64, 128), L.Linear(64, 128, bias=False), L.Linear(64, 128, activation="gelu")):
+        lin = lin.cuda().to(torch.bfloat16)
+        for res in (None, torch.empty(0, 128, device="cuda", dtype=torch.bfloat16)):
+            y = lin(x, res)
+            assert y.shape == (0, 128)
+            y.sum().backward()
+            assert all(not p.grad.any() for p in lin.parameters())
