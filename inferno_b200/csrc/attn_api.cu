@@ -492,7 +492,7 @@ bool gemm_wants_split_beside(const GemmDesc& d, int pairs) { return d.tiles() <=
 
 // A fused epilogue of the `whole` product (kEpi*): what it reads beside its accumulator, and what it writes beside c.
 struct GemmEpi {
-    int mode = kEpiBias;
+    int mode = kEpiPlain;           // (launch_gemms chooses the form)
     const void* aux = nullptr;      // residual (bf16) or gelu'(z) (fp16), [M, N]
     void* keep = nullptr;           // where gelu'(z) goes, fp16 [M, N]
     float* colsum = nullptr;        // [ceil(M / 32)][N]
@@ -570,11 +570,14 @@ int launch_gemms(const GemmDesc* whole, const GemmDesc* other, int split, float*
     void* builtin = nullptr;
     p.status = static_scratch(&builtin) == IB200_OK ? static_cast<int*>(builtin) : nullptr;
     IB200_SET_BOUNDS(0, 0, 0, 0, 0, 1, TR::TM_COLS, p.status, stream);
-    switch (epi.mode) {
+    const int mode = epi.mode != kEpiPlain ? epi.mode : split == kPartSlab ? kEpiSlab : split == kPartWhole && bias ? kEpiBias : kEpiPlain;
+    switch (mode) {
+        case kEpiSlab: return launch_gemm_form<kEpiSlab>(pairs, maps, p, stream);
+        case kEpiBias: return launch_gemm_form<kEpiBias>(pairs, maps, p, stream);
         case kEpiResidual: return launch_gemm_form<kEpiResidual>(pairs, maps, p, stream);
         case kEpiGelu: return launch_gemm_form<kEpiGelu>(pairs, maps, p, stream);
         case kEpiSlope: return launch_gemm_form<kEpiSlope>(pairs, maps, p, stream);
-        default: return launch_gemm_form<kEpiBias>(pairs, maps, p, stream);
+        default: return launch_gemm_form<kEpiPlain>(pairs, maps, p, stream);
     }
 }
 
@@ -704,7 +707,7 @@ int fused_linear_fwd_core(const GemmDesc& d, const void* bias, int bias_bf16, co
         return launch_fused_finish(p, ws, slabs, d.M, d.N, d.c, stream);
     }
     GemmEpi epi;
-    epi.mode = gelu ? kEpiGelu : residual ? kEpiResidual : kEpiBias;
+    epi.mode = gelu ? kEpiGelu : residual ? kEpiResidual : kEpiPlain;
     epi.aux = residual;
     epi.keep = slope;
     return launch_gemms(&d, nullptr, kPartWhole, nullptr, bias, bias_bf16, stream, epi);

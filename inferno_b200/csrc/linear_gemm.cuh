@@ -43,14 +43,17 @@
 
 namespace ib200 {
 
-// What the epilogue of task 0 does beyond adding the bias.  Each is a kernel of its own: a run-time branch would put every form's registers and
-// code into the plain one.
+// What the epilogue of task 0 does.  Each is a kernel of its own: a run-time branch would put every form's registers and code into the others.
 enum : int {
-    kEpiBias = 0,          // c = acc + bias
+    kEpiPlain = 0,         // c = acc; of parts of a tile, added up (with the bias in the first)
     kEpiResidual = 1,      // c = acc + bias + aux
     kEpiGelu = 2,          // z = acc + bias;  c = gelu(z) (+ aux);  gelu'(z) kept as fp16 if it is wanted
     kEpiSlope = 3,         // c = acc aux with aux = gelu'(z), and the column sums of c
+    kEpiBias = 4,          // c = acc + bias, of whole tiles
+    kEpiSlab = 5,          // c = acc; a part of a tile of task 1 goes to its slab
 };
+template <int EPI>
+constexpr bool kEpiFused = EPI == kEpiResidual || EPI == kEpiGelu || EPI == kEpiSlope;
 
 struct GemmTraits {
     static constexpr int BM = 256, BN = 256, BK = 64;            // tile of a CTA pair
@@ -68,10 +71,10 @@ struct GemmTraits {
 // output), which takes the place of one of the ring's six stages.
 template <int EPI>
 struct GemmSmem {
-    static constexpr int STAGES = EPI == kEpiBias ? GemmTraits::STAGES : 5;
+    static constexpr int STAGES = kEpiFused<EPI> ? 5 : GemmTraits::STAGES;
     static constexpr int OFF_OUT = STAGES * GemmTraits::STAGE_BYTES;
     static constexpr int OFF_AUX = OFF_OUT + GemmTraits::EPI_WARPS * GemmTraits::STAGING_BYTES;
-    static constexpr int OFF_BAR = OFF_AUX + (EPI == kEpiBias ? 0 : GemmTraits::EPI_WARPS * GemmTraits::STAGING_BYTES);
+    static constexpr int OFF_BAR = OFF_AUX + (kEpiFused<EPI> ? GemmTraits::EPI_WARPS * GemmTraits::STAGING_BYTES : 0);
     static constexpr int BYTES = OFF_BAR + 256 + 1024;
     static_assert(BYTES <= 232448, "shared memory budget");
     static_assert((2 * STAGES + 4 + GemmTraits::EPI_WARPS) * 8 + 8 <= 256, "barriers");
@@ -245,7 +248,7 @@ gemm_bf16_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ 
         *abort_flag = 0;
         for (int s = 0; s < NS; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * TR::EPI_WARPS); }
-        if (EPI != kEpiBias)
+        if (kEpiFused<EPI>)
             for (int w = 0; w < TR::EPI_WARPS; ++w) mbar_init(&aux_full[w], 1);
         fence_mbar_init();
     }
@@ -339,214 +342,263 @@ gemm_bf16_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ 
         // of the tile), so no barrier ties the warps together.  Registers straight to global memory (a 32-byte sector per thread) took 6200
         // cycles a tile, at three cycles per sector, and 2800 more in the release of the accumulator, which had to wait for the stores; four
         // warps that shared staging panels under named barriers took 7300.
-        // A thread holds pairs of columns of four rows (tmem_ld_16x256b_x8), the same columns in each, so a step's bias is eight shuffles, and the
-        // arithmetic is packed.  With a row per thread each element's bias came by a shuffle, and two warps a scheduler could not hide it
-        // all: 15000 cycles a 256 x 256 tile with GELU and z, 10800 with a residual (8192 x 1024 x 4096: 69.7 and 56.8 us).
+        // The accumulator comes in one of two layouts:
+        // - a row per lane (tmem_ld_x32) where nothing is done with it, and for the parts of a product that is cut, whose fp32 goes out 16 bytes a lane
+        //   (backward of 1000 x 768 x 768, us: 15.0; pairs, stored 8 bytes at a time, 15.5; added in memory straight from the registers 16.1);
+        // - pairs of columns of four rows (tmem_ld_16x256b_x8), the same columns in each, where there is an epilogue: a step's bias is eight shuffles, and
+        //   the arithmetic is packed.  With a row per lane each element's bias came by a shuffle, and two warps a scheduler could not hide it all:
+        //   15000 cycles a 256 x 256 tile with GELU and z, 10800 with a residual (8192 x 1024 x 4096: 69.7 and 56.8 us).
+        // A kernel has one of them, but for kEpiSlope, which shares its launch with a weight gradient.  Code that a launch does not run slows down the
+        // code that it does: backward of 2048 x 512 x 512, 1000 x 768 x 768 and 2048 x 768 x 256, whose dW is cut, us: 14.0, 15.1 and 13.8 with both layouts
+        // in one kernel, 14.1, 15.0 and 13.6 with parts that are added up and slabs in one, 13.7, 14.7 and 12.9 apart.  Forward of
+        // 2048 x 512 x 512 and 16384 x 768 x 768, whole tiles with a bias: 7.7 and 18.0 in one kernel, 7.4 and 17.8 apart.
         const int h = warp >> 2, row0 = (warp & 3) * 32;
         const uint32_t lane_base = static_cast<uint32_t>(row0) << 16;
         uint8_t* stage = sOut + warp * TR::STAGING_BYTES;
         uint8_t* second = smem + SM::OFF_AUX + warp * TR::STAGING_BYTES;      // fused forms: what is read beside the accumulator, or a second output
         const uint32_t free_bar[2] = {mapa_u32(smem_u32(&acc_empty[0]), 0), mapa_u32(smem_u32(&acc_empty[1]), 0)};
-        const bool has_aux = EPI == kEpiResidual || EPI == kEpiSlope || (EPI == kEpiGelu && prm.has_aux);
-        const int colf = h * (BN / 2), pair_col = 2 * (lane & 3);
-        uint32_t aux_n = 0;
-        auto request_aux = [&](const GemmPart& p, int c0) {      // the step's 32 x 64 tile; one at a time is on its way or being read
-            const int row = p.m0 + static_cast<int>(rank) * TR::CM + row0, col = p.n0 + c0;
-            if (has_aux && p.task == 0 && row < prm.t[0].M && col < prm.t[0].N && lane == 0) {
-                mbar_arrive_expect_tx(&aux_full[warp], TR::STAGING_BYTES);
-                tma_load_3d(second, &maps.aux, &aux_full[warp], col, row, 0);
-            }
-        };
-        uint2 bias = make_uint2(0u, 0u);                         // of columns 2 lane, 2 lane + 1 of a step, handed round by shuffles
-        auto request_bias = [&](const GemmPart& p, int c0) {
-            const int col = p.n0 + c0 + 2 * lane;
-            if (EPI != kEpiSlope && prm.bias && col < prm.t[p.task].N) bias = load_bias2(prm, col);
-        };
+        const int colf = h * (BN / 2);
         auto tile_free = [&] {                                   // the last copies have read the staging tiles
             if (lane == 0) tma_store_wait_read_all();
             __syncwarp();
         };
+        auto release = [&](uint32_t buf) {                       // every column of the accumulator is in registers: hand it back to the MMA warp
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster_relaxed(free_bar[buf]);
+        };
+        // 32 rows x 128 bytes, a row per lane: to their place, or added to what is there (rows and columns past M and N are clipped by the copy)
+        auto stage_out = [&](const CUtensorMap* m, bool add, int col, int row, int z, const uint4 (&w)[8]) {
+            tile_free();
+#pragma unroll
+            for (int c = 0; c < 8; ++c) st_shared_sw128(stage, lane, c, w[c]);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                if (add) tma_reduce_add_3d(m, stage, col, row, z);
+                else tma_store_3d(m, stage, col, row, z);
+                tma_store_commit();
+            }
+        };
+        auto stage_out_f32 = [&](const uint32_t (&r)[2][32], int col, int row, int slab, int N) {
+            uint4 w[8];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) w[c] = make_uint4(r[half][4 * c], r[half][4 * c + 1], r[half][4 * c + 2], r[half][4 * c + 3]);
+                if (col + 32 * half < N) stage_out(&maps.sum, EPI != kEpiSlab, col + 32 * half, row, slab, w);
+            }
+        };
         uint32_t n = 0;
-        bool more = walk.next(q);
-        if (more) {
-            request_aux(q, colf);
-            request_bias(q, colf);
-        }
-        for (; more; ++n) {
-            const GemmTask& k = prm.t[q.task];
-            const bool fused = EPI != kEpiBias && q.task == 0;
-            const uint32_t buf = n & 1;
-            const int row = q.m0 + static_cast<int>(rank) * TR::CM + row0;
-            const bool with_bias = EPI != kEpiSlope && prm.bias && q.ks0 == 0;      // the part that starts the tile's K range brings the bias in
-            const bool f32_part = (EPI == kEpiBias || EPI == kEpiSlope) && q.partial && prm.split >= kPartReduceF32;      // (the other forms are never cut)
-            mbar_wait(&acc_full[buf], (n >> 1) & 1, ab, 30);
-            tc_fence_after_sync();
-            GemmPart ahead;
-            bool more_ahead = false;
+        if constexpr (EPI == kEpiPlain || EPI == kEpiSlab) {
+            const int slab = EPI == kEpiSlab ? pair % prm.slabs : 0;
+            for (; walk.next(q); ++n) {
+                const GemmTask& k = prm.t[q.task];
+                const uint32_t buf = n & 1;
+                const int row = q.m0 + static_cast<int>(rank) * TR::CM + row0;
+                const bool with_bias = EPI == kEpiPlain && prm.bias && q.ks0 == 0;       // the part that starts the tile's K range brings the bias in
+                const bool f32_part = q.partial && (EPI == kEpiSlab || prm.split == kPartReduceF32);
+                const CUtensorMap* mc = q.partial ? &maps.sum : &maps.c[q.task];
+                // two columns of bias per lane and 64-column step, fetched under the wait and handed round by shuffles (broadcast loads in
+                // the element loop queued behind the MMAs' operand reads for 2000 cycles and more)
+                float2 bias0 = make_float2(0.f, 0.f), bias1 = bias0;
+                if (with_bias) {
+                    const int col = q.n0 + colf + 2 * lane;
+                    if (col < k.N) unpack_f32x2(bias_pair(prm, load_bias2(prm, col)), bias0.x, bias0.y);
+                    if (col + 64 < k.N) unpack_f32x2(bias_pair(prm, load_bias2(prm, col + 64)), bias1.x, bias1.y);
+                }
+                mbar_wait(&acc_full[buf], (n >> 1) & 1, ab, 30);
+                tc_fence_after_sync();
 #pragma unroll 1
-            for (int c0 = colf; c0 < colf + BN / 2; c0 += 64) {
-                const int col = q.n0 + c0;
-                const bool inside = row < k.M && col < k.N, last = c0 != colf;
-                uint32_t r[2][32];
-                if (f32_part) {
-                    // A row per lane, for 16-byte stores of fp32.  Backward of 1000 x 768 x 768 and 16384 x 768 x 768, us: 15.0 and 41.0; pairs stored 8 bytes
-                    // at a time 15.5 and 40.9; added in memory straight from the registers 16.1 and 45.
-                    tmem_ld_x32(tmem + buf * BN + c0 + lane_base, r[0]);
-                    tmem_ld_x32(tmem + buf * BN + c0 + 32 + lane_base, r[1]);
-                } else {
-                    tmem_ld_16x256b_x8(tmem + buf * BN + c0 + lane_base, r[0]);
-                    tmem_ld_16x256b_x8(tmem + buf * BN + c0 + lane_base + (16u << 16), r[1]);
-                }
-                tmem_wait_ld();
-                if (last) {
-                    // every column of the accumulator is in registers: hand it back to the MMA warp
-                    tc_fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster_relaxed(free_bar[buf]);
-                }
-                if (f32_part) {
-                    if (with_bias) {                             // (converted ahead of the shuffles: a choice of type around each cost 2 us of 128 x 8192 x 256's 14.4)
-                        float b0, b1;
-                        unpack_f32x2(bias_pair(prm, bias), b0, b1);
+                for (int c0 = colf; c0 < colf + BN / 2; c0 += 64) {
+                    const int col = q.n0 + c0;
+                    uint32_t v[2][32];
+                    tmem_ld_x32(tmem + buf * BN + c0 + lane_base, v[0]);
+                    tmem_ld_x32(tmem + buf * BN + c0 + 32 + lane_base, v[1]);
+                    tmem_wait_ld();
+                    if (c0 != colf) release(buf);
+                    if (row >= k.M || col >= k.N) continue;
+                    if (with_bias) {
+                        const float2 bc = c0 != colf ? bias1 : bias0;
 #pragma unroll
-                        for (int half = 0; half < 2; ++half)
-#pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                r[half][j] = __float_as_uint(__uint_as_float(r[half][j]) + __shfl_sync(0xffffffffu, j & 1 ? b1 : b0, 16 * half + j / 2));
+                        for (int e = 0; e < 64; ++e) v[e / 32][e % 32] = __float_as_uint(__uint_as_float(v[e / 32][e % 32]) + __shfl_sync(0xffffffffu, e & 1 ? bc.y : bc.x, e / 2));
                     }
-                    if (inside) {
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            if (col + 32 * half >= k.N) continue;
-                            tile_free();
-#pragma unroll
-                            for (int c = 0; c < 8; ++c) st_shared_sw128(stage, lane, c, make_uint4(r[half][4 * c], r[half][4 * c + 1], r[half][4 * c + 2], r[half][4 * c + 3]));
-                            fence_proxy_async_smem();
-                            __syncwarp();
-                            if (lane == 0) {
-                                // rows / columns past M / N are clipped by the copy
-                                if (prm.split == kPartSlab) tma_store_3d(&maps.sum, stage, col + 32 * half, row, pair % prm.slabs);
-                                else tma_reduce_add_3d(&maps.sum, stage, col + 32 * half, row, 0);
-                                tma_store_commit();
-                            }
-                        }
+                    if (f32_part) {
+                        stage_out_f32(v, col, row, slab, k.N);
+                        continue;
                     }
+                    uint4 w[8];
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        const uint32_t* x = &v[c / 4][c % 4 * 8];
+                        auto two = [&](int e) { return pack_bf16x2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])); };
+                        w[c] = make_uint4(two(0), two(2), two(4), two(6));
+                    }
+                    stage_out(mc, EPI == kEpiPlain && q.partial, col, row, 0, w);
                 }
-                // rows 8i + lane / 4, columns 8j + pair_col
-                uint64_t v[4][8];
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const uint32_t* x = &r[i >> 1][4 * j + 2 * (i & 1)];
-                        v[i][j] = pack_f32x2(__uint_as_float(x[0]), __uint_as_float(x[1]));
-                    }
-                if (with_bias && !f32_part) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const uint32_t lo = __shfl_sync(0xffffffffu, bias.x, 4 * j + (lane & 3));
-                        const uint64_t b = bias_pair(prm, make_uint2(lo, prm.bias_bf16 ? 0u : __shfl_sync(0xffffffffu, bias.y, 4 * j + (lane & 3))));
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) v[i][j] = fadd2(v[i][j], b);
-                    }
+            }
+        } else {
+            const bool has_aux = EPI == kEpiResidual || EPI == kEpiSlope || (EPI == kEpiGelu && prm.has_aux);
+            const int pair_col = 2 * (lane & 3);
+            uint32_t aux_n = 0;
+            auto request_aux = [&](const GemmPart& p, int c0) {      // the step's 32 x 64 tile; one at a time is on its way or being read
+                const int row = p.m0 + static_cast<int>(rank) * TR::CM + row0, col = p.n0 + c0;
+                if (has_aux && p.task == 0 && row < prm.t[0].M && col < prm.t[0].N && lane == 0) {
+                    mbar_arrive_expect_tx(&aux_full[warp], TR::STAGING_BYTES);
+                    tma_load_3d(second, &maps.aux, &aux_full[warp], col, row, 0);
                 }
-                if (last) {
-                    more_ahead = walk.next(ahead);
-                    if (more_ahead) request_bias(ahead, colf);
-                } else {
-                    request_bias(q, c0 + 64);
-                }
-                auto request_next_aux = [&] {                    // once every lane has read the tile that is there
-                    if (!last) request_aux(q, c0 + 64);
-                    else if (more_ahead) request_aux(ahead, colf);
-                };
-                if (!inside || !fused) request_next_aux();
-                if (!inside || f32_part) continue;
-                tile_free();
-                if (!fused) {
+            };
+            uint2 bias = make_uint2(0u, 0u);                         // of columns 2 lane, 2 lane + 1 of a step, handed round by shuffles
+            auto request_bias = [&](const GemmPart& p, int c0) {
+                const int col = p.n0 + c0 + 2 * lane;
+                if (EPI != kEpiSlope && prm.bias && col < prm.t[p.task].N) bias = load_bias2(prm, col);
+            };
+            bool more = walk.next(q);
+            if (more) {
+                request_aux(q, colf);
+                request_bias(q, colf);
+            }
+            for (; more; ++n) {
+                const GemmTask& k = prm.t[q.task];
+                const bool fused = kEpiFused<EPI> && q.task == 0;
+                const uint32_t buf = n & 1;
+                const int row = q.m0 + static_cast<int>(rank) * TR::CM + row0;
+                const bool with_bias = EPI != kEpiSlope && prm.bias;
+                const bool f32_part = EPI == kEpiSlope && q.partial;      // (dW beside it, in fp32; the other forms run whole tiles)
+                mbar_wait(&acc_full[buf], (n >> 1) & 1, ab, 30);
+                tc_fence_after_sync();
+                GemmPart ahead;
+                bool more_ahead = false;
+#pragma unroll 1
+                for (int c0 = colf; c0 < colf + BN / 2; c0 += 64) {
+                    const int col = q.n0 + c0;
+                    const bool inside = row < k.M && col < k.N, last = c0 != colf;
+                    uint32_t r[2][32];
+                    if (f32_part) {
+                        tmem_ld_x32(tmem + buf * BN + c0 + lane_base, r[0]);
+                        tmem_ld_x32(tmem + buf * BN + c0 + 32 + lane_base, r[1]);
+                    } else {
+                        tmem_ld_16x256b_x8(tmem + buf * BN + c0 + lane_base, r[0]);
+                        tmem_ld_16x256b_x8(tmem + buf * BN + c0 + lane_base + (16u << 16), r[1]);
+                    }
+                    tmem_wait_ld();
+                    if (last) release(buf);
+                    if (f32_part && inside) stage_out_f32(r, col, row, 0, k.N);
+                    // rows 8i + lane / 4, columns 8j + pair_col
+                    uint64_t v[4][8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const uint32_t w[4] = {pack_bf16_pair(v[0][j]), pack_bf16_pair(v[1][j]), pack_bf16_pair(v[2][j]), pack_bf16_pair(v[3][j])};
-                        st_matrix_sw128(stage, lane, j, w);
-                    }
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if (q.partial) tma_reduce_add_3d(&maps.sum, stage, col, row, 0);
-                        else tma_store_3d(&maps.c[q.task], stage, col, row, 0);
-                        tma_store_commit();
-                    }
-                    continue;
-                }
-                if constexpr (EPI != kEpiBias) {
-                    uint64_t sum[8];
-                    // One body for each combination: with the choice made element by element no two exponentials overlap (8192 x 1024 x 4096 with GELU
-                    // 53.7 -> 56.2 us, 16384 x 768 x 2304 54 -> 60).
-                    auto form = [&](auto keep_, auto aux_) {
-                        constexpr bool KEEP = decltype(keep_)::value, AUX = decltype(aux_)::value;
-                        uint32_t w[8][4];
+                    for (int i = 0; i < 4; ++i)
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
-                            uint32_t slope[4], a[4];
-                            if (AUX) ld_matrix_sw128(second, lane, j, a);
+                            const uint32_t* x = &r[i >> 1][4 * j + 2 * (i & 1)];
+                            v[i][j] = pack_f32x2(__uint_as_float(x[0]), __uint_as_float(x[1]));
+                        }
+                    if (with_bias) {
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                if (EPI == kEpiGelu) v[i][j] = KEEP ? gelu_with_slope2(v[i][j], slope[i]) : gelu2(v[i][j]);
-                                if (EPI == kEpiSlope) v[i][j] = fmul2(v[i][j], unpack_half2(a[i]));
-                                else if (AUX) v[i][j] = fadd2(v[i][j], unpack_bf16x2(a[i]));
-                                w[j][i] = pack_bf16_pair(v[i][j]);
-                            }
-                            if (EPI == kEpiSlope) sum[j] = fadd2(fadd2(v[0][j], v[1][j]), fadd2(v[2][j], v[3][j]));
-                            if (KEEP) st_matrix_sw128(stage, lane, j, slope);
-                            if (!KEEP || !AUX) st_matrix_sw128(KEEP ? second : stage, lane, j, w[j]);
+                        for (int j = 0; j < 8; ++j) {
+                            const uint32_t lo = __shfl_sync(0xffffffffu, bias.x, 4 * j + (lane & 3));
+                            const uint64_t b = bias_pair(prm, make_uint2(lo, prm.bias_bf16 ? 0u : __shfl_sync(0xffffffffu, bias.y, 4 * j + (lane & 3))));
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) v[i][j] = fadd2(v[i][j], b);
+                        }
+                    }
+                    if (last) {
+                        more_ahead = walk.next(ahead);
+                        if (more_ahead) request_bias(ahead, colf);
+                    } else {
+                        request_bias(q, c0 + 64);
+                    }
+                    auto request_next_aux = [&] {                    // once every lane has read the tile that is there
+                        if (!last) request_aux(q, c0 + 64);
+                        else if (more_ahead) request_aux(ahead, colf);
+                    };
+                    if (!inside || !fused) request_next_aux();
+                    if (!inside || f32_part) continue;
+                    tile_free();
+                    if (!fused) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const uint32_t w[4] = {pack_bf16_pair(v[0][j]), pack_bf16_pair(v[1][j]), pack_bf16_pair(v[2][j]), pack_bf16_pair(v[3][j])};
+                            st_matrix_sw128(stage, lane, j, w);
                         }
                         fence_proxy_async_smem();
                         __syncwarp();
                         if (lane == 0) {
-                            if (KEEP) tma_store_3d(&maps.keep, stage, col, row, 0);
-                            if (!KEEP || !AUX) tma_store_3d(&maps.c[0], KEEP ? second : stage, col, row, 0);
+                            tma_store_3d(&maps.c[q.task], stage, col, row, 0);
                             tma_store_commit();
                         }
-                        if (AUX) request_next_aux();
-                        if (KEEP && AUX) {               // the second tile is the residual's: c goes out of the first one, behind the slope
-                            tile_free();
+                        continue;
+                    }
+                    if constexpr (kEpiFused<EPI>) {
+                        uint64_t sum[8];
+                        // One body for each combination: with the choice made element by element no two exponentials overlap (8192 x 1024 x 4096 with GELU
+                        // 53.7 -> 56.2 us, 16384 x 768 x 2304 54 -> 60).
+                        auto form = [&](auto keep_, auto aux_) {
+                            constexpr bool KEEP = decltype(keep_)::value, AUX = decltype(aux_)::value;
+                            uint32_t w[8][4];
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) st_matrix_sw128(stage, lane, j, w[j]);
+                            for (int j = 0; j < 8; ++j) {
+                                uint32_t slope[4], a[4];
+                                if (AUX) ld_matrix_sw128(second, lane, j, a);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    if (EPI == kEpiGelu) v[i][j] = KEEP ? gelu_with_slope2(v[i][j], slope[i]) : gelu2(v[i][j]);
+                                    if (EPI == kEpiSlope) v[i][j] = fmul2(v[i][j], unpack_half2(a[i]));
+                                    else if (AUX) v[i][j] = fadd2(v[i][j], unpack_bf16x2(a[i]));
+                                    w[j][i] = pack_bf16_pair(v[i][j]);
+                                }
+                                if (EPI == kEpiSlope) sum[j] = fadd2(fadd2(v[0][j], v[1][j]), fadd2(v[2][j], v[3][j]));
+                                if (KEEP) st_matrix_sw128(stage, lane, j, slope);
+                                if (!KEEP || !AUX) st_matrix_sw128(KEEP ? second : stage, lane, j, w[j]);
+                            }
                             fence_proxy_async_smem();
                             __syncwarp();
                             if (lane == 0) {
-                                tma_store_3d(&maps.c[0], stage, col, row, 0);
+                                if (KEEP) tma_store_3d(&maps.keep, stage, col, row, 0);
+                                if (!KEEP || !AUX) tma_store_3d(&maps.c[0], KEEP ? second : stage, col, row, 0);
                                 tma_store_commit();
                             }
-                        }
-                    };
-                    if (has_aux) {
-                        mbar_wait(&aux_full[warp], aux_n & 1, ab, 31);
-                        ++aux_n;
-                    }
-                    constexpr std::true_type yes{};
-                    constexpr std::false_type no{};
-                    if constexpr (EPI != kEpiGelu) form(no, yes);
-                    else if (prm.keep_slope) has_aux ? form(yes, yes) : form(yes, no);
-                    else has_aux ? form(no, yes) : form(no, no);
-                    if (EPI == kEpiSlope && prm.colsum) {
-                        // the eight lanes that share columns add up their rows' sums, each ending with one of the eight pairs (rows past M are zeros)
+                            if (AUX) request_next_aux();
+                            if (KEEP && AUX) {               // the second tile is the residual's: c goes out of the first one, behind the slope
+                                tile_free();
 #pragma unroll
-                        for (int half = 4; half > 0; half >>= 1) {
-                            const bool upper = lane & (4 * half);
-#pragma unroll
-                            for (int j = 0; j < half; ++j) {
-                                const uint64_t send = upper ? sum[j] : sum[j + half], keep = upper ? sum[j + half] : sum[j];
-                                sum[j] = fadd2(keep, __shfl_xor_sync(0xffffffffu, static_cast<unsigned long long>(send), 4 * half));
+                                for (int j = 0; j < 8; ++j) st_matrix_sw128(stage, lane, j, w[j]);
+                                fence_proxy_async_smem();
+                                __syncwarp();
+                                if (lane == 0) {
+                                    tma_store_3d(&maps.c[0], stage, col, row, 0);
+                                    tma_store_commit();
+                                }
                             }
+                        };
+                        if (has_aux) {
+                            mbar_wait(&aux_full[warp], aux_n & 1, ab, 31);
+                            ++aux_n;
                         }
-                        const int at = col + 8 * (lane >> 2) + pair_col;
-                        if (at < k.N) *reinterpret_cast<uint64_t*>(prm.colsum + static_cast<long>(row >> 5) * k.N + at) = sum[0];
+                        constexpr std::true_type yes{};
+                        constexpr std::false_type no{};
+                        if constexpr (EPI != kEpiGelu) form(no, yes);
+                        else if (prm.keep_slope) has_aux ? form(yes, yes) : form(yes, no);
+                        else has_aux ? form(no, yes) : form(no, no);
+                        if (EPI == kEpiSlope && prm.colsum) {
+                            // the eight lanes that share columns add up their rows' sums, each ending with one of the eight pairs (rows past M are zeros)
+#pragma unroll
+                            for (int half = 4; half > 0; half >>= 1) {
+                                const bool upper = lane & (4 * half);
+#pragma unroll
+                                for (int j = 0; j < half; ++j) {
+                                    const uint64_t send = upper ? sum[j] : sum[j + half], keep = upper ? sum[j + half] : sum[j];
+                                    sum[j] = fadd2(keep, __shfl_xor_sync(0xffffffffu, static_cast<unsigned long long>(send), 4 * half));
+                                }
+                            }
+                            const int at = col + 8 * (lane >> 2) + pair_col;
+                            if (at < k.N) *reinterpret_cast<uint64_t*>(prm.colsum + static_cast<long>(row >> 5) * k.N + at) = sum[0];
+                        }
                     }
                 }
+                more = more_ahead;
+                q = ahead;
             }
-            more = more_ahead;
-            q = ahead;
         }
         if (lane == 0) tma_store_wait_read_all();    // the CTA may leave once its shared memory has been read; the writes complete on their own
     }
