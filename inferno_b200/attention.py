@@ -118,8 +118,8 @@ class AttentionBackward:
 
 def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | None = None,
                      math_mode: int = _capi.MATH_SPLIT_BF16, bthd_out: bool = False, total_heads: int | None = None) -> torch.Tensor:
-    """``softmax(mask(q k^T * scale)) v`` with a causal mask; differentiable.  q, k, v: [B,H,T,D] tensors or views.
-    ``total_heads`` as in ``attention_forward``."""
+    """``softmax(mask(q k^T * scale)) v`` with a causal mask; differentiable once (a second derivative raises
+    NotImplementedError).  q, k, v: [B,H,T,D] tensors or views.  ``total_heads`` as in ``attention_forward``."""
     return _capi.host().causal_attention(q, k, v, scale, True, math_mode, bthd_out, total_heads)
 
 
@@ -128,6 +128,6 @@ def causal_attention_packed(qkv: torch.Tensor, num_heads: int, scale: float | No
     """Attention straight on the fused projection output: ``qkv`` is [B, T, 3*C] (= [B,T,3,H,D]); returns [B, T, C].
     Replaces slice / contiguous / reshape / transpose / contiguous before the kernels and transpose / contiguous /
     reshape after them (InfernoApp/main.cpp:716-737, 758-761) with stride arithmetic: no copy kernel runs, and the
-    gradient is written into one [B, T, 3*C] buffer by the kernels themselves.  ``total_heads`` (batch times heads of the
+    gradient is written into one [B, T, 3*C] buffer by the kernels themselves.  Differentiable once, as above.  ``total_heads`` (batch times heads of the
     whole problem) as in ``attention_forward``."""
     return _capi.host().causal_attention_packed(qkv, num_heads, scale, math_mode, total_heads)

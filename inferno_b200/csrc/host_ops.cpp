@@ -321,6 +321,29 @@ void refuse_tangents(std::initializer_list<const Tensor*> ts, const char* op) {
 
 // The backward node of the fused op: saves q, k, v, out and lse; produces dq, dk, dv.  Plays the role a
 // `class AttentionBackward : public Node` has in the reference (src/inferno/gradfn/node.h:23-45).
+// The gradients of the operators below are not differentiable themselves.  Made with create_graph they get this node, so that a second derivative
+// raises; without one it would come out short by their part of it.
+struct NoSecondDerivative : torch::autograd::Node {
+    const char* op;
+    explicit NoSecondDerivative(const char* op_) : op(op_) {}
+    variable_list apply(variable_list&&) override {
+        TORCH_CHECK_NOT_IMPLEMENTED(false, op, ": second derivatives are not implemented");
+    }
+    std::string name() const override { return "NoSecondDerivative"; }
+};
+// `from`: which of the backward node's inputs the gradients depend on, saved there or not; all of them depend on dy.
+void refuse_second_derivative(std::initializer_list<Tensor*> grads, const torch::autograd::Node& backward, std::initializer_list<uint32_t> from, const Tensor& dy,
+                              const char* op) {
+    if (!at::GradMode::is_enabled()) return;
+    torch::autograd::edge_list edges = torch::autograd::collect_next_edges(dy);
+    for (uint32_t i : from) edges.push_back(backward.next_edge(i));
+    if (std::none_of(edges.begin(), edges.end(), [](const torch::autograd::Edge& e) { return e.is_valid(); })) return;
+    auto node = std::shared_ptr<NoSecondDerivative>(new NoSecondDerivative(op), torch::autograd::deleteNode);
+    node->set_next_edges(std::move(edges));
+    for (Tensor* g : grads)
+        if (g->defined()) torch::autograd::set_history(*g, node);
+}
+
 struct AttentionBackward : torch::autograd::Node {
     SavedVariable q, k, v, o, lse;
     double scale = 0;
@@ -345,7 +368,8 @@ struct AttentionBackward : torch::autograd::Node {
             dk = g.select(2, 1).transpose(1, 2);
             dv = g.select(2, 2).transpose(1, 2);
         }
-        const Grads r = attention_backward(tq, tk, tv, to, grads[0], tl, scale, causal, math_mode, dq, dk, dv);
+        Grads r = attention_backward(tq, tk, tv, to, grads[0], tl, scale, causal, math_mode, dq, dk, dv);
+        refuse_second_derivative({&r.dq, &r.dk, &r.dv}, *this, {0, 1, 2}, grads[0], "causal_attention");
         return {r.dq, r.dk, r.dv};
     }
     void release_variables() override {
@@ -411,6 +435,7 @@ struct PackedAttentionBackward : torch::autograd::Node {
         launch_bwd(s, packed_operand(p, 0, C, D), packed_operand(p, 1, C, D), packed_operand(p, 2, C, D), packed_operand(to, 0, C, D),
                    packed_operand(dy, 0, C, D), tl.data_ptr<float>(), packed_operand(g, 0, C, D), packed_operand(g, 1, C, D), packed_operand(g, 2, C, D), scale,
                    true, math_mode, p.device());
+        refuse_second_derivative({&g}, *this, {0}, grads[0], "causal_attention");
         return {g};
     }
     void release_variables() override {
@@ -546,29 +571,6 @@ LinearGrads linear_backward(const Tensor& x, const Tensor& w, const Tensor& dy, 
                                   reinterpret_cast<ib200_stream_t>(stream)),
                  "ib200_linear_bwd_ws");
     return g;
-}
-
-// The gradients of the operators below are not differentiable themselves.  Made with create_graph they get this node, so that a second derivative
-// raises; without one it would come out short by their part of it.
-struct NoSecondDerivative : torch::autograd::Node {
-    const char* op;
-    explicit NoSecondDerivative(const char* op_) : op(op_) {}
-    variable_list apply(variable_list&&) override {
-        TORCH_CHECK_NOT_IMPLEMENTED(false, op, ": second derivatives are not implemented");
-    }
-    std::string name() const override { return "NoSecondDerivative"; }
-};
-// `from`: which of the backward node's inputs the gradients depend on, saved there or not; all of them depend on dy.
-void refuse_second_derivative(std::initializer_list<Tensor*> grads, const torch::autograd::Node& backward, std::initializer_list<uint32_t> from, const Tensor& dy,
-                              const char* op) {
-    if (!at::GradMode::is_enabled()) return;
-    torch::autograd::edge_list edges = torch::autograd::collect_next_edges(dy);
-    for (uint32_t i : from) edges.push_back(backward.next_edge(i));
-    if (std::none_of(edges.begin(), edges.end(), [](const torch::autograd::Edge& e) { return e.is_valid(); })) return;
-    auto node = std::shared_ptr<NoSecondDerivative>(new NoSecondDerivative(op), torch::autograd::deleteNode);
-    node->set_next_edges(std::move(edges));
-    for (Tensor* g : grads)
-        if (g->defined()) torch::autograd::set_history(*g, node);
 }
 
 struct LinearBackward : torch::autograd::Node {

@@ -3,6 +3,7 @@ behind one they depend on the bias as well, also where the bias is all that need
 import pytest
 import torch
 
+from inferno_b200 import attention as A
 from inferno_b200 import linear as L
 
 pytestmark = pytest.mark.gpu
@@ -96,3 +97,24 @@ def test_plain_projection(form):
     gx, = torch.autograd.grad(y, x, dy, create_graph=True)
     with pytest.raises(NotImplementedError, match="second derivatives"):
         (y.float().sum() + (gx.float() ** 2).sum()).backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("form", ["qkv", "slices", "packed"])
+def test_attention(form, dtype):
+    """Gradients of the queries depend on keys and values, and the other way round."""
+    dense = bf16(2, 40, 3 * 128, seed=8).to(dtype).requires_grad_()
+    if form == "packed":
+        leaves, call, shape = (dense,), lambda: A.causal_attention_packed(dense, 2), (2, 40, 128)
+    else:
+        q, k, v = (t.detach().transpose(1, 2) for t in dense.view(2, 40, 3, 2, 64).unbind(2))
+        leaves = tuple((t if form == "slices" else t.contiguous()).requires_grad_() for t in (q, k, v))
+        call, shape = lambda: A.causal_attention(*leaves), (2, 2, 40, 64)
+    dy = bf16(*shape, seed=9).to(dtype).requires_grad_()
+    want = torch.autograd.grad(call(), leaves, dy)
+    assert all(not g.requires_grad for g in want)
+    got = torch.autograd.grad(call(), leaves, dy, create_graph=True)
+    for g, c in zip(got, want):
+        assert float((g.detach().double() - c.double()).norm()) <= 1e-3 * float(c.double().norm())      # (dq is added up in an order that varies)
+        for of in leaves + (dy,):
+            refused([g], of)
