@@ -74,6 +74,8 @@ class Linear(torch.nn.Module):
     """``x @ W + b`` with W stored [in, out] like the reference's Linear; bf16 weight, fp32-accumulated GEMM.
     With an activation ("gelu") or a residual given to forward, these are part of the kernel's epilogue."""
 
+    activation: str | None = None      # (also of a module that was pickled before it could have one)
+
     def __init__(self, in_features: int, out_features: int, bias: bool = True, activation: str | None = None):
         super().__init__()
         self.activation = activation

@@ -60,3 +60,15 @@ def test_module_without_rows_in_every_form():
             assert y.shape == (0, 128)
             y.sum().backward()
             assert all(not p.grad.any() for p in lin.parameters())
+
+
+def test_module_saved_before_it_had_an_activation(built_lib):
+    """A module that was pickled whole has only the attributes of its time."""
+    import pickle
+    lin = L.Linear(32, 64).bfloat16()
+    del lin.__dict__["activation"]
+    lin = pickle.loads(pickle.dumps(lin))
+    x = z(4, 32, device="cpu")
+    for call in (lambda: lin(x), lambda: lin(x, z(4, 64, device="cpu"))):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            call()
