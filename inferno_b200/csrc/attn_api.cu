@@ -806,8 +806,11 @@ struct FusedBwdWorkspace {
 // dw2 = h^T dy; then dx = dz w1^T and dw1 = x^T dz in another.  Workspace: [acc1 | acc2 | dy's column sums | dz's column sums | dz | dx's slabs].
 struct FfWorkspace {
     size_t acc1, acc2, part2, part1, dz, slabs, bytes;
-    FfWorkspace(int M, int C, int H, int parts) {
-        const size_t w = round_up(static_cast<size_t>(C) * H * 4, 256);
+    // The accumulators are needed where a dW may be cut; whether it is depends on what is asked for beside it.  The two weight gradients have the same
+    // number of tiles and of slices.
+    FfWorkspace(int M, int C, int H, int parts, int pairs) {
+        const bool cut = gemm_wants_split_beside(GemmDesc{nullptr, nullptr, nullptr, C, H, M, 1, 1}, pairs);
+        const size_t w = cut ? round_up(static_cast<size_t>(C) * H * 4, 256) : 0;
         acc1 = 0;
         acc2 = w;
         part2 = 2 * w;
@@ -821,7 +824,7 @@ int ff_bwd_core(const void* x, const void* w1, const void* kept, const void* h, 
                 void* dw2, void* db2, int db2_bf16, int M, int C, int H, uint8_t* ws, cudaStream_t stream) {
     const DeviceInfo* dev = device_info();
     const int pairs = (dev ? dev->sms : 148) / 2, parts = dx ? dx_parts(M, C, H, pairs) : 1;
-    const FfWorkspace L(M, C, H, parts);
+    const FfWorkspace L(M, C, H, parts, pairs);
     const bool inner = dx || dw1 || db1;
     void* dz = ws + L.dz;
     const GemmDesc gz{dy, w2, dz, M, H, C, 0, 0}, gw2{h, dy, dw2, H, C, M, 1, 1}, gx{dz, w1, dx, M, C, H, 0, 0}, gw1{x, dz, dw1, C, H, M, 1, 1};
@@ -1239,7 +1242,8 @@ int ib200_fused_linear_bwd(const void* x, const void* w, const void* dy, const v
 size_t ib200_feed_forward_workspace_bytes(int M, int C, int H) {
     if (M <= 0 || C <= 0 || H <= 0) return 0;
     const DeviceInfo* dev = device_info();
-    return FfWorkspace(M, C, H, dx_parts(M, C, H, (dev ? dev->sms : 148) / 2)).bytes;
+    const int pairs = (dev ? dev->sms : 148) / 2;
+    return FfWorkspace(M, C, H, dx_parts(M, C, H, pairs), pairs).bytes;
 }
 
 int ib200_feed_forward_bwd(const void* x, const void* w1, const void* slope, const void* h, const void* w2, const void* dy, void* dx, void* dw1, void* db1,
