@@ -146,7 +146,7 @@ int ib200_linear_bwd_ws(const void* x, const void* w, const void* dy, void* dx, 
 
 /* y[M,N] = act(x[M,K] w[K,N] + bias[N]) + residual[M,N], all but the product in its epilogue.  activation IB200_ACT_GELU is the reference's
  * tanh form, gelu(z) = z / (1 + exp(-2u)) with u = sqrt(2 / pi) (z + 0.044715 z^3).  bias (of type bias_dtype) and residual (bf16, dense) may be
- * NULL.  slope: if not NULL (activation GELU only), gelu'(x w + bias) is kept there for the backward as fp16, [M, N].  K and N multiples of 8, any M, each
+ * NULL.  slope: if not NULL (activation GELU only), gelu'(x w + bias) is kept there for the backward as fp16, [M, N]: off by 2^-11 of itself, or by 2^-25.  K and N multiples of 8, any M, each
  * up to 2^31 - 257 (beyond: IB200_ERR_UNSUPPORTED); bases 16-byte aligned.  The workspace is used by products that are cut along K
  * (ib200_fused_linear_workspace_bytes, 0: none); without one they are not cut.  y and slope must not overlap the operands, y not slope.
  * Replaces Linear::forward, the gelu op and the residual addition behind them (src/inferno/modules/linear.cpp:99-106,
@@ -228,7 +228,7 @@ int ib200_attn_bwd_static(const void* q, const void* k, const void* v, const voi
 int ib200_attn_check(const void* workspace, ib200_stream_t stream, int* device_code);
 
 /* The same check for the calls that have no caller workspace: ib200_attn_bwd_static and the
- * projection entry points (ib200_gemm_bf16, ib200_linear_*) record an expired
+ * projection entry points (ib200_gemm_bf16, ib200_linear_*, ib200_fused_linear_*, ib200_feed_forward_bwd) record an expired
  * wait in the header of the library's built-in buffer on the current device; this reads and clears
  * it after synchronising `stream`.  Same return values as ib200_attn_check.  Replaces the same
  * check_cuda() convention (src/inferno/cuda/cudaops.h:198-210). */

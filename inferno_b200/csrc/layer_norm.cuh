@@ -10,12 +10,16 @@
 // (src/inferno/cuda/cudalayernorm.cu:16-160, 212-400; modules: src/inferno/modules/layernorm.cpp:25-98).
 //
 // Memory-bound: a row is read from global memory once, into the ring, and everything is computed from there, so the variance is the sum of
-// squared differences from the mean and not a difference of two sums.  A row belongs to 32, 64, 128, 256 or 512 threads (LnShape), each of
+// squared differences from the mean and not a difference of two sums.  (bf16 rows that do not begin on 4 bytes, which no asynchronous copy can fetch,
+// have no ring: they are read from global memory in each pass, three times forward and twice backward.)  A row belongs to 32, 64, 128, 256 or 512 threads (LnShape), each of
 // which has up to four 16-byte chunks of it: a row of one warp needs no barrier.  The backward's threads keep their columns from row to row
 // and sum dw and db in registers; a block's sums meet in the workspace, which ln_finish_kernel adds up in a fixed order.  All sums are
 // fp32; the only rounding to fewer bits is that of the results.
 // Measured (us; floor at the measured copy rate): bf16 16384 x 8192 forward 101 (82), backward 126 (123); 16384 x 4096 55 (41), 68 (61); 16384 x 768 10.8 (7.7),
 // 19.8 (11.5); fp32 16384 x 1024 27 (20), 37 (31).  The forward is bound by issue slots (0.75 a cycle), the backward by memory.
+// Further off: narrow rows, where lanes of a row's warp have nothing to do (24 of 32 at 64 bf16 columns) and what is done per row counts, bf16 196608 x 64
+// 44 (7.7), 56 (11.5), 98304 x 128 23 (7.7), 32 (11.5); rows in pieces of 4 bytes, 32768 x 778 39 (15.6), 51 (23.4) next to 28 and 39 for 776 columns;
+// rows of odd bf16 width, 32768 x 777 53 (15.5), 79 (23.3).
 #pragma once
 
 #include <cuda_bf16.h>

@@ -21,7 +21,7 @@
 // MMAs into one of two 256-column TMEM accumulators, and eight warps drain the other accumulator (TMEM -> registers -> +bias ->
 // TMA store), so the epilogue of a tile overlaps the main loop of the next.
 //
-// Measured, us: 8192 x 1024 x 4096 47 (1470 TFLOP/s), with a residual 54, GELU 50, GELU with its slope kept 62; 16384 x 768 x 2304 43, 49, 50, 63.  The operands of a
+// Measured, us: 8192 x 1024 x 4096 47 (1470 TFLOP/s), with a residual 54, GELU 49, GELU with its slope kept 59; 16384 x 768 x 2304 43, 48, 47, 57.  The operands of a
 // pair at the tensor pipe's full rate are 64 bytes per clock and SM, all that an SM takes from L2: what an epilogue reads or writes more is added.
 //
 // One launch runs up to two products ("tasks"), so that dX and dW of a projection share a grid:
@@ -195,7 +195,8 @@ __device__ __forceinline__ uint64_t gelu_gate2(uint64_t z, uint64_t zz) {       
 }
 __device__ __forceinline__ uint64_t gelu2(uint64_t z) { return fmul2(z, gelu_gate2(z, fmul2(z, z))); }
 // The backward needs gelu'(z) = s + z (2u)' s (1 - s) and nothing else of z, and all of it is at hand here, so the slope is what is kept, as
-// fp16: 2^-11 of itself, an eighth of what the gradient loses when it is rounded to bf16.  (With z kept as bf16 the gradients are half as far off
+// fp16: off by 2^-11 of itself, an eighth of what the gradient loses when it is rounded to bf16, or by 2^-25 where it is below 2^-14 in magnitude (z under
+// about -4.4: up to 2 % at z = -5, and 0 under about -5.6, where what reaches the gradient is 2^-25 of dy).  (With z kept as bf16 the gradients are half as far off
 // again as their rounding leaves them, and with z kept in any type their kernels pay for the exponentials once more: 8192 x 4096, dy -> dz
 // 62 us, 127 us for the product that does it in its epilogue.)  Beyond 16 the slope is 0 or 1 to the last bit, so z is limited
 // there, where the formula would meet infinity times zero; a NaN is kept by s.

@@ -25,7 +25,9 @@ def linear_backward(x, w, dy, need_dx=True, need_dw=True, need_db=True):
     """(dx, dw, db) of ``linear_forward``; db is fp32; what is not needed comes back as None.
 
     A dW whose tiles alone would not fill the GPU evenly is cut along the tokens and its parts are added up in fp32 in the order in
-    which they finish: its bits can differ from run to run in the last place.  dx, db and y repeat bit for bit."""
+    which they finish: its bits can differ from run to run in the last place.  db repeats bit for bit, and so do dx beside a dW and
+    y, unless they have few tiles and a contraction of 1024 or more: y is then cut like dW, and a dx that is asked for without dW is
+    cut as well and its parts, at most eight, are rounded to bf16 as they are added (``ib200_linear_bwd_ws``)."""
     return _capi.host().linear_backward(x, w, dy, need_dx, need_dw, need_db)
 
 
@@ -49,7 +51,8 @@ def fused_linear_forward(x, w, bias=None, activation: str | None = None, residua
 def fused_linear_backward(x, w, dy, slope=None, activation: str | None = None, need_dx=True, need_dw=True, need_db=True):
     """(dx, dw, db) of ``fused_linear_forward``; db is fp32; what is not needed comes back as None.  The residual's gradient is dy.
 
-    dw is added up as in ``linear_backward``; dx and db repeat bit for bit."""
+    With an activation dz = dy * slope is rounded to bf16 ahead of the two products, db is summed before that.  dw is added up as in
+    ``linear_backward``; dx and db repeat bit for bit."""
     return _capi.host().fused_linear_backward(x, w, dy, slope, activation, need_dx, need_dw, need_db)
 
 
