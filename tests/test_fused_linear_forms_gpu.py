@@ -1,5 +1,9 @@
 """Forms of the fused projections that their sizes choose, each with its values checked, and the bias gradient of the hidden layer with a bound tight
 enough to miss no block of rows."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 from test_fused_linear_gpu import ONE, check, check_ff, ff_problem, gelu64, problem
@@ -7,6 +11,7 @@ from test_fused_linear_gpu import ONE, check, check_ff, ff_problem, gelu64, prob
 from inferno_b200 import linear as L
 
 pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 # Few rows: blocks of a cluster split K in two from 2048 of it (at most 74 strips of 64 columns), in four from 4096 (at most 37 strips); up to 16 rows and
 # up to 32 have a kernel each.  Depths that leave the last block a shorter share, and widths that end inside a strip.
@@ -54,3 +59,34 @@ def test_bias_gradient_of_the_hidden_layer(M, C, H, bias_type):
     assert g.dtype == bias_type and float((g.double() - want).norm()) <= tol
     lost = float(dz[M // 64 * 32:M // 64 * 32 + 32].sum(0).norm())      # a block of 32 rows in the middle would be noticed
     assert lost > 2 * tol
+
+
+# The kernel that a process meets first may be met in a capture: each of the product's forms in a process of its own.
+FORMS = {"bias": "lambda: L.linear_forward(x, w, b)", "plain": "lambda: L.linear_forward(x, w)", "residual": "lambda: L.fused_linear_forward(x, w, b, None, r)[0]",
+         "gelu": "lambda: L.fused_linear_forward(x, w, b, 'gelu', r, True)[0]", "slabs": "lambda: L.fused_linear_backward(x[:40], w, r[:40])[0]",
+         "cut": "lambda: L.linear_backward(x, w, r)[0]", "few": "lambda: L.fused_linear(x[:5], w, b, 'gelu')", "norm": "lambda: N.layer_norm(x)"}
+
+_FIRST = r"""
+import sys, torch
+from inferno_b200 import linear as L, norm as N
+bf16 = lambda *s: torch.randn(*s, device="cuda").to(torch.bfloat16)
+x, w, b, r = bf16(2000, 512), bf16(512, 4096), bf16(4096), bf16(2000, 4096)
+call = eval(sys.argv[1])
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = call()
+want = call().clone()
+for _ in range(2):
+    out.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and bool(want.any())
+print("the same")
+"""
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_first_call_of_a_process_captured(form):
+    res = subprocess.run([sys.executable, "-c", _FIRST, FORMS[form]], env=dict(os.environ, PYTHONPATH=ROOT), cwd=ROOT, capture_output=True, text=True, timeout=150)
+    assert res.returncode == 0 and "the same" in res.stdout, res.stdout[-500:] + res.stderr[-2000:]
